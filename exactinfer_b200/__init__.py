@@ -13,7 +13,7 @@ import numpy as np
 from . import capi, synth
 from .capi import Config, ElbError, check, lib
 
-__all__ = ["Weight", "Backend", "cuda_available", "matvec", "get_row", "rmsnorm", "split_limbs", "synth", "Config",
+__all__ = ["Weight", "Backend", "Rope", "KvCache", "KvBatch", "beam_select", "beam_select_work", "cuda_available", "matvec", "get_row", "rmsnorm", "split_limbs", "synth", "Config",
            "ElbError"]
 
 
@@ -143,6 +143,128 @@ def split_limbs(x: np.ndarray, nl: int, device: int = 0):
     inv = np.empty(b, dtype=np.float32)
     check(lib().elb_split_limbs(device, capi.fptr(x), b, n, nl, limbs.ctypes.data_as(C.POINTER(C.c_int8)), capi.fptr(inv)))
     return limbs, inv
+
+
+# ---- the paged cache, rotary positions and beam selection (device pointers, stream-ordered: see include/elb.h)
+
+def _ptr(x):
+    """Device address of x: a number, a DeviceBuffer, anything with data_ptr() (a torch tensor, say) or None."""
+    if x is None or isinstance(x, int):
+        return x
+    return x.ptr if isinstance(x, DeviceBuffer) else x.data_ptr()
+
+
+ROPE_HALF, ROPE_INTERLEAVED = 0, 1
+ROPE_PLAIN, ROPE_LINEAR, ROPE_YARN, ROPE_BANDS = range(4)
+KV_F16, KV_PAIR = 1, 2
+
+
+def rope_config(head_dim: int = 128, dim: int | None = None, layout: int = ROPE_HALF, base: float = 1e6, scaling: int = ROPE_PLAIN,
+                factor: float = 1.0, orig_ctx: float = 0.0, beta_fast: float = 32.0, beta_slow: float = 1.0, attn_factor: float = 0.0,
+                low_freq: float = 1.0, high_freq: float = 4.0) -> capi.RopeConfig:
+    return capi.RopeConfig(head_dim, head_dim if dim is None else dim, layout, scaling, base, factor, orig_ctx, beta_fast, beta_slow, attn_factor,
+                           low_freq, high_freq)
+
+
+def rope_frequencies(cfg: capi.RopeConfig):
+    """(f_i, m) of a configuration (elb_rope_frequencies); host arithmetic."""
+    f, m = np.empty(max(cfg.dim // 2, 1), np.float64), C.c_double()
+    check(lib().elb_rope_frequencies(C.byref(cfg), f.ctypes.data_as(C.POINTER(C.c_double)), C.byref(m)))
+    return f, m.value
+
+
+class Rope:
+    """Rotary positions (elb_rope): see rope_config for the arguments."""
+
+    def __init__(self, head_dim: int = 128, device: int = 0, **config):
+        self.config = rope_config(head_dim, **config)
+        self.head_dim, h = head_dim, C.c_void_p()
+        check(lib().elb_rope_create(device, C.byref(self.config), C.byref(h)))
+        self._h = h
+
+    def apply(self, x, pos, y, n: int, heads: int, ldx: int | None = None, ldy: int | None = None, norm=None, eps: float = 0.0, stream: int = 0):
+        """y[n][heads] = x rotated at the positions pos[n] (elb_rope_dev); strides in floats, default the row's width."""
+        w = heads * self.head_dim
+        check(lib().elb_rope_dev(self._h, _ptr(x), w if ldx is None else ldx, _ptr(y), w if ldy is None else ldy, n, heads, _ptr(pos), _ptr(norm), eps,
+                                 stream))
+
+    def close(self):
+        if getattr(self, "_h", None):
+            lib().elb_rope_destroy(self._h)
+            self._h = None
+
+    def __del__(self):
+        self.close()
+
+
+class KvBatch:
+    """New tokens of several sequences (elb_kv_batch): device arrays q_start[n_seq + 1], length[n_seq], table[n_seq][table_ld]."""
+
+    def __init__(self, n_seq: int, n_tok: int, max_q: int, max_len: int, q_start, length, table, table_ld: int):
+        self._keep = (q_start, length, table)
+        self.n_seq, self.n_tok = n_seq, n_tok
+        self._s = capi.KvBatchStruct(n_seq, n_tok, max_q, max_len, _ptr(q_start), _ptr(length), _ptr(table), table_ld)
+        self._as_parameter_ = C.byref(self._s)
+
+
+class KvCache:
+    """A paged cache of keys and values (elb_kv). mem: device memory for the pool (kept alive here), or None."""
+
+    def __init__(self, n_layer: int, n_head_kv: int, page: int, n_pages: int, type: int = KV_F16, mem=None, head_dim: int = 128, device: int = 0):
+        h = C.c_void_p()
+        self._mem, self.head_dim, self.n_head_kv = mem, head_dim, n_head_kv
+        check(lib().elb_kv_create(device, n_layer, n_head_kv, head_dim, page, n_pages, type, _ptr(mem), C.byref(h)))
+        self._h = h
+
+    @staticmethod
+    def bytes(n_layer: int, n_head_kv: int, page: int, n_pages: int, type: int = KV_F16, head_dim: int = 128) -> int:
+        return lib().elb_kv_bytes(n_layer, n_head_kv, head_dim, page, n_pages, type)
+
+    @property
+    def memory(self) -> int:
+        """Device address of the pool."""
+        return lib().elb_kv_memory(self._h)
+
+    def append(self, layer: int, batch: KvBatch, k, v, ldk: int, ldv: int, rope: Rope | None = None, k_norm=None, eps: float = 0.0, q=None,
+               ldq: int = 0, n_head: int = 0, q_norm=None, q_out=None, ldqo: int = 0, stream: int = 0):
+        """Keys and values of the batch's rows into their pages, its queries rotated into q_out (elb_kv_append_dev)."""
+        check(lib().elb_kv_append_dev(self._h, layer, batch._as_parameter_, rope._h if rope else None, _ptr(k), ldk, _ptr(v), ldv, _ptr(k_norm), eps,
+                                      _ptr(q), ldq, n_head, _ptr(q_norm), _ptr(q_out), ldqo, stream))
+
+    def attention_work(self, batch: KvBatch, n_head: int) -> int:
+        """Bytes of working memory that attention() needs for a batch."""
+        return lib().elb_kv_attention_work(self._h, batch._as_parameter_, n_head)
+
+    def attention(self, layer: int, batch: KvBatch, q, out, n_head: int, scale: float, work, work_bytes: int, ldq: int | None = None,
+                  ldo: int | None = None, stream: int = 0):
+        """Attention of the batch's rows over their sequences' pages (elb_kv_attention_dev)."""
+        w = n_head * self.head_dim
+        check(lib().elb_kv_attention_dev(self._h, layer, batch._as_parameter_, _ptr(q), w if ldq is None else ldq, n_head, scale, _ptr(out),
+                                         w if ldo is None else ldo, _ptr(work), work_bytes, stream))
+
+    def reorder(self, n: int, parent, length, table, table_ld: int, spare, length_out, table_out, taken, stream: int = 0):
+        """Row r goes on from row parent[r]: tables and lengths, last pages copied where they are shared (elb_kv_reorder_dev)."""
+        check(lib().elb_kv_reorder_dev(self._h, n, _ptr(parent), _ptr(length), _ptr(table), table_ld, _ptr(spare), _ptr(length_out), _ptr(table_out),
+                                       _ptr(taken), stream))
+
+    def close(self):
+        if getattr(self, "_h", None):
+            lib().elb_kv_destroy(self._h)
+            self._h = self._mem = None
+
+    def __del__(self):
+        self.close()
+
+
+def beam_select_work(n_vocab: int, n_group: int, beams: int, k: int) -> int:
+    return lib().elb_beam_select_work(n_vocab, n_group, beams, k)
+
+
+def beam_select(logits, n_vocab: int, n_group: int, beams: int, scores, k: int, parent, token, score, work, work_bytes: int, ld: int | None = None,
+                allowed=None, allowed_ld: int = 0, device: int = 0, stream: int = 0):
+    """The k best continuations of every group of beams (elb_beam_select_dev): parent[n_group][k], token, score (double)."""
+    check(lib().elb_beam_select_dev(device, _ptr(logits), n_vocab if ld is None else ld, n_vocab, n_group, beams, _ptr(scores), _ptr(allowed),
+                                    allowed_ld, k, _ptr(parent), _ptr(token), _ptr(score), _ptr(work), work_bytes, stream))
 
 
 def spec_config(spec: "synth.Spec", max_batch: int = 0, n_seq: int = 0) -> Config:

@@ -84,6 +84,39 @@ SIGNATURES = {
     "elb_bench_matmul": (C.c_int, [C.POINTER(_vp), C.c_int, _vp, C.c_int64, _vp, C.c_int, C.c_int, _f32p]),
 }
 
+_f64p = C.POINTER(C.c_double)
+
+
+class RopeConfig(C.Structure):
+    """elb_rope_config"""
+    _fields_ = [("head_dim", C.c_int32), ("dim", C.c_int32), ("layout", C.c_int32), ("scaling", C.c_int32)] + [
+        (n, C.c_double) for n in ("base", "factor", "orig_ctx", "beta_fast", "beta_slow", "attn_factor", "low_freq", "high_freq")]
+
+
+class KvBatchStruct(C.Structure):
+    """elb_kv_batch"""
+    _fields_ = [("n_seq", C.c_int32), ("n_tok", C.c_int32), ("max_q", C.c_int32), ("max_len", C.c_int32), ("d_q_start", _vp), ("d_len", _vp),
+                ("d_table", _vp), ("table_ld", C.c_int64)]
+
+
+_i, _l, _kvb = C.c_int, C.c_int64, C.POINTER(KvBatchStruct)
+SIGNATURES |= {
+    "elb_rope_create": (_i, [_i, C.POINTER(RopeConfig), C.POINTER(_vp)]),
+    "elb_rope_destroy": (None, [_vp]),
+    "elb_rope_frequencies": (_i, [C.POINTER(RopeConfig), _f64p, _f64p]),
+    "elb_rope_dev": (_i, [_vp, _vp, _l, _vp, _l, _l, _i, _vp, _vp, C.c_float, _vp]),
+    "elb_kv_bytes": (C.c_size_t, [_i] * 6),
+    "elb_kv_create": (_i, [_i] * 7 + [_vp, C.POINTER(_vp)]),
+    "elb_kv_destroy": (None, [_vp]),
+    "elb_kv_memory": (_vp, [_vp]),
+    "elb_kv_append_dev": (_i, [_vp, _i, _kvb, _vp, _vp, _l, _vp, _l, _vp, C.c_float, _vp, _l, _i, _vp, _vp, _l, _vp]),
+    "elb_kv_attention_work": (C.c_size_t, [_vp, _kvb, _i]),
+    "elb_kv_attention_dev": (_i, [_vp, _i, _kvb, _vp, _l, _i, C.c_float, _vp, _l, _vp, C.c_size_t, _vp]),
+    "elb_kv_reorder_dev": (_i, [_vp, _i, _vp, _vp, _vp, _l, _vp, _vp, _vp, _vp, _vp]),
+    "elb_beam_select_work": (C.c_size_t, [_i] * 4),
+    "elb_beam_select_dev": (_i, [_i, _vp, _l, _i, _i, _i, _vp, _vp, _l, _i, _vp, _vp, _vp, _vp, C.c_size_t, _vp]),
+}
+
 _lib = None
 
 

@@ -7,6 +7,7 @@
 
 #include "common.cuh"
 #include "decode.cuh"
+#include "kv.cuh"
 
 namespace elb {
 static thread_local std::string g_error;
@@ -134,6 +135,11 @@ static Weight* W(elb_weight* w) { return reinterpret_cast<Weight*>(w); }
 static const Weight* W(const elb_weight* w) { return reinterpret_cast<const Weight*>(w); }
 static Model* M(elb_model* m) { return reinterpret_cast<Model*>(m); }
 static const Model* M(const elb_model* m) { return reinterpret_cast<const Model*>(m); }
+static Rope* R(elb_rope* r) { return reinterpret_cast<Rope*>(r); }
+static const Rope* R(const elb_rope* r) { return reinterpret_cast<const Rope*>(r); }
+static Kv* K(elb_kv* k) { return reinterpret_cast<Kv*>(k); }
+static const Kv* K(const elb_kv* k) { return reinterpret_cast<const Kv*>(k); }
+static cudaStream_t S(void* s) { return static_cast<cudaStream_t>(s); }
 
 extern "C" {
 
@@ -517,6 +523,64 @@ int elb_selftest_decode_plan(const int32_t* shape, const int32_t* types, int cta
 int elb_selftest_decode_exchange(elb_model* m, int byte) { return model_fill_exchange(M(m), byte); }
 size_t elb_model_weight_bytes(const elb_model* m) { return model_weight_bytes(M(m)); }
 size_t elb_model_kv_bytes_per_token(const elb_model* m) { return model_kv_bytes_per_token(M(m)); }
+
+// ---------------------------------------------------------------- paged cache, rotary positions, beam selection
+
+int elb_rope_frequencies(const elb_rope_config* cfg, double* freq, double* m) {
+    std::vector<double> f;
+    double scale = 1.0;
+    ELB_TRY(rope_frequencies(cfg, &f, &scale));
+    if (freq) std::copy(f.begin(), f.end(), freq);
+    if (m) *m = scale;
+    return ELB_OK;
+}
+int elb_rope_create(int device, const elb_rope_config* cfg, elb_rope** out) {
+    if (!out) return fail(ELB_ERR_INVALID, "rope_create: null argument");
+    ELB_TRY(elb_rope_frequencies(cfg, nullptr, nullptr));
+    if (elb_device_count() == 0) return fail(ELB_ERR_CUDA, std::string("no usable CUDA device: ") + g_error);
+    Rope* r = nullptr;
+    ELB_TRY(rope_create(device, cfg, &r));
+    *out = reinterpret_cast<elb_rope*>(r);
+    return ELB_OK;
+}
+void elb_rope_destroy(elb_rope* r) { rope_destroy(R(r)); }
+int elb_rope_dev(const elb_rope* r, const float* d_x, int64_t ldx, float* d_y, int64_t ldy, int64_t n, int heads, const int32_t* d_pos,
+                 const float* d_norm, float eps, void* stream) {
+    return rope_launch(R(r), d_x, ldx, d_y, ldy, n, heads, d_pos, d_norm, eps, S(stream));
+}
+size_t elb_kv_bytes(int n_layer, int n_head_kv, int head_dim, int page, int n_pages, int type) {
+    return kv_bytes(n_layer, n_head_kv, head_dim, page, n_pages, type);
+}
+int elb_kv_create(int device, int n_layer, int n_head_kv, int head_dim, int page, int n_pages, int type, void* d_mem, elb_kv** out) {
+    Kv* kv = nullptr;
+    if (!out) return fail(ELB_ERR_INVALID, "kv_create: null argument");
+    ELB_TRY(kv_create(device, n_layer, n_head_kv, head_dim, page, n_pages, type, d_mem, &kv));
+    *out = reinterpret_cast<elb_kv*>(kv);
+    return ELB_OK;
+}
+void elb_kv_destroy(elb_kv* kv) { kv_destroy(K(kv)); }
+void* elb_kv_memory(const elb_kv* kv) { return kv ? K(kv)->mem : nullptr; }
+int elb_kv_append_dev(elb_kv* kv, int layer, const elb_kv_batch* b, const elb_rope* rope, const float* d_k, int64_t ldk, const float* d_v,
+                      int64_t ldv, const float* d_k_norm, float eps, const float* d_q, int64_t ldq, int n_head, const float* d_q_norm,
+                      float* d_q_out, int64_t ldqo, void* stream) {
+    return kv_append_launch(K(kv), layer, b, R(rope), d_k, ldk, d_v, ldv, d_k_norm, eps, d_q, ldq, n_head, d_q_norm, d_q_out, ldqo, S(stream));
+}
+size_t elb_kv_attention_work(const elb_kv* kv, const elb_kv_batch* b, int n_head) { return kv_attention_work(K(kv), b, n_head); }
+int elb_kv_attention_dev(const elb_kv* kv, int layer, const elb_kv_batch* b, const float* d_q, int64_t ldq, int n_head, float scale,
+                         float* d_out, int64_t ldo, void* d_work, size_t work_bytes, void* stream) {
+    return kv_attention_launch(K(kv), layer, b, d_q, ldq, n_head, scale, d_out, ldo, d_work, work_bytes, S(stream));
+}
+int elb_kv_reorder_dev(elb_kv* kv, int n, const int32_t* d_parent, const int32_t* d_len, const int32_t* d_table, int64_t table_ld,
+                       const int32_t* d_spare, int32_t* d_len_out, int32_t* d_table_out, int32_t* d_taken, void* stream) {
+    return kv_reorder_launch(K(kv), n, d_parent, d_len, d_table, table_ld, d_spare, d_len_out, d_table_out, d_taken, S(stream));
+}
+size_t elb_beam_select_work(int n_vocab, int n_group, int beams, int k) { return beam_select_work(n_vocab, n_group, beams, k); }
+int elb_beam_select_dev(int device, const float* d_logits, int64_t ld, int n_vocab, int n_group, int beams, const double* d_scores,
+                        const uint32_t* d_allowed, int64_t allowed_ld, int k, int32_t* d_parent, int32_t* d_token, double* d_score, void* d_work,
+                        size_t work_bytes, void* stream) {
+    return beam_select_launch(device, d_logits, ld, n_vocab, n_group, beams, d_scores, d_allowed, allowed_ld, k, d_parent, d_token, d_score, d_work,
+                              work_bytes, S(stream));
+}
 
 // ---------------------------------------------------------------- microbenchmarks
 

@@ -1,0 +1,354 @@
+// Rotary positions, alone (elb_rope_dev) and on the way into the pages of a cache (elb_kv_append_dev): per head an optional
+// RMSNorm x * (1 / sqrt(mean x^2 + eps)) * w (src/ops.cpp:155-160 of the reference, sum of squares in double), then pair i
+// of the first `dim` values turned by pos * f_i and multiplied by m (src/model.cpp:23-32 with its scaled forms).
+//
+// Bound by memory: every value is read and written once. A block takes a few tokens, computes the cosines and sines that
+// all their heads share once, in double, into shared memory, and streams the heads through registers: a thread takes 8
+// values (a "unit": 4 pairs, or 8 values that are kept), 16-byte loads. Angles are formed in turns, t = pos * (f / 2 pi) and
+// the fraction of t, so that no position needs more than one double-precision product and a sine of at most one turn.
+#include <algorithm>
+#include <cmath>
+#include <new>
+#include <vector>
+
+#include "kv.cuh"
+
+namespace elb {
+
+namespace {
+
+constexpr int RP_THREADS = 256, RP_TOKENS = 4, RP_MAXHALF = 128;
+
+struct RopeArgs {
+    const double* turns;  // [half] or null: no rotation
+    int dim, layout, head_dim;
+    float mscale, eps;
+    // queries: n_head heads of row t at q + t * ldq -> q_out + t * ldqo
+    const float* q;
+    float* q_out;
+    const float* q_norm;
+    int64_t ldq, ldqo;
+    int n_head;
+    // keys and values into pages (HKV = 0: none)
+    const float *k, *v, *k_norm;
+    int64_t ldk, ldv;
+    int HKV, planes;
+    __half* pool;  // this layer
+    int64_t n;
+    const int* pos;  // positions of the rows, or null: from the batch
+    KvRows rows;
+};
+
+// 1 / sqrt(ms) for a mean square in double: an fp32 estimate and one Newton step (2^-44), double division outside fp32's range
+__device__ __forceinline__ float inv_rms(double ms) {
+    if (!(ms > 1e-30 && ms < 1e30)) return float(1.0 / sqrt(ms));
+    const double y = rsqrtf(float(ms));
+    return float(y * (1.5 - 0.5 * ms * y * y));
+}
+
+__device__ __forceinline__ void split_pair(float x, __half& hi, __half& lo) {
+    hi = __float2half_rn(x);
+    lo = __hisinf(hi) ? __float2half_rn(0.f) : __float2half_rn(x - __half2float(hi));
+}
+
+// four values -> the fp16 planes of a pool row (lo plane: `plane` halves behind)
+__device__ __forceinline__ void store4(__half* dst, int planes, int64_t plane, const float* v) {
+    __half hi[4], lo[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) split_pair(v[i], hi[i], lo[i]);
+    *reinterpret_cast<uint2*>(dst) = *reinterpret_cast<const uint2*>(hi);
+    if (planes == 2) *reinterpret_cast<uint2*>(dst + plane) = *reinterpret_cast<const uint2*>(lo);
+}
+
+// What a block knows of one of its tokens
+struct Tok {
+    int pos;      // position
+    int on;       // there is such a row and it belongs to a sequence
+    int64_t row;  // halves from the layer's first to the token's first in its page (kv 0, head 0), or -1: not stored
+};
+
+// Positions and page rows of the block's tokens. Batch: sequence s holds row t when q_start[s] <= t < q_start[s + 1]; all threads
+// look, one finds it (of overlapping ranges the last counts).
+__device__ __forceinline__ void find_tokens(const RopeArgs& a, int64_t t0, int tokens, Tok* tok, int* seq) {
+    const int tid = threadIdx.x;
+    if (a.pos) {
+        if (tid < tokens) tok[tid] = Tok{t0 + tid < a.n ? a.pos[t0 + tid] : 0, t0 + tid < a.n, -1};
+        __syncthreads();
+        return;
+    }
+    if (tid < tokens) seq[tid] = -1;
+    __syncthreads();
+    for (int s = tid; s < a.rows.n_seq; s += RP_THREADS) {
+        const int lo = a.rows.q_start[s], hi = a.rows.q_start[s + 1];
+        for (int i = 0; i < tokens; ++i)
+            if (lo <= t0 + i && t0 + i < hi && t0 + i < a.n) atomicMax(seq + i, s);
+    }
+    __syncthreads();
+    if (tid < tokens) {
+        Tok t{0, 0, -1};
+        if (seq[tid] >= 0) {
+            const KvSeq q = kv_seq(a.rows, seq[tid]);
+            t.pos = q.len - q.nq + int(t0 + tid - q.row0);
+            t.on = t.pos >= 0;
+            const int pg = kv_page(a.rows, seq[tid], t.pos);
+            if (t.on && pg >= 0) t.row = (int64_t(pg) * 2 * a.HKV * a.planes * a.rows.page + (t.pos & (a.rows.page - 1))) * KV_D;
+        }
+        tok[tid] = t;
+    }
+    __syncthreads();
+}
+
+__device__ __forceinline__ void fill_angles(const RopeArgs& a, int tokens, const Tok* tok, float2 (*cs)[RP_MAXHALF]) {
+    const int half = a.dim / 2;
+    for (int i = threadIdx.x; i < tokens * half; i += RP_THREADS) {
+        const int t = i / half, f = i - t * half;
+        const double turn = double(tok[t].pos) * a.turns[f];
+        double sn, c;
+        sincospi(2.0 * (turn - rint(turn)), &sn, &c);
+        cs[t][f] = make_float2(float(c * a.mscale), float(sn * a.mscale));
+    }
+}
+
+// head_dim 32, 64, 128 or 256, dim a multiple of 8, rows on 16-byte boundaries; grid (token groups, head groups)
+__global__ void __launch_bounds__(RP_THREADS) k_rope(const RopeArgs a, int tokens, int heads_per_block) {
+    __shared__ float2 cs[RP_TOKENS][RP_MAXHALF];
+    __shared__ Tok tok[RP_TOKENS];
+    __shared__ int seq[RP_TOKENS];
+    const int64_t t0 = int64_t(blockIdx.x) * tokens;
+    const int heads = a.n_head + 2 * a.HKV, h0 = blockIdx.y * heads_per_block, nh = min(heads_per_block, heads - h0);
+    find_tokens(a, t0, tokens, tok, seq);
+    if (a.turns) fill_angles(a, tokens, tok, cs);
+    __syncthreads();
+    const int upt = a.head_dim / 8, total = tokens * nh * upt, half = a.dim / 2;
+    for (int i0 = 0; i0 < total; i0 += RP_THREADS) {  // (whole warps stay together for the reduction)
+        const int i = i0 + int(threadIdx.x), u = i % upt, hh = i / upt % nh, t = min(i / upt / nh, tokens - 1), h = h0 + hh;
+        const bool is_v = h >= a.n_head + a.HKV, is_k = !is_v && h >= a.n_head;
+        const bool on = i < total && tok[t].on && (!(is_k || is_v) || tok[t].row >= 0);
+        const int kh = h - a.n_head - (is_v ? a.HKV : 0);
+        const bool turn = a.turns && !is_v && 8 * u < a.dim, split = turn && a.layout == ELB_ROPE_HALF;
+        const int e0 = split ? 4 * u : 8 * u, e1 = split ? half + 4 * u : 8 * u + 4;
+        float v[8] = {};
+        if (on) {
+            const float* src = is_v ? a.v + (t0 + t) * a.ldv + kh * KV_D : is_k ? a.k + (t0 + t) * a.ldk + kh * KV_D : a.q + (t0 + t) * a.ldq + int64_t(h) * a.head_dim;
+            *reinterpret_cast<float4*>(v) = __ldcg(reinterpret_cast<const float4*>(src + e0));
+            *reinterpret_cast<float4*>(v + 4) = __ldcg(reinterpret_cast<const float4*>(src + e1));
+        }
+        const float* w = is_v ? nullptr : is_k ? a.k_norm : a.q_norm;
+        if (a.q_norm || a.k_norm) {
+            double ss = 0.0;
+#pragma unroll
+            for (int j = 0; j < 8; ++j) ss += double(v[j]) * double(v[j]);
+            for (int o = upt / 2; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
+            if (w) {
+                const float inv = inv_rms(ss / a.head_dim + double(a.eps));
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    v[j] = __fmul_rn(__fmul_rn(v[j], inv), w[e0 + j]);
+                    v[j + 4] = __fmul_rn(__fmul_rn(v[j + 4], inv), w[e1 + j]);
+                }
+            }
+        }
+        if (turn) {
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                const float2 c = cs[t][4 * u + j];
+                float& x = split ? v[j] : v[2 * j];
+                float& y = split ? v[j + 4] : v[2 * j + 1];
+                const float x0 = x, y0 = y;
+                x = x0 * c.x - y0 * c.y;
+                y = x0 * c.y + y0 * c.x;
+            }
+        }
+        if (!on) continue;
+        if (is_k || is_v) {
+            const int64_t plane = int64_t(a.rows.page) * KV_D;
+            __half* dst = a.pool + tok[t].row + (int64_t(is_v) * a.HKV + kh) * a.planes * plane;
+            store4(dst + e0, a.planes, plane, v);
+            store4(dst + e1, a.planes, plane, v + 4);
+        } else {
+            float* dst = a.q_out + (t0 + t) * a.ldqo + int64_t(h) * a.head_dim;
+            *reinterpret_cast<float4*>(dst + e0) = *reinterpret_cast<const float4*>(v);
+            *reinterpret_cast<float4*>(dst + e1) = *reinterpret_cast<const float4*>(v + 4);
+        }
+    }
+}
+
+// any even head_dim and dim, any alignment: a warp per (row, head), pair by pair
+__global__ void __launch_bounds__(RP_THREADS) k_rope_any(const RopeArgs a) {
+    __shared__ float2 cs[RP_TOKENS][RP_MAXHALF];
+    __shared__ Tok tok[RP_TOKENS];
+    __shared__ int seq[RP_TOKENS];
+    const int64_t t0 = blockIdx.x;
+    find_tokens(a, t0, 1, tok, seq);
+    fill_angles(a, 1, tok, cs);
+    __syncthreads();
+    const int lane = threadIdx.x & 31, half = a.dim / 2;
+    for (int h = int(threadIdx.x) / 32 + 8 * int(blockIdx.y); h < a.n_head; h += 8 * int(gridDim.y)) {
+        const float* x = a.q + t0 * a.ldq + int64_t(h) * a.head_dim;
+        float* y = a.q_out + t0 * a.ldqo + int64_t(h) * a.head_dim;
+        float inv = 1.f;
+        if (a.q_norm) {
+            double ss = 0.0;
+            for (int i = lane; i < a.head_dim; i += 32) ss += double(x[i]) * double(x[i]);
+            inv = inv_rms(warp_sum(ss) / a.head_dim + double(a.eps));
+        }
+        auto get = [&](int i) { return a.q_norm ? __fmul_rn(__fmul_rn(x[i], inv), a.q_norm[i]) : x[i]; };
+        for (int i = lane; i < half; i += 32) {
+            const int i0 = a.layout == ELB_ROPE_HALF ? i : 2 * i, i1 = a.layout == ELB_ROPE_HALF ? i + half : 2 * i + 1;
+            const float2 c = cs[0][i];
+            const float u = get(i0), v = get(i1);
+            y[i0] = u * c.x - v * c.y;
+            y[i1] = u * c.y + v * c.x;
+        }
+        for (int i = a.dim + lane; i < a.head_dim; i += 32) y[i] = get(i);
+    }
+}
+
+bool aligned16(const void* p, int64_t ld) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0 && ld % 4 == 0; }
+
+int rope_run(RopeArgs& a, cudaStream_t s) {
+    // one token per block until there are enough of them to fill the GPU; then four share the block's start-up. Heads are cut
+    // over blocks while the grid is small
+    const int heads = a.n_head + 2 * a.HKV, tokens = a.n >= 2048 ? RP_TOKENS : 1;
+    const int64_t groups = (a.n + tokens - 1) / tokens;
+    int per = heads;
+    while (per > 8 && groups * ((heads + per - 1) / per) < 592) per = (per + 1) / 2;
+    if (groups > 0x7fffffff) return fail(ELB_ERR_UNSUPPORTED, "rope: too many rows");
+    k_rope<<<dim3(unsigned(groups), unsigned((heads + per - 1) / per)), RP_THREADS, 0, s>>>(a, tokens, per);
+    ELB_CUDA(cudaGetLastError());
+    return ELB_OK;
+}
+
+}  // namespace
+
+int rope_frequencies(const elb_rope_config* c, std::vector<double>* freq, double* m) {
+    if (!c) return fail(ELB_ERR_INVALID, "rope: null configuration");
+    if (c->head_dim < 2 || c->head_dim > 256 || c->head_dim % 2 || c->dim < 2 || c->dim > c->head_dim || c->dim % 2)
+        return fail(ELB_ERR_INVALID, "rope: head_dim must be even and at most 256, dim even and at most head_dim");
+    if (c->layout != ELB_ROPE_HALF && c->layout != ELB_ROPE_INTERLEAVED) return fail(ELB_ERR_INVALID, "rope: unknown layout");
+    if (c->scaling < ELB_ROPE_PLAIN || c->scaling > ELB_ROPE_BANDS) return fail(ELB_ERR_INVALID, "rope: unknown scaling");
+    if (!(c->base > 1.0) || !std::isfinite(c->base)) return fail(ELB_ERR_INVALID, "rope: base must be finite and above 1");
+    if (c->scaling != ELB_ROPE_PLAIN && (!(c->factor >= 1.0) || !std::isfinite(c->factor))) return fail(ELB_ERR_INVALID, "rope: factor must be finite and at least 1");
+    const bool yarn = c->scaling == ELB_ROPE_YARN, bands = c->scaling == ELB_ROPE_BANDS;
+    if ((yarn || bands) && (!(c->orig_ctx > 0.0) || !std::isfinite(c->orig_ctx))) return fail(ELB_ERR_INVALID, "rope: orig_ctx must be positive");
+    if (yarn && (!(c->beta_slow > 0.0) || !(c->beta_fast >= c->beta_slow) || !std::isfinite(c->beta_fast) || !(c->attn_factor >= 0.0) || !std::isfinite(c->attn_factor)))
+        return fail(ELB_ERR_INVALID, "rope: beta_fast >= beta_slow > 0 and attn_factor >= 0 are needed");
+    if (bands && (!(c->low_freq > 0.0) || !(c->high_freq > c->low_freq) || !std::isfinite(c->high_freq)))
+        return fail(ELB_ERR_INVALID, "rope: high_freq > low_freq > 0 is needed");
+    const double pi = 3.14159265358979323846, dim = c->dim;
+    double lo = 0.0, hi = 0.0;
+    *m = 1.0;
+    if (yarn) {
+        auto at = [&](double turns) { return dim * std::log(c->orig_ctx / (2.0 * pi * turns)) / (2.0 * std::log(c->base)); };
+        lo = std::max(std::floor(at(c->beta_fast)), 0.0);
+        hi = std::min(std::ceil(at(c->beta_slow)), dim - 1.0);
+        if (lo == hi) hi += 0.001;
+        *m = c->attn_factor > 0.0 ? c->attn_factor : 0.1 * std::log(c->factor) + 1.0;
+    }
+    freq->resize(size_t(c->dim / 2));
+    for (int i = 0; i < c->dim / 2; ++i) {
+        double f = std::pow(c->base, -2.0 * i / dim);
+        if (c->scaling == ELB_ROPE_LINEAR) {
+            f /= c->factor;
+        } else if (yarn) {
+            const double r = std::min(std::max((i - lo) / (hi - lo), 0.0), 1.0);
+            f = f / c->factor * r + f * (1.0 - r);
+        } else if (bands) {
+            const double turns = c->orig_ctx * f / (2.0 * pi);
+            if (turns < c->low_freq) {
+                f /= c->factor;
+            } else if (turns <= c->high_freq) {
+                const double t = (turns - c->low_freq) / (c->high_freq - c->low_freq);
+                f = (1.0 - t) * f / c->factor + t * f;
+            }
+        }
+        (*freq)[size_t(i)] = f;
+    }
+    return ELB_OK;
+}
+
+int rope_create(int device, const elb_rope_config* c, Rope** out) {
+    std::vector<double> freq;
+    double m = 1.0;
+    if (!out) return fail(ELB_ERR_INVALID, "rope_create: null argument");
+    ELB_TRY(rope_frequencies(c, &freq, &m));
+    DeviceScope on(device);
+    if (on.rc != ELB_OK) return on.rc;
+    for (double& f : freq) f /= 2.0 * 3.14159265358979323846;
+    auto* r = new (std::nothrow) Rope;
+    if (!r) return fail(ELB_ERR_MEMORY, "rope_create: out of memory");
+    r->device = device; r->head_dim = c->head_dim; r->dim = c->dim; r->layout = c->layout; r->mscale = float(m);
+    if (device_malloc(&r->d_turns, freq.size() * sizeof(double)) != cudaSuccess) {
+        delete r;
+        return fail(ELB_ERR_MEMORY, "rope_create: out of device memory");
+    }
+    const cudaError_t e = cudaMemcpy(r->d_turns, freq.data(), freq.size() * sizeof(double), cudaMemcpyHostToDevice);
+    if (e != cudaSuccess) {
+        rope_destroy(r);
+        return fail(ELB_ERR_CUDA, std::string("rope_create: ") + cudaGetErrorString(e));
+    }
+    *out = r;
+    return ELB_OK;
+}
+
+void rope_destroy(Rope* r) {
+    if (!r) return;
+    DeviceScope on(r->device);
+    cudaFree(r->d_turns);
+    delete r;
+}
+
+int rope_launch(const Rope* r, const float* x, int64_t ldx, float* y, int64_t ldy, int64_t n, int heads, const int* pos, const float* norm,
+                float eps, cudaStream_t s) {
+    if (!r) return fail(ELB_ERR_INVALID, "rope: null handle");
+    if (n < 0 || heads <= 0 || heads > 65536) return fail(ELB_ERR_INVALID, "rope: bad row or head count");
+    if (n == 0) return ELB_OK;
+    if (!x || !y || !pos) return fail(ELB_ERR_INVALID, "rope: null argument");
+    const int64_t width = int64_t(heads) * r->head_dim;
+    if (ldx < width || ldy < width) return fail(ELB_ERR_INVALID, "rope: a row stride is shorter than the row");
+    if (x == y && ldx != ldy) return fail(ELB_ERR_INVALID, "rope: in place needs equal strides");
+    if (n > 0x7fffffff) return fail(ELB_ERR_UNSUPPORTED, "rope: too many rows");
+    if (norm && !(eps >= 0.f)) return fail(ELB_ERR_INVALID, "rope: eps must not be negative");
+    DeviceScope on(r->device);
+    if (on.rc != ELB_OK) return on.rc;
+    RopeArgs a{};
+    a.turns = r->d_turns; a.dim = r->dim; a.layout = r->layout; a.head_dim = r->head_dim; a.mscale = r->mscale; a.eps = eps;
+    a.q = x; a.q_out = y; a.q_norm = norm; a.ldq = ldx; a.ldqo = ldy; a.n_head = heads; a.n = n; a.pos = pos;
+    const int d = r->head_dim;
+    if ((d == 32 || d == 64 || d == 128 || d == 256) && r->dim % 8 == 0 && aligned16(x, ldx) && aligned16(y, ldy)) return rope_run(a, s);
+    k_rope_any<<<dim3(unsigned(n), unsigned(std::min((heads + 7) / 8, n < 512 ? 8 : 1))), RP_THREADS, 0, s>>>(a);
+    ELB_CUDA(cudaGetLastError());
+    return ELB_OK;
+}
+
+int kv_append_launch(Kv* kv, int layer, const elb_kv_batch* b, const Rope* rope, const float* k, int64_t ldk, const float* v, int64_t ldv,
+                     const float* k_norm, float eps, const float* q, int64_t ldq, int n_head, const float* q_norm, float* q_out, int64_t ldqo,
+                     cudaStream_t s) {
+    ELB_TRY(kv_check_batch(kv, layer, b, "kv_append"));
+    if (!k || !v) return fail(ELB_ERR_INVALID, "kv_append: null argument");
+    const int64_t kd = int64_t(kv->HKV) * KV_D;
+    if (ldk < kd || ldv < kd) return fail(ELB_ERR_INVALID, "kv_append: a row stride is shorter than the row");
+    if (!aligned16(k, ldk) || !aligned16(v, ldv)) return fail(ELB_ERR_UNSUPPORTED, "kv_append: rows must start on 16-byte boundaries");
+    if (q) {
+        if (n_head <= 0 || n_head > 65536 || !q_out) return fail(ELB_ERR_INVALID, "kv_append: queries need their head count and an output");
+        if (ldq < int64_t(n_head) * KV_D || ldqo < int64_t(n_head) * KV_D) return fail(ELB_ERR_INVALID, "kv_append: a row stride is shorter than the row");
+        if (q == q_out && ldq != ldqo) return fail(ELB_ERR_INVALID, "kv_append: in place needs equal strides");
+        if (!aligned16(q, ldq) || !aligned16(q_out, ldqo)) return fail(ELB_ERR_UNSUPPORTED, "kv_append: rows must start on 16-byte boundaries");
+    }
+    if ((k_norm || (q && q_norm)) && !(eps >= 0.f)) return fail(ELB_ERR_INVALID, "kv_append: eps must not be negative");
+    if (rope && (rope->head_dim != KV_D || rope->device != kv->device)) return fail(ELB_ERR_INVALID, "kv_append: the positions are for another head_dim or device");
+    if (rope && rope->dim % 8) return fail(ELB_ERR_UNSUPPORTED, "kv_append: the rotated part of a head must be a multiple of 8");
+    if (b->n_tok == 0 || b->n_seq == 0) return ELB_OK;
+    DeviceScope on(kv->device);
+    if (on.rc != ELB_OK) return on.rc;
+    RopeArgs a{};
+    if (rope) { a.turns = rope->d_turns; a.dim = rope->dim; a.layout = rope->layout; a.mscale = rope->mscale; }
+    a.head_dim = KV_D; a.eps = eps;
+    a.n_head = q ? n_head : 0; a.q = q; a.q_out = q_out; a.q_norm = q ? q_norm : nullptr; a.ldq = ldq; a.ldqo = ldqo;
+    a.k = k; a.v = v; a.k_norm = k_norm; a.ldk = ldk; a.ldv = ldv; a.HKV = kv->HKV; a.planes = kv->planes;
+    a.pool = kv->mem + int64_t(layer) * kv->layer_halves();
+    a.n = b->n_tok; a.rows = kv_rows(kv, b);
+    return rope_run(a, s);
+}
+
+}  // namespace elb

@@ -252,6 +252,112 @@ int elb_model_create_tp(const elb_config* cfg, int n_ctx, int device, int tp_ran
 int elb_model_load_gguf_tp(const char* path, int n_ctx, int device, int max_batch, int n_seq, int tp_rank, int tp_size,
                            const void* id128, elb_model** out);
 
+/* ---- a paged cache of keys and values, for hosts that serve many sequences --------------------------------------
+ * The reference keeps one contiguous fp32 cache for its one sequence (src/model.cpp:153) and evaluates one sequence at a
+ * time; none of these calls has a counterpart there beyond the operators they are made of (RoPE src/model.cpp:23-32, head
+ * norms :178-184, attention :191-214, the sampler's log-sum-exp src/main.cpp:309-320).
+ *
+ * The calls named *_dev of this section are stream-ordered: they enqueue on `stream` (a cudaStream_t of the handle's
+ * device; NULL: the legacy default stream) and return. They allocate nothing, keep nothing between calls and may be
+ * captured into a CUDA graph; lengths and tables are read from device memory when the kernels run. All d_* pointers are
+ * memory of the handle's device, and the caller's current device stays as it is. Calls that may overlap need work buffers
+ * of their own. Errors that only the device can see (a page number outside the pool, lengths longer than a table) touch no
+ * memory outside the given buffers: such a page is not written, and reads as zeros. */
+
+/* Rotary positions (rope of the reference, src/model.cpp:23-32, with what other checkpoints and longer contexts need). The
+ * first `dim` values of a head are rotated in pairs, pair i by the angle pos * f_i in double precision, and multiplied
+ * by a factor m; the others are kept.
+ *   layout   ELB_ROPE_HALF: pair i is (i, i + dim/2), as Qwen3; ELB_ROPE_INTERLEAVED: (2i, 2i + 1)
+ *   scaling  ELB_ROPE_PLAIN   f_i = base^(-2i/dim), m = 1
+ *            ELB_ROPE_LINEAR  f_i / factor
+ *            ELB_ROPE_YARN    f_i (1 - r_i) + f_i / factor * r_i, r_i = clamp((i - lo) / (hi - lo), 0, 1) with
+ *                             lo = max(floor(c(beta_fast)), 0), hi = min(ceil(c(beta_slow)), dim - 1) (hi + 0.001 when equal),
+ *                             c(b) = dim ln(orig_ctx / (2 pi b)) / (2 ln base); m = attn_factor, or 0.1 ln(factor) + 1 when that is 0
+ *            ELB_ROPE_BANDS   by full turns w = orig_ctx f_i / (2 pi): f_i / factor below low_freq, f_i above high_freq, and
+ *                             f_i ((1 - s) / factor + s), s = (w - low_freq) / (high_freq - low_freq), between
+ * head_dim: 2..256, even; dim: 2..head_dim, even. */
+enum { ELB_ROPE_HALF = 0, ELB_ROPE_INTERLEAVED = 1 };
+enum { ELB_ROPE_PLAIN = 0, ELB_ROPE_LINEAR = 1, ELB_ROPE_YARN = 2, ELB_ROPE_BANDS = 3 };
+typedef struct {
+    int32_t head_dim, dim, layout, scaling;
+    double base, factor, orig_ctx, beta_fast, beta_slow, attn_factor, low_freq, high_freq;
+} elb_rope_config;
+typedef struct elb_rope elb_rope;
+int elb_rope_create(int device, const elb_rope_config* cfg, elb_rope** out);
+void elb_rope_destroy(elb_rope* r); /* waits for the device */
+/* f_0 .. f_(dim/2 - 1) and m of a configuration: host arithmetic, needs no GPU. */
+int elb_rope_frequencies(const elb_rope_config* cfg, double* freq, double* m);
+/* Rows of `heads` heads: y[row][head] = rotation of x[row][head] at position d_pos[row] (any int32), after the per-head
+ * RMSNorm with weights d_norm[head_dim] when that is not NULL (sum of squares in double). Row strides in floats, at least
+ * heads * head_dim; y may be x with the same stride, and must not overlap it otherwise. n = 0: nothing is done. */
+int elb_rope_dev(const elb_rope* r, const float* d_x, int64_t ldx, float* d_y, int64_t ldy, int64_t n, int heads,
+                 const int32_t* d_pos, const float* d_norm, float eps, void* stream);
+
+/* The cache. A pool of n_pages pages of `page` positions (16, 32, 64, 128 or 256) for n_layer layers; head_dim must be 128. A
+ * value is held as fp16 (ELB_KV_F16), or as two fp16 numbers hi = fp16(x), lo = fp16(x - hi) whose sum has 22
+ * significant bits (ELB_KV_PAIR: an absolute error of 2^-25 at most below 2^-2). Beyond fp16's range (65 504) both hold an
+ * infinity. Layout: [n_layer][n_pages][2: keys, values][n_head_kv][planes][page][128] fp16, planes = type (1, or hi then lo).
+ * d_mem: the pool's memory (elb_kv_bytes of it, 128-byte aligned, owned by the caller), or NULL: the library allocates it,
+ * zeroed. Which page belongs to which sequence is the caller's table. */
+enum { ELB_KV_F16 = 1, ELB_KV_PAIR = 2 };
+typedef struct elb_kv elb_kv;
+size_t elb_kv_bytes(int n_layer, int n_head_kv, int head_dim, int page, int n_pages, int type); /* 0: bad argument */
+int elb_kv_create(int device, int n_layer, int n_head_kv, int head_dim, int page, int n_pages, int type, void* d_mem, elb_kv** out);
+void elb_kv_destroy(elb_kv* kv); /* waits for the device */
+void* elb_kv_memory(const elb_kv* kv);
+
+/* New tokens of several sequences, in device memory. Rows d_q_start[s] .. d_q_start[s + 1] - 1 are the newest tokens of
+ * sequence s, which then has d_len[s] positions (the new ones included): its i-th new row is at position
+ * d_len[s] - (number of its rows) + i. Position p lies in page d_table[s * table_ld + p / page] at p % page. Rows outside every
+ * range, and rows at negative positions (more rows than positions), belong to nothing. n_tok: rows of the buffers. max_q and
+ * max_len: the most rows and positions of one sequence that the caller expects; they choose kernels, results do not depend
+ * on them being right. */
+typedef struct {
+    int32_t n_seq, n_tok, max_q, max_len;
+    const int32_t *d_q_start, *d_len, *d_table; /* [n_seq + 1], [n_seq], [n_seq][table_ld] */
+    int64_t table_ld;
+} elb_kv_batch;
+
+/* Keys and values of the new tokens into their pages of one layer: k = rotation(norm(k)), v as it is; with d_q also
+ * q_out = rotation(norm(q)) for n_head query heads (q_out may be q with the same stride). rope NULL: no rotation. d_k_norm,
+ * d_q_norm: [128] weights of the per-head RMSNorm or NULL. Row strides in floats; every row starts on a 16-byte boundary.
+ * Rows that belong to nothing are left as they are, and so is their q_out. Two rows must not share a position. */
+int elb_kv_append_dev(elb_kv* kv, int layer, const elb_kv_batch* b, const elb_rope* rope, const float* d_k, int64_t ldk, const float* d_v,
+                      int64_t ldv, const float* d_k_norm, float eps, const float* d_q, int64_t ldq, int n_head, const float* d_q_norm,
+                      float* d_q_out, int64_t ldqo, void* stream);
+
+/* Attention of the new tokens over the pages: head h of the row at position p attends to positions 0..p of its sequence, with
+ * key head h / (n_head / n_head_kv): out = sum_j softmax_j(scale q.k_j) v_j. Every row's queries are used as given (append's
+ * q_out). A row at a negative position has no keys: its output is 0. Rows outside every range are left as they are.
+ * What lies in a page behind a sequence's length has no influence, infinities and NaN included; nor has a key or value that
+ * a row does not attend to. n_head: a multiple of n_head_kv, at most 64 times it. Row strides in floats, rows on 16-byte
+ * boundaries. d_work: elb_kv_attention_work bytes, 256-byte aligned; what it holds before and after does not matter. */
+size_t elb_kv_attention_work(const elb_kv* kv, const elb_kv_batch* b, int n_head); /* 0: bad argument */
+int elb_kv_attention_dev(const elb_kv* kv, int layer, const elb_kv_batch* b, const float* d_q, int64_t ldq, int n_head, float scale,
+                         float* d_out, int64_t ldo, void* d_work, size_t work_bytes, void* stream);
+
+/* States of a beam search (or sequences forked from a shared prefix): row r goes on from row d_parent[r], which has
+ * d_len[d_parent[r]] positions. d_table_out[r] receives the parent's pages that hold them and -1 behind, d_len_out[r] the
+ * length. Full pages are shared. A last page that is not full belongs to the parent's first child (the lowest r); for
+ * every other child its content is copied, in every layer, into the page d_spare[r], which takes its place, and d_taken[r]
+ * is 1 (0 otherwise). A parent outside [0, n): an empty row, length 0. The spare pages must be in no table. The output
+ * arrays must not overlap the inputs. n <= 4096. */
+int elb_kv_reorder_dev(elb_kv* kv, int n, const int32_t* d_parent, const int32_t* d_len, const int32_t* d_table, int64_t table_ld,
+                       const int32_t* d_spare, int32_t* d_len_out, int32_t* d_table_out, int32_t* d_taken, void* stream);
+
+/* Beam search's selection: n_group groups of `beams` rows of logits (row stride ld floats). The score of token t behind row
+ * b is d_scores[b] + (logit - log-sum-exp of the row over the whole vocabulary), in double precision; of the beams * n_vocab
+ * candidates of a group the k best (1 <= k <= 64) come back, best first: the row they continue (counted over all groups), the token,
+ * the score. Equal scores: the lower row first; within a row the larger logit, then the lower token. d_allowed, when not NULL: bit t
+ * of row b's words d_allowed[b * allowed_ld + t / 32] says whether t may be picked (allowed_ld 0: one mask for all rows). Not
+ * candidates: logits of -infinity or NaN, rows whose score or log-sum-exp is not finite (a beam that does not exist has score
+ * -infinity). Where candidates run out, row and token are -1 and the score is -infinity. beams <= 64. d_work:
+ * elb_beam_select_work bytes, 256-byte aligned. */
+size_t elb_beam_select_work(int n_vocab, int n_group, int beams, int k); /* 0: bad argument */
+int elb_beam_select_dev(int device, const float* d_logits, int64_t ld, int n_vocab, int n_group, int beams, const double* d_scores,
+                        const uint32_t* d_allowed, int64_t allowed_ld, int k, int32_t* d_parent, int32_t* d_token, double* d_score, void* d_work,
+                        size_t work_bytes, void* stream);
+
 /* ---- timing helpers for microbenchmarks: run the device-pointer matvec `iters` times over `n_w` weights in
  * rotation (so that the working set exceeds L2) and return the average device time per call in ms. */
 int elb_bench_matvec(elb_weight* const* ws, int n_w, const float* d_x, float* d_y, int nl, int iters, float* avg_ms);
