@@ -1,0 +1,70 @@
+// Attention over a paged cache: what its two kernels and the joining of their partial results share.
+#pragma once
+
+#include "kv.cuh"
+
+namespace elb {
+
+struct KvAttnArgs {
+    KvRows rows;
+    const __half* pool;  // this layer
+    const float* q;
+    float* out;
+    int64_t ldq, ldo;
+    int H, HKV, group, planes;
+    float scale2;        // scale * log2(e): weights are powers of two
+    // the cut: tiles of R query rows (row r of a sequence and key head: token r / group, head r % group), their keys in `splits`
+    // ranges of `chunk` (the last takes what is left). Tiles from tiles_max on are not cut.
+    int splits, chunk, tiles_max;
+    float* part;         // [sequence][tile][key head][split]: R rows of 128 sums, then R maxima, then R denominators
+};
+
+constexpr float KA_P = 14.f;  // weights are formed as 2^(x - m + 14): small ones keep their bits in fp16
+
+// what is visible: positions 0 .. kv_visible - 1 to token t of a sequence (as far as the table goes)
+__device__ __forceinline__ int kv_visible(const KvRows& b, const KvSeq& s, int t) {
+    const int64_t cap = b.table_ld << b.page_log;
+    return int(min(int64_t(max(s.len - s.nq + t + 1, 0)), cap));
+}
+
+__device__ __forceinline__ float ex2(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+
+// (x, y) -> two packed fp16 and what they leave, packed; a remainder of an infinity is 0
+__device__ __forceinline__ void half_pair(float x, float y, uint32_t& hi, uint32_t& lo) {
+    const __half2 h = __floats2half2_rn(x, y);
+    const float2 f = __half22float2(h);
+    const __half2 l = __floats2half2_rn(isinf(f.x) ? 0.f : x - f.x, isinf(f.y) ? 0.f : y - f.y);
+    hi = *reinterpret_cast<const uint32_t*>(&h);
+    lo = *reinterpret_cast<const uint32_t*>(&l);
+}
+// the same for finite values
+__device__ __forceinline__ void half_pair_finite(float x, float y, uint32_t& hi, uint32_t& lo) {
+    const __half2 h = __floats2half2_rn(x, y);
+    const float2 f = __half22float2(h);
+    const __half2 l = __floats2half2_rn(x - f.x, y - f.y);
+    hi = *reinterpret_cast<const uint32_t*>(&h);
+    lo = *reinterpret_cast<const uint32_t*>(&l);
+}
+
+// Power of two that brings a row of queries with largest magnitude m into [2^14, 2^15), and what undoes it in the scale
+struct RowScale {
+    Pow2 up;
+    float f;  // scale2 * 2^-k
+};
+__device__ __forceinline__ RowScale row_scale(float m, float scale2) {
+    const int e = int((__float_as_uint(m) >> 23) & 255u);
+    const int k = m > 0.f && e < 255 ? 14 - (max(e, 1) - 127) : 0;
+    RowScale r{make_pow2(k), 0.f};
+    const Pow2 down = make_pow2(-k);
+    r.f = scale2 * down.s1 * down.s2;
+    return r;
+}
+
+int kv_attn_few_launch(const Kv* kv, KvAttnArgs a, const elb_kv_batch* b, cudaStream_t s);
+size_t kv_attn_few_work(const Kv* kv, const elb_kv_batch* b, int n_head);
+
+}  // namespace elb
