@@ -9,9 +9,14 @@
 
 namespace elb {
 
+// Up to 16 query rows per key head go to the narrow kernel, more to the 128-row tiles
+static bool few_rows(const Kv* kv, const elb_kv_batch* b, int n_head) {
+    return int64_t(std::min(b->max_q, b->n_tok)) * (n_head / kv->HKV) <= 16;
+}
+
 size_t kv_attention_work(const Kv* kv, const elb_kv_batch* b, int n_head) {
     if (!kv || !b || n_head <= 0 || n_head % kv->HKV) return 0;
-    return std::max<size_t>(256, kv_attn_few_work(kv, b, n_head));
+    return std::max<size_t>(256, few_rows(kv, b, n_head) ? kv_attn_few_work(kv, b, n_head) : kv_attn_tile_work(kv, b, n_head));
 }
 
 int kv_attention_launch(const Kv* kv, int layer, const elb_kv_batch* b, const float* q, int64_t ldq, int n_head, float scale, float* out,
@@ -36,7 +41,7 @@ int kv_attention_launch(const Kv* kv, int layer, const elb_kv_batch* b, const fl
     a.H = n_head; a.HKV = kv->HKV; a.group = n_head / kv->HKV; a.planes = kv->planes;
     a.scale2 = scale * 1.44269504088896340736f;
     a.part = static_cast<float*>(work);
-    return kv_attn_few_launch(kv, a, b, s);
+    return few_rows(kv, b, n_head) ? kv_attn_few_launch(kv, a, b, s) : kv_attn_tile_launch(kv, layer, a, b, s);
 }
 
 }  // namespace elb

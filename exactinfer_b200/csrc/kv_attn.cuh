@@ -66,5 +66,10 @@ __device__ __forceinline__ RowScale row_scale(float m, float scale2) {
 
 int kv_attn_few_launch(const Kv* kv, KvAttnArgs a, const elb_kv_batch* b, cudaStream_t s);
 size_t kv_attn_few_work(const Kv* kv, const elb_kv_batch* b, int n_head);
+// rows whose keys were cut: `tiles` tiles of `rows` (8, 16 or 128) query rows
+int kv_attn_join(const KvAttnArgs& a, int rows, int64_t tiles, cudaStream_t s);
+int kv_attn_tile_launch(const Kv* kv, int layer, KvAttnArgs a, const elb_kv_batch* b, cudaStream_t s);
+size_t kv_attn_tile_work(const Kv* kv, const elb_kv_batch* b, int n_head);
+int kv_attn_tile_check();
 
 }  // namespace elb

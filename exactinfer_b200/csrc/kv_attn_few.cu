@@ -365,14 +365,19 @@ template <int PL, int NT> int few_run(const KvAttnArgs& a, int64_t blocks, cudaS
     ELB_TRY(ensure_dyn_smem(reinterpret_cast<const void*>(kernel), S::SMEM));
     kernel<<<unsigned(blocks * a.splits), KF_THREADS, S::SMEM, s>>>(a);
     ELB_CUDA(cudaGetLastError());
-    if (a.splits > 1) {
-        k_kv_attn_join<S::ROWS><<<unsigned((blocks * S::ROWS + 7) / 8), 256, 0, s>>>(a);
-        ELB_CUDA(cudaGetLastError());
-    }
-    return ELB_OK;
+    return a.splits > 1 ? kv_attn_join(a, S::ROWS, blocks, s) : ELB_OK;
 }
 
 }  // namespace
+
+int kv_attn_join(const KvAttnArgs& a, int rows, int64_t tiles, cudaStream_t s) {
+    const unsigned blocks = unsigned((tiles * rows + 7) / 8);
+    if (rows == 8) k_kv_attn_join<8><<<blocks, 256, 0, s>>>(a);
+    else if (rows == 16) k_kv_attn_join<16><<<blocks, 256, 0, s>>>(a);
+    else k_kv_attn_join<128><<<blocks, 256, 0, s>>>(a);
+    ELB_CUDA(cudaGetLastError());
+    return ELB_OK;
+}
 
 size_t kv_attn_few_work(const Kv* kv, const elb_kv_batch* b, int n_head) {
     const FewPlan p = few_plan(kv, b, n_head);

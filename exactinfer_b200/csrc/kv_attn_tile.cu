@@ -1,0 +1,566 @@
+// Attention over a paged cache for many query rows per key head (prompts, chunks of a prompt, turns of a conversation), on the
+// 5th-generation tensor cores.
+//
+// A CTA takes 128 query rows of one sequence and key head (tokens x the query heads that share the key head) and walks the keys
+// that they see, 64 at a time: S = Q K^T, weights 2^(scale2 S - m + 14), O += P V. fp32 accuracy from fp16 operands as in
+// kv_attn_few.cu: a query row is scaled by a power of two and held as hi + lo (22 bits), the weights as well, keys and
+// values are one fp16 or a pair as the cache holds them; lo lo is left out, so that a product costs 2 MMAs (F16 cache) or 3 (pairs).
+// The tensor core adds with truncation: the small products of a step go first, hi hi (8 links for S, 4 for O) last, and
+// a step's O starts from zero and joins the running sum in registers, in fp32 with rounding, behind the factor
+// 2^(m_old - m_new) - tensor memory never needs rescaling.
+//
+// Two teams of four warps work on alternate key tiles, a thread per query row (= TMEM lane), each with its own running
+// maximum, denominator and 128 sums, joined once at the end: while one team forms its weights, the tensor core
+// multiplies for the other. One warp brings keys and values by TMA, page by page, into a ring of 64-key tiles in the
+// order of their use; one thread issues the MMAs. TMEM: Q hi | lo (128 columns, the A operand of S: read from there, the
+// shared memory has only K to deliver), per team S (64 columns, overwritten by the weights hi | lo, the A operand of O) and
+// O (128). V lies [key][dimension] as in the page and is a B operand with N along the rows.
+// A tile's 64 keys take 1024 (F16) or 1536 (pairs) clocks of the tensor pipe.
+//
+// Behind the last visible key the weights are 0, but 0 * NaN is not: the PV product stops at the last 16 keys, and the rows of
+// V behind the last key are emptied in shared memory. In the few tiles that only some rows see, V is searched for infinities and
+// NaN; where there are any, the tile's product is done by the threads, key by key, for the rows that see it.
+#include <algorithm>
+
+#include "kv_attn.cuh"
+
+namespace elb {
+
+namespace {
+
+constexpr int KT_ROWS = 128, KT_KEYS = 64, KT_THREADS = 384, KT_MAXEDGE = 4;
+constexpr unsigned KT_SPIN = 1u << 24;
+constexpr int KT_LD = KV_D + 4;  // floats per row when the teams meet
+
+template <int PL> struct TileShape {
+    static constexpr int HALF = KT_KEYS * 128;           // 64 rows of 64 values
+    static constexpr int PLANE = 2 * HALF;               // 64 keys of one plane
+    static constexpr int SLOT = PL * PLANE;              // keys or values of a tile
+    static constexpr int SLOTS = 12 / PL;
+    static constexpr int RING = SLOTS * SLOT;
+    static constexpr int SMEM = RING + 4096 + 1024;
+    static_assert(RING >= KT_ROWS * KT_LD * 4, "the teams' sums take the place of the ring");
+};
+
+struct TileBars {
+    uint64_t full[12], empty[12], s_full[2], p_full[2], o_full[2], q_full, edge[KT_MAXEDGE];
+    uint32_t tmem;
+    int odd[KT_MAXEDGE];  // edge tile k has infinities or NaN among its values
+    int fail;
+};
+
+__device__ __forceinline__ uint32_t su32(const void* p) { return uint32_t(__cvta_generic_to_shared(p)); }
+__device__ __forceinline__ void bar_init(uint64_t* b, int count) { asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(su32(b)), "r"(count) : "memory"); }
+__device__ __forceinline__ void bar_inval(uint64_t* b) { asm volatile("mbarrier.inval.shared::cta.b64 [%0];" ::"r"(su32(b)) : "memory"); }
+__device__ __forceinline__ void bar_expect(uint64_t* b, uint32_t bytes) {
+    asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(su32(b)), "r"(bytes) : "memory");
+}
+__device__ __forceinline__ void bar_arrive(uint64_t* b) { asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(su32(b)) : "memory"); }
+__device__ __forceinline__ bool bar_try(uint64_t* b, uint32_t parity) {
+    uint32_t done;
+    asm volatile("{\n .reg .pred p;\n mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n selp.u32 %0, 1, 0, p;\n}\n"
+                 : "=r"(done) : "r"(su32(b)), "r"(parity) : "memory");
+    return done != 0;
+}
+// bounded: false when it ran out, or when another warp's wait has
+__device__ __forceinline__ bool bar_wait(uint64_t* b, uint32_t parity, TileBars* bars) {
+    for (unsigned it = 0; it < KT_SPIN; ++it) {
+        if (bar_try(b, parity)) return true;
+        if ((it & 1023u) == 1023u && *reinterpret_cast<volatile int*>(&bars->fail)) return false;
+    }
+    *reinterpret_cast<volatile int*>(&bars->fail) = 1;
+    return false;
+}
+__device__ __forceinline__ bool warp_wait(uint64_t* b, uint32_t parity, TileBars* bars) {  // the same answer in every lane
+    return __all_sync(0xffffffffu, bar_wait(b, parity, bars));
+}
+__device__ __forceinline__ void tma_rows(uint32_t dst, const CUtensorMap* map, int x, int y, uint64_t* bar) {
+    asm volatile("cp.async.bulk.tensor.2d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];"
+                 ::"r"(dst), "l"(map), "r"(x), "r"(y), "r"(su32(bar)) : "memory");
+}
+__device__ __forceinline__ void before_sync() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
+__device__ __forceinline__ void after_sync() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
+// D (+)= A B, A in tensor memory, B in shared memory
+__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, bool add) {
+    asm volatile("{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n}\n"
+                 ::"r"(d), "r"(a), "l"(b), "r"(idesc), "r"(uint32_t(add)) : "memory");
+}
+__device__ __forceinline__ void commit(uint64_t* bar) {
+    asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(su32(bar)) : "memory");
+}
+#define KT_R8(r, o) "=r"(r[o]), "=r"(r[o + 1]), "=r"(r[o + 2]), "=r"(r[o + 3]), "=r"(r[o + 4]), "=r"(r[o + 5]), "=r"(r[o + 6]), "=r"(r[o + 7])
+#define KT_I8(r, o) "r"(r[o]), "r"(r[o + 1]), "r"(r[o + 2]), "r"(r[o + 3]), "r"(r[o + 4]), "r"(r[o + 5]), "r"(r[o + 6]), "r"(r[o + 7])
+__device__ __forceinline__ void tm_ld32(uint32_t a, uint32_t (&r)[32]) {
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,%22,"
+        "%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
+        : KT_R8(r, 0), KT_R8(r, 8), KT_R8(r, 16), KT_R8(r, 24) : "r"(a) : "memory");
+}
+__device__ __forceinline__ uint32_t tm_ld1(uint32_t a) {
+    uint32_t r;
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x1.b32 {%0}, [%1];" : "=r"(r) : "r"(a) : "memory");
+    asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+    return r;
+}
+__device__ __forceinline__ void tm_wait_ld() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
+__device__ __forceinline__ void tm_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+__device__ __forceinline__ void tm_st32(uint32_t a, const uint32_t (&r)[32]) {
+    asm volatile(
+        "tcgen05.st.sync.aligned.32x32b.x32.b32 [%32], {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,%22,"
+        "%23,%24,%25,%26,%27,%28,%29,%30,%31};"
+        ::KT_I8(r, 0), KT_I8(r, 8), KT_I8(r, 16), KT_I8(r, 24), "r"(a) : "memory");
+}
+// Shared-memory operands with 128-byte swizzle. Keys: 64 rows (N) of 64 values (K) in a row, 8-row groups 1024 bytes apart.
+// Values: rows are K (keys), 8-row groups 1024 bytes apart, 64 of the N = 128 dimensions in a row, the others `HALF` bytes behind.
+__device__ __forceinline__ uint64_t desc_rows(uint32_t a) {
+    return uint64_t((a & 0x3FFFF) >> 4) | uint64_t(1024 >> 4) << 32 | uint64_t(1) << 46 | uint64_t(2) << 61;
+}
+__device__ __forceinline__ uint64_t desc_cols(uint32_t a, uint32_t far) { return desc_rows(a) | uint64_t(far >> 4) << 16; }
+// fp16 x fp16 -> fp32, M = 128 from tensor memory, N columns; B with N along the rows when `cols`
+__host__ __device__ constexpr uint32_t idesc_f16(int n, bool cols) {
+    return (1u << 4) | (cols ? 1u << 16 : 0u) | (uint32_t(n >> 3) << 17) | (uint32_t(KT_ROWS >> 4) << 24);
+}
+
+// What a CTA works on
+struct TileJob {
+    int s, j, i, c, kb, ke, vis, vis_min, tiles, edge0;
+    KvSeq sq;
+    bool cut;
+};
+
+template <int PL>
+__global__ void __launch_bounds__(KT_THREADS, 1) k_kv_attn_tile(const __grid_constant__ CUtensorMap map, const KvAttnArgs a, int row0,
+                                                                int rows_total, int* err) {
+    using S = TileShape<PL>;
+    extern __shared__ uint8_t tile_raw[];
+    uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(tile_raw) + 1023) & ~uintptr_t(1023));
+    TileBars* bars = reinterpret_cast<TileBars*>(smem + S::RING);
+    float* ex = reinterpret_cast<float*>(smem + S::RING + 1024);  // [2][128] x 2 words between the teams
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    TileJob b;
+    {   // block -> (tile, sequence, key head, split): the last tiles, which see most, first; splits fastest
+        int64_t x = blockIdx.x;
+        b.c = int(x % a.splits);
+        x /= a.splits;
+        b.j = int(x % a.HKV);
+        x /= a.HKV;
+        b.s = int(x % a.rows.n_seq);
+        b.i = a.tiles_max - 1 - int(x / a.rows.n_seq);
+    }
+    b.sq = kv_seq(a.rows, b.s);
+    const int nrows = b.sq.nq * a.group;
+    if (b.i * KT_ROWS >= nrows) return;
+    if (warp == 9) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(su32(&bars->tmem)) : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    }
+    if (tid == 0) bars->fail = 0;
+    bool ok = true;
+    // the next tile of query rows of this CTA (more than one only when there are more rows than announced)
+    auto take = [&]() {
+        for (;; b.i += a.tiles_max) {
+            if (b.i * KT_ROWS >= nrows) return false;
+            b.cut = a.splits > 1 && b.i < a.tiles_max;
+            if (!b.cut && b.c) return false;
+            b.vis = kv_visible(a.rows, b.sq, min(((b.i + 1) * KT_ROWS - 1) / a.group, b.sq.nq - 1));
+            b.vis_min = kv_visible(a.rows, b.sq, b.i * KT_ROWS / a.group);
+            b.kb = b.cut ? b.c * a.chunk : 0;
+            b.ke = b.cut && b.c < a.splits - 1 ? min(b.vis, b.kb + a.chunk) : b.vis;
+            if (b.c && b.kb >= b.ke) continue;  // nothing here; the join does not look at it
+            b.tiles = max(0, (b.ke - b.kb + KT_KEYS - 1) / KT_KEYS);
+            // edge tiles: those with keys that not every row sees, and a last one that ends inside (at most 3)
+            b.edge0 = max(0, min(b.vis_min, b.vis / KT_KEYS * KT_KEYS) - b.kb) / KT_KEYS;
+            return true;
+        }
+    };
+    auto all_here = [] { asm volatile("bar.sync 0, %0;" ::"n"(KT_THREADS) : "memory"); };
+    // Ring elements in the order of use: K0, K1, V0, K2, V1, K3, V2, ...: K of tile n is element 2n - 1 (K0: 0), V of tile n is 2n + 2
+    // (the last tile's one earlier: no K comes before it)
+    auto k_elem = [&](int n) { return n == 0 ? 0 : 2 * n - 1; };
+    auto v_elem = [&](int n) { return n == b.tiles - 1 ? 2 * n + 1 : 2 * n + 2; };
+
+    if (warp >= 8) {
+        // 384 threads start with 168 registers; 128 of them give what the 256 rows take: 128 * 56 + 256 * 224 = 384 * 168
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
+        for (; take(); b.i += a.tiles_max) {
+        const int N = b.tiles, edge0 = b.edge0;
+        before_sync();
+        all_here();
+        after_sync();
+        const uint32_t tmem = bars->tmem;
+        if (warp == 8) {  // ---- keys and values
+            int searched = edge0;  // edge tiles before this one are done with
+            auto search = [&](int upto) {  // V of the edge tiles below `upto`: their loads are under way
+                for (; searched < upto && ok; ++searched) {
+                    const int e = v_elem(searched), key0 = b.kb + searched * KT_KEYS;
+                    ok = warp_wait(bars->full + e % S::SLOTS, (e / S::SLOTS) & 1, bars);
+                    if (!ok) break;
+                    uint8_t* v = smem + (e % S::SLOTS) * S::SLOT;
+                    const int have = min(KT_KEYS, b.vis - key0), up = (have + 15) / 16 * 16;
+                    for (int w = lane; w < (up - have) * 8 * 2 * PL; w += 32) {  // rows behind the last key
+                        const int part = w / ((up - have) * 8), rest = w % ((up - have) * 8);
+                        *reinterpret_cast<uint4*>(v + part * S::HALF + have * 128 + rest * 16) = make_uint4(0, 0, 0, 0);
+                    }
+                    uint32_t any = 0;
+                    if (b.vis_min < b.vis)
+                        for (int w = lane; w < have * 8 * 2 * PL; w += 32) {
+                            const int part = w / (have * 8), rest = w % (have * 8);
+                            const uint4 u = *reinterpret_cast<const uint4*>(v + part * S::HALF + rest * 16);
+                            for (uint32_t h : {u.x, u.y, u.z, u.w}) any |= uint32_t((h & 0x7c00u) == 0x7c00u) | uint32_t((h & 0x7c000000u) == 0x7c000000u);
+                        }
+                    const bool odd = __any_sync(0xffffffffu, any != 0);
+                    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+                    __syncwarp();
+                    if (lane == 0) {
+                        bars->odd[searched - edge0] = odd;
+                        bar_arrive(bars->edge + (searched - edge0));
+                    }
+                }
+            };
+            int v_issued = 0, issued = 0;
+            for (int e = 0; e < 2 * N && ok; ++e) {
+                const bool is_v = e == 2 * N - 1 || (e >= 2 && e % 2 == 0);
+                const int n = is_v ? (e == 2 * N - 1 ? N - 1 : e / 2 - 1) : (e + 1) / 2;
+                const int slot = e % S::SLOTS;
+                const uint32_t parity = ((e / S::SLOTS) & 1) ^ 1;
+                if (!__all_sync(0xffffffffu, bar_try(bars->empty + slot, parity))) {
+                    search(min(v_issued, N));  // the slot may be waiting for this
+                    if (ok) ok = warp_wait(bars->empty + slot, parity, bars);
+                    if (!ok) break;
+                }
+                const int key0 = b.kb + n * KT_KEYS;
+                const int box = min(a.rows.page, KT_KEYS), boxes = (min(KT_KEYS, b.vis - key0) + box - 1) / box;  // pages with visible keys
+                if (lane == 0) bar_expect(bars->full + slot, uint32_t(boxes * box * 128 * 2 * PL));
+                __syncwarp();
+                if (lane < boxes * 2 * PL) {  // a lane per (page, half, plane)
+                    const int pl = lane % PL, half = lane / PL % 2, q = lane / PL / 2, key = key0 + q * box;
+                    const int pg = kv_page(a.rows, b.s, key);
+                    // a page outside the pool: rows behind the pool, which arrive as zeros
+                    const int y = pg < 0 ? rows_total
+                                         : row0 + int((((int64_t(pg) * 2 + is_v) * a.HKV + b.j) * PL + pl) * a.rows.page) + (key & (a.rows.page - 1));
+                    tma_rows(su32(smem + slot * S::SLOT + pl * S::PLANE + half * S::HALF + q * box * 128), &map, half * 64, y, bars->full + slot);
+                }
+                ++issued;
+                if (is_v) v_issued = n + 1;
+            }
+            search(N);
+            if (!ok)  // nothing may still be arriving when the CTA ends
+                for (int e = max(0, issued - S::SLOTS); e < issued; ++e)
+                    for (unsigned it = 0; it < KT_SPIN && !bar_try(bars->full + e % S::SLOTS, (e / S::SLOTS) & 1); ++it) {}
+        } else if (warp == 9) {
+            if (lane == 0 && N > 0) {  // ---- MMA issuer
+                constexpr uint32_t id_s = idesc_f16(KT_KEYS, false), id_o = idesc_f16(KV_D, true);
+                ok = bar_wait(&bars->q_full, 0, bars);
+                after_sync();
+                auto scores = [&](int n) {
+                    const int e = k_elem(n), slot = e % S::SLOTS;
+                    if (ok) ok = bar_wait(bars->full + slot, (e / S::SLOTS) & 1, bars);
+                    if (!ok) return;
+                    after_sync();
+                    const uint32_t d = tmem + 128 + (n & 1) * 64, k = su32(smem + slot * S::SLOT), qh = tmem, ql = tmem + 64;
+#pragma unroll
+                    for (int ks = 0; ks < 8; ++ks) {
+                        const uint32_t at = k + (ks >> 2) * S::HALF + (ks & 3) * 32;
+                        mma_ts(d, ql + ks * 8, desc_rows(at), id_s, ks != 0);
+                        if (PL == 2) mma_ts(d, qh + ks * 8, desc_rows(at + S::PLANE), id_s, true);
+                    }
+#pragma unroll
+                    for (int ks = 0; ks < 8; ++ks) mma_ts(d, qh + ks * 8, desc_rows(k + (ks >> 2) * S::HALF + (ks & 3) * 32), id_s, true);
+                    commit(bars->empty + slot);
+                    commit(bars->s_full + (n & 1));
+                };
+                scores(0);
+                if (N > 1) scores(1);
+                for (int n = 0; n < N && ok; ++n) {
+                    const int e = v_elem(n), slot = e % S::SLOTS, w = n & 1;
+                    ok = bar_wait(bars->p_full + w, (n >> 1) & 1, bars) && bar_wait(bars->full + slot, (e / S::SLOTS) & 1, bars);
+                    if (ok && n >= edge0) ok = bar_wait(bars->edge + (n - edge0), 0, bars);
+                    if (!ok) break;
+                    after_sync();
+                    const uint32_t d = tmem + 256 + w * 128, p = tmem + 128 + w * 64, v = su32(smem + slot * S::SLOT);
+                    const int steps = min(KT_KEYS / 16, (b.vis - (b.kb + n * KT_KEYS) + 15) / 16);
+                    for (int ks = 0; ks < steps; ++ks) {  // weights of keys 32 c + ..: columns 32 c, hi 16, lo 16
+                        const uint32_t at = p + (ks >> 1) * 32 + (ks & 1) * 8;
+                        mma_ts(d, at + 16, desc_cols(v + ks * 2048, S::HALF), id_o, ks != 0);
+                        if (PL == 2) mma_ts(d, at, desc_cols(v + S::PLANE + ks * 2048, S::HALF), id_o, true);
+                    }
+                    for (int ks = 0; ks < steps; ++ks) mma_ts(d, p + (ks >> 1) * 32 + (ks & 1) * 8, desc_cols(v + ks * 2048, S::HALF), id_o, true);
+                    commit(bars->empty + slot);
+                    commit(bars->o_full + w);
+                    if (n + 2 < N) scores(n + 2);
+                }
+            }
+        }
+        __syncwarp();
+        before_sync();
+        all_here();
+        after_sync();
+        if (bars->fail) break;
+        }
+    } else {
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 224;");
+        for (; take(); b.i += a.tiles_max) {
+        const int N = b.tiles, edge0 = b.edge0;
+        if (tid == 0) {
+            for (int s = 0; s < S::SLOTS; ++s) { bar_init(bars->full + s, 1); bar_init(bars->empty + s, 1); }
+            for (int w = 0; w < 2; ++w) { bar_init(bars->s_full + w, 1); bar_init(bars->p_full + w, 4); bar_init(bars->o_full + w, 1); }
+            bar_init(&bars->q_full, 8);
+            for (int k = 0; k < KT_MAXEDGE; ++k) bar_init(bars->edge + k, 1);
+            asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+        }
+        before_sync();
+        all_here();
+        after_sync();
+        const uint32_t tmem = bars->tmem;
+        {  // ---- two teams: rows
+            const int team = warp >> 2, r = (warp & 3) * 32 + lane, row = b.i * KT_ROWS + r;
+            const uint32_t mine = tmem + (uint32_t((warp & 3) * 32) << 16);
+            const bool real = row < nrows;
+            const int token = real ? row / a.group : 0, head = b.j * a.group + row % a.group;
+            const int see = real ? kv_visible(a.rows, b.sq, token) : b.vis;
+            float f;
+            {   // queries: this team brings 64 of the 128 values of every row
+                float4 q[16];
+                const float4* src = reinterpret_cast<const float4*>(a.q + (b.sq.row0 + token) * a.ldq + head * KV_D + team * 64);
+                float m = 0.f;
+#pragma unroll
+                for (int u = 0; u < 16; ++u) {
+                    q[u] = real ? __ldg(src + u) : make_float4(0.f, 0.f, 0.f, 0.f);
+                    m = fmaxf(m, fmaxf(fmaxf(fabsf(q[u].x), fabsf(q[u].y)), fmaxf(fabsf(q[u].z), fabsf(q[u].w))));
+                }
+                ex[team * 128 + r] = m;
+                asm volatile("bar.sync 1, 256;" ::: "memory");
+                const RowScale rs = row_scale(fmaxf(ex[r], ex[128 + r]), fabsf(a.scale2));  // (a negative scale goes into the queries)
+                f = rs.f;
+                const float sg = a.scale2 < 0.f ? -1.f : 1.f;
+                uint32_t hi[32], lo[32];
+#pragma unroll
+                for (int u = 0; u < 16; ++u) {
+                    half_pair(q[u].x * sg * rs.up.s1 * rs.up.s2, q[u].y * sg * rs.up.s1 * rs.up.s2, hi[2 * u], lo[2 * u]);
+                    half_pair(q[u].z * sg * rs.up.s1 * rs.up.s2, q[u].w * sg * rs.up.s1 * rs.up.s2, hi[2 * u + 1], lo[2 * u + 1]);
+                }
+                tm_st32(mine + team * 32, hi);
+                tm_st32(mine + 64 + team * 32, lo);
+                tm_wait_st();
+                before_sync();
+                __syncwarp();
+                if (lane == 0) bar_arrive(&bars->q_full);
+            }
+            float O[KV_D], m = -INFINITY, l = 0.f;
+#pragma unroll
+            for (int d = 0; d < KV_D; ++d) O[d] = 0.f;
+            const uint32_t sp = mine + 128 + team * 64, so = mine + 256 + team * 128;
+#pragma unroll 1
+            for (int n = team; n < N; n += 2) {
+                ok = warp_wait(bars->s_full + team, (n >> 1) & 1, bars);
+                if (!ok) break;
+                after_sync();
+                const int left = see - (b.kb + n * KT_KEYS);  // keys of the tile that the row sees
+                const bool edge = n >= edge0;
+                uint32_t x[32];
+                float mx = -INFINITY;
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    tm_ld32(sp + h * 32, x);
+                    tm_wait_ld();
+                    if (edge) {
+#pragma unroll
+                        for (int i = 0; i < 32; ++i) mx = fmaxf(mx, h * 32 + i < left ? __uint_as_float(x[i]) : -INFINITY);
+                    } else {
+#pragma unroll
+                        for (int i = 0; i < 32; ++i) mx = fmaxf(mx, __uint_as_float(x[i]));
+                    }
+                }
+                mx = fmaxf(m, mx == -INFINITY ? -INFINITY : mx * f);
+                const float corr = mx == -INFINITY ? 1.f : ex2(m - mx), base = mx == -INFINITY ? 0.f : mx - KA_P;
+                m = mx;
+                float sum[4] = {};
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    if (h == 0) {
+                        tm_ld32(sp, x);
+                        tm_wait_ld();
+                    } else {
+                        tm_ld32(sp + 32, x);
+                        tm_wait_ld();
+                    }
+                    uint32_t p[32];  // 16 words of hi, 16 of lo
+#pragma unroll
+                    for (int i = 0; i < 32; i += 2) {
+                        float p0 = ex2(fmaf(__uint_as_float(x[i]), f, -base)), p1 = ex2(fmaf(__uint_as_float(x[i + 1]), f, -base));
+                        if (edge) {
+                            p0 = h * 32 + i < left && __uint_as_float(x[i]) != -INFINITY ? p0 : 0.f;
+                            p1 = h * 32 + i + 1 < left && __uint_as_float(x[i + 1]) != -INFINITY ? p1 : 0.f;
+                        }
+                        sum[(i >> 1) & 3] += p0 + p1;
+                        half_pair_finite(p0, p1, p[i / 2], p[16 + i / 2]);
+                    }
+                    tm_st32(sp + h * 32, p);
+                }
+                l = l * corr + ((sum[0] + sum[1]) + (sum[2] + sum[3]));
+                tm_wait_st();
+                bool odd = false;
+                if (edge) {
+                    ok = warp_wait(bars->edge + (n - edge0), 0, bars);
+                    if (!ok) break;
+                    odd = *reinterpret_cast<volatile int*>(bars->odd + (n - edge0)) != 0;
+                    if (odd) {  // key by key, for the rows that see it
+                        const int e = v_elem(n);
+                        ok = warp_wait(bars->full + e % S::SLOTS, (e / S::SLOTS) & 1, bars);
+                        if (!ok) break;
+                        const uint8_t* v = smem + (e % S::SLOTS) * S::SLOT;
+#pragma unroll
+                        for (int d = 0; d < KV_D; ++d) O[d] *= corr;
+#pragma unroll 1
+                        for (int key = 0; key < KT_KEYS; ++key) {
+                            __syncwarp();
+                            const uint32_t at = sp + (key >> 5) * 32 + ((key & 31) >> 1);
+                            const uint32_t sh = (key & 1) * 16;
+                            const float w = h2f_bits((tm_ld1(at) >> sh) & 0xffffu) + h2f_bits((tm_ld1(at + 16) >> sh) & 0xffffu);
+                            if (key >= left) continue;
+#pragma unroll
+                            for (int d = 0; d < KV_D; d += 2) {
+                                const int off = (d >> 6) * S::HALF + key * 128 + ((((d & 63) >> 3) ^ (key & 7)) << 4) + (d & 7) * 2;
+                                float2 u = __half22float2(*reinterpret_cast<const __half2*>(v + off));
+                                if (PL == 2) {
+                                    const float2 u2 = __half22float2(*reinterpret_cast<const __half2*>(v + S::PLANE + off));
+                                    u.x += u2.x; u.y += u2.y;
+                                }
+                                O[d] += w * u.x;
+                                O[d + 1] += w * u.y;
+                            }
+                        }
+                    }
+                }
+                before_sync();
+                __syncwarp();
+                if (lane == 0) bar_arrive(bars->p_full + team);
+                ok = warp_wait(bars->o_full + team, (n >> 1) & 1, bars);
+                if (!ok) break;
+                after_sync();
+                if (!odd) {
+#pragma unroll
+                    for (int h = 0; h < 4; ++h) {
+                        tm_ld32(so + h * 32, x);
+                        tm_wait_ld();
+#pragma unroll
+                        for (int i = 0; i < 32; ++i) O[h * 32 + i] = O[h * 32 + i] * corr + __uint_as_float(x[i]);
+                    }
+                }
+                before_sync();
+            }
+            // the teams' results: through shared memory (the ring is used up once both are here)
+            ex[256 + (team * 128 + r) * 2] = m;
+            ex[257 + (team * 128 + r) * 2] = l;
+            asm volatile("bar.sync 1, 256;" ::: "memory");
+            const float m0 = ex[256 + r * 2], l0 = ex[257 + r * 2], m1 = ex[512 + r * 2], l1 = ex[513 + r * 2];
+            const float M = fmaxf(m0, m1), k0 = M == -INFINITY ? 1.f : ex2(m0 - M), k1 = M == -INFINITY ? 1.f : ex2(m1 - M);
+            const float den = k0 * l0 + k1 * l1, k = team ? k1 : k0;
+            const bool final_here = !b.cut || b.vis <= a.chunk;
+            const float inv = final_here ? (den == 0.f ? 0.f : 1.f / den) : 1.f;
+            float4* stage = reinterpret_cast<float4*>(reinterpret_cast<float*>(smem) + r * KT_LD);
+            if (team == 1) {
+#pragma unroll
+                for (int d = 0; d < KV_D; d += 4) stage[d / 4] = make_float4(O[d] * k, O[d + 1] * k, O[d + 2] * k, O[d + 3] * k);
+            }
+            asm volatile("bar.sync 1, 256;" ::: "memory");
+            if (team == 0) {
+#pragma unroll
+                for (int d = 0; d < KV_D; d += 4) {
+                    const float4 u = stage[d / 4];
+                    stage[d / 4] = make_float4((O[d] * k + u.x) * inv, (O[d + 1] * k + u.y) * inv, (O[d + 2] * k + u.z) * inv, (O[d + 3] * k + u.w) * inv);
+                }
+            }
+            const int64_t slot = ((int64_t(b.s) * a.tiles_max + b.i) * a.HKV + b.j) * a.splits + b.c;
+            float* part = a.part + slot * KT_ROWS * (KV_D + 2);
+            if (!final_here && team == 0) { part[KT_ROWS * KV_D + r] = M; part[KT_ROWS * (KV_D + 1) + r] = den; }
+            asm volatile("bar.sync 1, 256;" ::: "memory");
+            if (ok)
+                for (int q = warp; q < KT_ROWS && b.i * KT_ROWS + q < nrows; q += 8) {
+                    const int rw = b.i * KT_ROWS + q;
+                    const float4 u = *reinterpret_cast<const float4*>(reinterpret_cast<float*>(smem) + q * KT_LD + lane * 4);
+                    float* dst = final_here ? a.out + (b.sq.row0 + rw / a.group) * a.ldo + (b.j * a.group + rw % a.group) * KV_D : part + q * KV_D;
+                    *reinterpret_cast<float4*>(dst + lane * 4) = u;
+                }
+        }
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");  // the ring is written by TMA again
+        before_sync();
+        all_here();
+        after_sync();
+        if (bars->fail) break;
+        if (tid == 0) {
+            for (int s = 0; s < S::SLOTS; ++s) { bar_inval(bars->full + s); bar_inval(bars->empty + s); }
+            for (int w = 0; w < 2; ++w) { bar_inval(bars->s_full + w); bar_inval(bars->p_full + w); bar_inval(bars->o_full + w); }
+            bar_inval(&bars->q_full);
+            for (int k = 0; k < KT_MAXEDGE; ++k) bar_inval(bars->edge + k);
+        }
+        }
+    }
+    all_here();
+    if (tid == 0 && bars->fail) atomicExch(err, 1);
+    if (warp == 9) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(bars->tmem) : "memory");
+}
+
+int* tile_error_word() {  // pinned, mapped: raised by a kernel whose bounded wait ran out
+    static int* host = [] {
+        int* p = nullptr;
+        if (cudaHostAlloc(&p, sizeof(int), cudaHostAllocMapped | cudaHostAllocPortable) != cudaSuccess) return static_cast<int*>(nullptr);
+        *p = 0;
+        return p;
+    }();
+    return host;
+}
+
+struct TilePlan { int tiles, splits, chunk; };
+
+TilePlan tile_plan(const Kv* kv, const elb_kv_batch* b, int n_head) {
+    TilePlan p{};
+    const int64_t rows = int64_t(std::max(1, std::min(b->max_q, b->n_tok))) * (n_head / kv->HKV);
+    p.tiles = int((rows + KT_ROWS - 1) / KT_ROWS);
+    const int64_t base = int64_t(b->n_seq) * kv->HKV * p.tiles;
+    const int len = std::max(b->max_len, 1);
+    int64_t want = base >= 2 * kv->sm_count ? 1 : std::max<int64_t>(1, (int64_t(kv->sm_count) * (b->n_seq > 1 ? 4 : 1)) / base);
+    want = std::min<int64_t>(want, (len + 255) / 256);
+    p.chunk = int((len + want - 1) / want + KT_KEYS - 1) / KT_KEYS * KT_KEYS;
+    p.splits = (len + p.chunk - 1) / p.chunk;
+    return p;
+}
+
+}  // namespace
+
+int kv_attn_tile_check() {  // did a call's kernel give up on a wait?
+    int* e = tile_error_word();
+    if (e && *reinterpret_cast<volatile int*>(e)) {
+        *e = 0;
+        return fail(ELB_ERR_CUDA, "kv_attention: a bounded wait ran out in an earlier call");
+    }
+    return ELB_OK;
+}
+
+size_t kv_attn_tile_work(const Kv* kv, const elb_kv_batch* b, int n_head) {
+    const TilePlan p = tile_plan(kv, b, n_head);
+    if (p.splits == 1) return 0;
+    return size_t(b->n_seq) * p.tiles * kv->HKV * p.splits * KT_ROWS * (KV_D + 2) * 4;
+}
+
+int kv_attn_tile_launch(const Kv* kv, int layer, KvAttnArgs a, const elb_kv_batch* b, cudaStream_t s) {
+    int* err = nullptr;
+    if (!tile_error_word() || cudaHostGetDevicePointer(&err, tile_error_word(), 0) != cudaSuccess) return fail(ELB_ERR_CUDA, "kv_attention: no error word");
+    ELB_TRY(kv_attn_tile_check());
+    const TilePlan p = tile_plan(kv, b, a.H);
+    a.splits = p.splits; a.chunk = p.chunk; a.tiles_max = p.tiles;
+    const int64_t blocks = int64_t(b->n_seq) * p.tiles * kv->HKV;
+    if (blocks * p.splits > 0x7fffffff || blocks * KT_ROWS / 8 > 0x7fffffff) return fail(ELB_ERR_UNSUPPORTED, "kv_attention: too many rows");
+    const int64_t layer_rows = kv->layer_halves() / KV_D;
+    auto run = [&](auto kernel, int smem) -> int {
+        ELB_TRY(ensure_dyn_smem(reinterpret_cast<const void*>(kernel), size_t(smem)));
+        kernel<<<unsigned(blocks * p.splits), KT_THREADS, smem, s>>>(kv->map, a, int(layer * layer_rows), int(kv->n_layer * layer_rows), err);
+        ELB_CUDA(cudaGetLastError());
+        return ELB_OK;
+    };
+    if (kv->planes == 1) ELB_TRY(run(k_kv_attn_tile<1>, TileShape<1>::SMEM));
+    else ELB_TRY(run(k_kv_attn_tile<2>, TileShape<2>::SMEM));
+    return p.splits > 1 ? kv_attn_join(a, KT_ROWS, blocks, s) : ELB_OK;
+}
+
+}  // namespace elb
