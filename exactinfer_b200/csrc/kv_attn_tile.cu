@@ -80,10 +80,16 @@ __device__ __forceinline__ void tma_rows(uint32_t dst, const CUtensorMap* map, i
 }
 __device__ __forceinline__ void before_sync() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
 __device__ __forceinline__ void after_sync() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
-// D (+)= A B, A in tensor memory, B in shared memory
-__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, bool add) {
-    asm volatile("{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n}\n"
-                 ::"r"(d), "r"(a), "l"(b), "r"(idesc), "r"(uint32_t(add)) : "memory");
+// D (+)= A B, A in tensor memory, B in shared memory (descriptor in two words: what varies, what does not)
+template <bool ADD> __device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint32_t b, uint32_t b_hi, uint32_t idesc) {
+    asm volatile("{\n .reg .pred p;\n .reg .b64 db;\n setp.ne.b32 p, %5, 0;\n mov.b64 db, {%2, %3};\n"
+                 " tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], db, %4, p;\n}\n"
+                 ::"r"(d), "r"(a), "r"(b), "r"(b_hi), "r"(idesc), "n"(int(ADD)) : "memory");
+}
+__device__ __forceinline__ bool elect() {
+    uint32_t p;
+    asm volatile("{\n .reg .pred p;\n elect.sync _|p, 0xffffffff;\n selp.u32 %0, 1, 0, p;\n}\n" : "=r"(p));
+    return p != 0;
 }
 __device__ __forceinline__ void commit(uint64_t* bar) {
     asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(su32(bar)) : "memory");
@@ -95,6 +101,14 @@ __device__ __forceinline__ void tm_ld32(uint32_t a, uint32_t (&r)[32]) {
         "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,%22,"
         "%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
         : KT_R8(r, 0), KT_R8(r, 8), KT_R8(r, 16), KT_R8(r, 24) : "r"(a) : "memory");
+}
+__device__ __forceinline__ void tm_ld16(uint32_t a, uint32_t (&r)[16]) {
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
+                 : KT_R8(r, 0), KT_R8(r, 8) : "r"(a) : "memory");
+}
+__device__ __forceinline__ void tm_st16(uint32_t a, const uint32_t (&r)[16]) {
+    asm volatile("tcgen05.st.sync.aligned.32x32b.x16.b32 [%16], {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15};"
+                 ::KT_I8(r, 0), KT_I8(r, 8), "r"(a) : "memory");
 }
 __device__ __forceinline__ uint32_t tm_ld1(uint32_t a) {
     uint32_t r;
@@ -111,14 +125,98 @@ __device__ __forceinline__ void tm_st32(uint32_t a, const uint32_t (&r)[32]) {
         ::KT_I8(r, 0), KT_I8(r, 8), KT_I8(r, 16), KT_I8(r, 24), "r"(a) : "memory");
 }
 // Shared-memory operands with 128-byte swizzle. Keys: 64 rows (N) of 64 values (K) in a row, 8-row groups 1024 bytes apart.
-// Values: rows are K (keys), 8-row groups 1024 bytes apart, 64 of the N = 128 dimensions in a row, the others `HALF` bytes behind.
-__device__ __forceinline__ uint64_t desc_rows(uint32_t a) {
-    return uint64_t((a & 0x3FFFF) >> 4) | uint64_t(1024 >> 4) << 32 | uint64_t(1) << 46 | uint64_t(2) << 61;
-}
-__device__ __forceinline__ uint64_t desc_cols(uint32_t a, uint32_t far) { return desc_rows(a) | uint64_t(far >> 4) << 16; }
+// Values: rows are K (keys), 8-row groups 1024 bytes apart, 64 of the N = 128 dimensions in a row, the others HALF bytes behind.
+// Low word: address / 16 and (values) HALF / 16 << 16; high word: 1024 / 16, version 1, swizzle 128.
+constexpr uint32_t KT_DESC_HI = (1024u >> 4) | (1u << 14) | (2u << 29);
+__device__ __forceinline__ uint32_t desc_lo(uint32_t a, uint32_t far) { return ((a & 0x3FFFF) >> 4) | (far >> 4) << 16; }
 // fp16 x fp16 -> fp32, M = 128 from tensor memory, N columns; B with N along the rows when `cols`
 __host__ __device__ constexpr uint32_t idesc_f16(int n, bool cols) {
     return (1u << 4) | (cols ? 1u << 16 : 0u) | (uint32_t(n >> 3) << 17) | (uint32_t(KT_ROWS >> 4) << 24);
+}
+
+// two fp32 numbers in one instruction
+using Two = unsigned long long;
+__device__ __forceinline__ Two two(uint32_t a, uint32_t b) {
+    Two r;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "r"(a), "r"(b));
+    return r;
+}
+__device__ __forceinline__ Two two(float a, float b) { return two(__float_as_uint(a), __float_as_uint(b)); }
+__device__ __forceinline__ float2 parts(Two x) {
+    uint32_t a, b;
+    asm("mov.b64 {%0, %1}, %2;" : "=r"(a), "=r"(b) : "l"(x));
+    return make_float2(__uint_as_float(a), __uint_as_float(b));
+}
+__device__ __forceinline__ Two fma2(Two a, Two b, Two c) {
+    Two r;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+    return r;
+}
+__device__ __forceinline__ Two add2(Two a, Two b) {
+    Two r;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
+__device__ __forceinline__ float max3(float a, float b, float c) {
+    float r;
+    asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+    return r;
+}
+
+// A row's scores of one key tile in tensor memory (64 columns from sp) -> weights in their place, per 16 keys 8 columns of hi and 8
+// of lo; running maximum m and denominator l. Returns what earlier sums are to be multiplied by. EDGE: only the first
+// `left` keys are seen. The loops stay rolled: straight-line code that a warp runs once per tile comes in at the
+// speed of instruction fetch (unrolled, with both forms in one body, this took 3000 clocks a tile).
+template <bool EDGE> __device__ __forceinline__ float tile_weights(uint32_t sp, float f, int left, float& m, float& l) {
+    float mx = -INFINITY;
+#pragma unroll 1
+    for (int h = 0; h < KT_KEYS; h += 32) {
+        uint32_t x[32];
+        tm_ld32(sp + h, x);
+        tm_wait_ld();
+        float u[4] = {mx, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+        for (int i = 0; i < 32; i += 2) {
+            const float x0 = EDGE && h + i >= left ? -INFINITY : __uint_as_float(x[i]);
+            const float x1 = EDGE && h + i + 1 >= left ? -INFINITY : __uint_as_float(x[i + 1]);
+            u[(i >> 1) & 3] = max3(u[(i >> 1) & 3], x0, x1);
+        }
+        mx = fmaxf(max3(u[0], u[1], u[2]), u[3]);
+    }
+    mx = fmaxf(m, mx == -INFINITY ? -INFINITY : mx * f);
+    const float corr = mx == -INFINITY ? 1.f : ex2(m - mx), base = mx == -INFINITY ? 0.f : mx - KA_P;
+    m = mx;
+    const Two ff = two(f, f), nb = two(-base, -base), minus = two(-1.f, -1.f);
+    Two sum = two(0.f, 0.f), sum_b = sum;
+#pragma unroll 1
+    for (int h = 0; h < KT_KEYS; h += 16) {
+        uint32_t x[16], p[16];
+        tm_ld16(sp + h, x);
+        tm_wait_ld();
+#pragma unroll
+        for (int i = 0; i < 16; i += 2) {
+            const float2 y = parts(fma2(two(x[i], x[i + 1]), ff, nb));
+            float p0 = ex2(y.x), p1 = ex2(y.y);
+            if (EDGE) {
+                p0 = h + i < left && __uint_as_float(x[i]) != -INFINITY ? p0 : 0.f;
+                p1 = h + i + 1 < left && __uint_as_float(x[i + 1]) != -INFINITY ? p1 : 0.f;
+            }
+            const Two pp = two(p0, p1);
+            if (i & 2) sum_b = add2(sum_b, pp);
+            else sum = add2(sum, pp);
+            // hi: the upper 11 bits (exact in fp16 from 2^-14 on, 2^-25 off at most below: weights go up to 2^14); lo: the rest
+            const float h0 = __uint_as_float(__float_as_uint(p0) & 0xffffe000u), h1 = __uint_as_float(__float_as_uint(p1) & 0xffffe000u);
+            const float2 r = parts(fma2(two(h0, h1), minus, pp));
+            const __half2 hi = __floats2half2_rn(h0, h1), lo = __floats2half2_rn(r.x, r.y);
+            p[i / 2] = *reinterpret_cast<const uint32_t*>(&hi);
+            p[8 + i / 2] = *reinterpret_cast<const uint32_t*>(&lo);
+        }
+        tm_st16(sp + h, p);
+    }
+    const float2 t = parts(add2(sum, sum_b));
+    l = l * corr + (t.x + t.y);
+    tm_wait_st();
+    return corr;
 }
 
 // What a CTA works on
@@ -174,9 +272,8 @@ __global__ void __launch_bounds__(KT_THREADS, 1) k_kv_attn_tile(const __grid_con
         }
     };
     auto all_here = [] { asm volatile("bar.sync 0, %0;" ::"n"(KT_THREADS) : "memory"); };
-    // Ring elements in the order of use: K0, K1, V0, K2, V1, K3, V2, ...: K of tile n is element 2n - 1 (K0: 0), V of tile n is 2n + 2
+    // Ring elements in the order of use: K0, K1, V0, K2, V1, K3, V2, ...: V of tile n is element 2n + 2
     // (the last tile's one earlier: no K comes before it)
-    auto k_elem = [&](int n) { return n == 0 ? 0 : 2 * n - 1; };
     auto v_elem = [&](int n) { return n == b.tiles - 1 ? 2 * n + 1 : 2 * n + 2; };
 
     if (warp >= 8) {
@@ -187,7 +284,6 @@ __global__ void __launch_bounds__(KT_THREADS, 1) k_kv_attn_tile(const __grid_con
         before_sync();
         all_here();
         after_sync();
-        const uint32_t tmem = bars->tmem;
         if (warp == 8) {  // ---- keys and values
             int searched = edge0;  // edge tiles before this one are done with
             auto search = [&](int upto) {  // V of the edge tiles below `upto`: their loads are under way
@@ -247,48 +343,65 @@ __global__ void __launch_bounds__(KT_THREADS, 1) k_kv_attn_tile(const __grid_con
             if (!ok)  // nothing may still be arriving when the CTA ends
                 for (int e = max(0, issued - S::SLOTS); e < issued; ++e)
                     for (unsigned it = 0; it < KT_SPIN && !bar_try(bars->full + e % S::SLOTS, (e / S::SLOTS) & 1); ++it) {}
-        } else if (warp == 9) {
-            if (lane == 0 && N > 0) {  // ---- MMA issuer
-                constexpr uint32_t id_s = idesc_f16(KT_KEYS, false), id_o = idesc_f16(KV_D, true);
-                ok = bar_wait(&bars->q_full, 0, bars);
+        } else if (warp == 9 && N > 0) {  // ---- MMA issuer: the whole warp walks the tiles, one lane issues
+            // (with all of it inside `if (lane == 0)` every operand went through a vector register: 100 clocks per MMA)
+            constexpr uint32_t id_s = idesc_f16(KT_KEYS, false), id_o = idesc_f16(KV_D, true);
+            const uint32_t ring_k = desc_lo(su32(smem), 0), ring_v = desc_lo(su32(smem), S::HALF);
+            uint32_t slot = 0, phase = 0;
+            auto next = [&]() {
+                if (++slot == S::SLOTS) { slot = 0; phase ^= 1; }
+            };
+            ok = warp_wait(&bars->q_full, 0, bars);
+            auto scores = [&](int n) {
+                if (ok) ok = warp_wait(bars->full + slot, phase, bars);
+                if (!ok) return;
                 after_sync();
-                auto scores = [&](int n) {
-                    const int e = k_elem(n), slot = e % S::SLOTS;
-                    if (ok) ok = bar_wait(bars->full + slot, (e / S::SLOTS) & 1, bars);
-                    if (!ok) return;
-                    after_sync();
-                    const uint32_t d = tmem + 128 + (n & 1) * 64, k = su32(smem + slot * S::SLOT), qh = tmem, ql = tmem + 64;
+                const uint32_t d = 128 + (n & 1) * 64, k = ring_k + slot * (S::SLOT >> 4);
+                if (elect()) {
 #pragma unroll
                     for (int ks = 0; ks < 8; ++ks) {
-                        const uint32_t at = k + (ks >> 2) * S::HALF + (ks & 3) * 32;
-                        mma_ts(d, ql + ks * 8, desc_rows(at), id_s, ks != 0);
-                        if (PL == 2) mma_ts(d, qh + ks * 8, desc_rows(at + S::PLANE), id_s, true);
+                        const uint32_t at = k + (ks >> 2) * (S::HALF >> 4) + (ks & 3) * 2;
+                        if (ks == 0) mma_ts<false>(d, 64, at, KT_DESC_HI, id_s);
+                        else mma_ts<true>(d, 64 + ks * 8, at, KT_DESC_HI, id_s);
+                        if (PL == 2) mma_ts<true>(d, ks * 8, at + (S::PLANE >> 4), KT_DESC_HI, id_s);
                     }
 #pragma unroll
-                    for (int ks = 0; ks < 8; ++ks) mma_ts(d, qh + ks * 8, desc_rows(k + (ks >> 2) * S::HALF + (ks & 3) * 32), id_s, true);
+                    for (int ks = 0; ks < 8; ++ks) mma_ts<true>(d, ks * 8, k + (ks >> 2) * (S::HALF >> 4) + (ks & 3) * 2, KT_DESC_HI, id_s);
                     commit(bars->empty + slot);
                     commit(bars->s_full + (n & 1));
-                };
-                scores(0);
-                if (N > 1) scores(1);
-                for (int n = 0; n < N && ok; ++n) {
-                    const int e = v_elem(n), slot = e % S::SLOTS, w = n & 1;
-                    ok = bar_wait(bars->p_full + w, (n >> 1) & 1, bars) && bar_wait(bars->full + slot, (e / S::SLOTS) & 1, bars);
-                    if (ok && n >= edge0) ok = bar_wait(bars->edge + (n - edge0), 0, bars);
-                    if (!ok) break;
-                    after_sync();
-                    const uint32_t d = tmem + 256 + w * 128, p = tmem + 128 + w * 64, v = su32(smem + slot * S::SLOT);
-                    const int steps = min(KT_KEYS / 16, (b.vis - (b.kb + n * KT_KEYS) + 15) / 16);
-                    for (int ks = 0; ks < steps; ++ks) {  // weights of keys 32 c + ..: columns 32 c, hi 16, lo 16
-                        const uint32_t at = p + (ks >> 1) * 32 + (ks & 1) * 8;
-                        mma_ts(d, at + 16, desc_cols(v + ks * 2048, S::HALF), id_o, ks != 0);
-                        if (PL == 2) mma_ts(d, at, desc_cols(v + S::PLANE + ks * 2048, S::HALF), id_o, true);
+                }
+                __syncwarp();
+                next();
+            };
+            scores(0);
+            if (N > 1) scores(1);
+            for (int n = 0; n < N && ok; ++n) {
+                const int w = n & 1;
+                ok = warp_wait(bars->p_full + w, (n >> 1) & 1, bars) && warp_wait(bars->full + slot, phase, bars);
+                if (ok && n >= edge0) ok = warp_wait(bars->edge + (n - edge0), 0, bars);
+                if (!ok) break;
+                after_sync();
+                const uint32_t d = 256 + w * 128, p = 128 + w * 64, v = ring_v + slot * (S::SLOT >> 4);
+                const int steps = min(KT_KEYS / 16, (b.vis - (b.kb + n * KT_KEYS) + 15) / 16);
+                if (elect()) {
+#pragma unroll
+                    for (int ks = 0; ks < KT_KEYS / 16; ++ks) {  // weights of 16 keys: 8 columns of hi, 8 of lo
+                        if (ks >= steps) break;
+                        if (ks == 0) mma_ts<false>(d, p + 8, v, KT_DESC_HI, id_o);
+                        else mma_ts<true>(d, p + ks * 16 + 8, v + ks * 128, KT_DESC_HI, id_o);
+                        if (PL == 2) mma_ts<true>(d, p + ks * 16, v + (S::PLANE >> 4) + ks * 128, KT_DESC_HI, id_o);
                     }
-                    for (int ks = 0; ks < steps; ++ks) mma_ts(d, p + (ks >> 1) * 32 + (ks & 1) * 8, desc_cols(v + ks * 2048, S::HALF), id_o, true);
+#pragma unroll
+                    for (int ks = 0; ks < KT_KEYS / 16; ++ks) {
+                        if (ks >= steps) break;
+                        mma_ts<true>(d, p + ks * 16, v + ks * 128, KT_DESC_HI, id_o);
+                    }
                     commit(bars->empty + slot);
                     commit(bars->o_full + w);
-                    if (n + 2 < N) scores(n + 2);
                 }
+                __syncwarp();
+                next();
+                if (n + 2 < N) scores(n + 2);
             }
         }
         __syncwarp();
@@ -311,10 +424,9 @@ __global__ void __launch_bounds__(KT_THREADS, 1) k_kv_attn_tile(const __grid_con
         before_sync();
         all_here();
         after_sync();
-        const uint32_t tmem = bars->tmem;
         {  // ---- two teams: rows
             const int team = warp >> 2, r = (warp & 3) * 32 + lane, row = b.i * KT_ROWS + r;
-            const uint32_t mine = tmem + (uint32_t((warp & 3) * 32) << 16);
+            const uint32_t mine = uint32_t((warp & 3) * 32) << 16;  // (all 512 columns are this CTA's: they start at 0)
             const bool real = row < nrows;
             const int token = real ? row / a.group : 0, head = b.j * a.group + row % a.group;
             const int see = real ? kv_visible(a.rows, b.sq, token) : b.vis;
@@ -346,61 +458,23 @@ __global__ void __launch_bounds__(KT_THREADS, 1) k_kv_attn_tile(const __grid_con
                 __syncwarp();
                 if (lane == 0) bar_arrive(&bars->q_full);
             }
-            float O[KV_D], m = -INFINITY, l = 0.f;
+            Two O[KV_D / 2];
+            float m = -INFINITY, l = 0.f;
 #pragma unroll
-            for (int d = 0; d < KV_D; ++d) O[d] = 0.f;
+            for (int d = 0; d < KV_D / 2; ++d) O[d] = two(0.f, 0.f);
             const uint32_t sp = mine + 128 + team * 64, so = mine + 256 + team * 128;
 #pragma unroll 1
             for (int n = team; n < N; n += 2) {
                 ok = warp_wait(bars->s_full + team, (n >> 1) & 1, bars);
                 if (!ok) break;
                 after_sync();
-                const int left = see - (b.kb + n * KT_KEYS);  // keys of the tile that the row sees
-                const bool edge = n >= edge0;
-                uint32_t x[32];
-                float mx = -INFINITY;
-#pragma unroll
-                for (int h = 0; h < 2; ++h) {
-                    tm_ld32(sp + h * 32, x);
-                    tm_wait_ld();
-                    if (edge) {
-#pragma unroll
-                        for (int i = 0; i < 32; ++i) mx = fmaxf(mx, h * 32 + i < left ? __uint_as_float(x[i]) : -INFINITY);
-                    } else {
-#pragma unroll
-                        for (int i = 0; i < 32; ++i) mx = fmaxf(mx, __uint_as_float(x[i]));
-                    }
-                }
-                mx = fmaxf(m, mx == -INFINITY ? -INFINITY : mx * f);
-                const float corr = mx == -INFINITY ? 1.f : ex2(m - mx), base = mx == -INFINITY ? 0.f : mx - KA_P;
-                m = mx;
-                float sum[4] = {};
-#pragma unroll
-                for (int h = 0; h < 2; ++h) {
-                    if (h == 0) {
-                        tm_ld32(sp, x);
-                        tm_wait_ld();
-                    } else {
-                        tm_ld32(sp + 32, x);
-                        tm_wait_ld();
-                    }
-                    uint32_t p[32];  // 16 words of hi, 16 of lo
-#pragma unroll
-                    for (int i = 0; i < 32; i += 2) {
-                        float p0 = ex2(fmaf(__uint_as_float(x[i]), f, -base)), p1 = ex2(fmaf(__uint_as_float(x[i + 1]), f, -base));
-                        if (edge) {
-                            p0 = h * 32 + i < left && __uint_as_float(x[i]) != -INFINITY ? p0 : 0.f;
-                            p1 = h * 32 + i + 1 < left && __uint_as_float(x[i + 1]) != -INFINITY ? p1 : 0.f;
-                        }
-                        sum[(i >> 1) & 3] += p0 + p1;
-                        half_pair_finite(p0, p1, p[i / 2], p[16 + i / 2]);
-                    }
-                    tm_st32(sp + h * 32, p);
-                }
-                l = l * corr + ((sum[0] + sum[1]) + (sum[2] + sum[3]));
-                tm_wait_st();
                 bool odd = false;
-                if (edge) {
+                float corr;
+                if (n < edge0) {
+                    corr = tile_weights<false>(sp, f, KT_KEYS, m, l);
+                } else {
+                    const int left = see - (b.kb + n * KT_KEYS);  // keys of the tile that the row sees
+                    corr = tile_weights<true>(sp, f, left, m, l);
                     ok = warp_wait(bars->edge + (n - edge0), 0, bars);
                     if (!ok) break;
                     odd = *reinterpret_cast<volatile int*>(bars->odd + (n - edge0)) != 0;
@@ -409,15 +483,16 @@ __global__ void __launch_bounds__(KT_THREADS, 1) k_kv_attn_tile(const __grid_con
                         ok = warp_wait(bars->full + e % S::SLOTS, (e / S::SLOTS) & 1, bars);
                         if (!ok) break;
                         const uint8_t* v = smem + (e % S::SLOTS) * S::SLOT;
+                        const Two cc = two(corr, corr), zero = two(0.f, 0.f);
 #pragma unroll
-                        for (int d = 0; d < KV_D; ++d) O[d] *= corr;
+                        for (int d = 0; d < KV_D / 2; ++d) O[d] = fma2(O[d], cc, zero);
 #pragma unroll 1
                         for (int key = 0; key < KT_KEYS; ++key) {
                             __syncwarp();
-                            const uint32_t at = sp + (key >> 5) * 32 + ((key & 31) >> 1);
-                            const uint32_t sh = (key & 1) * 16;
-                            const float w = h2f_bits((tm_ld1(at) >> sh) & 0xffffu) + h2f_bits((tm_ld1(at + 16) >> sh) & 0xffffu);
+                            const uint32_t at = sp + (key >> 4) * 16 + ((key & 15) >> 1), sh = (key & 1) * 16;
+                            const float w = h2f_bits((tm_ld1(at) >> sh) & 0xffffu) + h2f_bits((tm_ld1(at + 8) >> sh) & 0xffffu);
                             if (key >= left) continue;
+                            const Two ww = two(w, w);
 #pragma unroll
                             for (int d = 0; d < KV_D; d += 2) {
                                 const int off = (d >> 6) * S::HALF + key * 128 + ((((d & 63) >> 3) ^ (key & 7)) << 4) + (d & 7) * 2;
@@ -426,10 +501,10 @@ __global__ void __launch_bounds__(KT_THREADS, 1) k_kv_attn_tile(const __grid_con
                                     const float2 u2 = __half22float2(*reinterpret_cast<const __half2*>(v + S::PLANE + off));
                                     u.x += u2.x; u.y += u2.y;
                                 }
-                                O[d] += w * u.x;
-                                O[d + 1] += w * u.y;
+                                O[d / 2] = fma2(ww, two(u.x, u.y), O[d / 2]);
                             }
                         }
+                        __syncwarp();
                     }
                 }
                 before_sync();
@@ -438,13 +513,16 @@ __global__ void __launch_bounds__(KT_THREADS, 1) k_kv_attn_tile(const __grid_con
                 ok = warp_wait(bars->o_full + team, (n >> 1) & 1, bars);
                 if (!ok) break;
                 after_sync();
-                if (!odd) {
+                if (!odd) {  // the next 32 sums are on their way while these are added
+                    const Two cc = two(corr, corr);
+                    uint32_t x[2][32];
+                    tm_ld32(so, x[0]);
 #pragma unroll
                     for (int h = 0; h < 4; ++h) {
-                        tm_ld32(so + h * 32, x);
                         tm_wait_ld();
+                        if (h < 3) tm_ld32(so + h * 32 + 32, x[(h + 1) & 1]);
 #pragma unroll
-                        for (int i = 0; i < 32; ++i) O[h * 32 + i] = O[h * 32 + i] * corr + __uint_as_float(x[i]);
+                        for (int i = 0; i < 32; i += 2) O[h * 16 + i / 2] = fma2(O[h * 16 + i / 2], cc, two(x[h & 1][i], x[h & 1][i + 1]));
                     }
                 }
                 before_sync();
@@ -461,14 +539,18 @@ __global__ void __launch_bounds__(KT_THREADS, 1) k_kv_attn_tile(const __grid_con
             float4* stage = reinterpret_cast<float4*>(reinterpret_cast<float*>(smem) + r * KT_LD);
             if (team == 1) {
 #pragma unroll
-                for (int d = 0; d < KV_D; d += 4) stage[d / 4] = make_float4(O[d] * k, O[d + 1] * k, O[d + 2] * k, O[d + 3] * k);
+                for (int d = 0; d < KV_D; d += 4) {
+                    const float2 x = parts(O[d / 2]), y = parts(O[d / 2 + 1]);
+                    stage[d / 4] = make_float4(x.x * k, x.y * k, y.x * k, y.y * k);
+                }
             }
             asm volatile("bar.sync 1, 256;" ::: "memory");
             if (team == 0) {
 #pragma unroll
                 for (int d = 0; d < KV_D; d += 4) {
                     const float4 u = stage[d / 4];
-                    stage[d / 4] = make_float4((O[d] * k + u.x) * inv, (O[d + 1] * k + u.y) * inv, (O[d + 2] * k + u.z) * inv, (O[d + 3] * k + u.w) * inv);
+                    const float2 x = parts(O[d / 2]), y = parts(O[d / 2 + 1]);
+                    stage[d / 4] = make_float4((x.x * k + u.x) * inv, (x.y * k + u.y) * inv, (y.x * k + u.z) * inv, (y.y * k + u.w) * inv);
                 }
             }
             const int64_t slot = ((int64_t(b.s) * a.tiles_max + b.i) * a.HKV + b.j) * a.splits + b.c;
