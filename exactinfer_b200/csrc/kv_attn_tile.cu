@@ -2,7 +2,7 @@
 // 5th-generation tensor cores.
 //
 // A CTA takes 128 query rows of one sequence and key head (tokens x the query heads that share the key head) and walks the keys
-// that they see, 64 at a time: S = Q K^T, weights 2^(scale2 S - m + 14), O += P V. fp32 accuracy from fp16 operands as in
+// that they see, 128 at a time: S = Q K^T, weights 2^(scale2 S - m + 14), O += P V. fp32 accuracy from fp16 operands as in
 // kv_attn_few.cu: a query row is scaled by a power of two and held as hi + lo (22 bits), the weights as well, keys and
 // values are one fp16 or a pair as the cache holds them; lo lo is left out, so that a product costs 2 MMAs (F16 cache) or 3 (pairs).
 // The tensor core adds with truncation: the small products of a step go first, hi hi (8 links for S, 4 for O) last, and
@@ -11,11 +11,12 @@
 //
 // Two teams of four warps work on alternate key tiles, a thread per query row (= TMEM lane), each with its own running
 // maximum, denominator and 128 sums, joined once at the end: while one team forms its weights, the tensor core
-// multiplies for the other. One warp brings keys and values by TMA, page by page, into a ring of 64-key tiles in the
+// multiplies for the other. One warp brings keys and values by TMA, page by page, into a ring of 128-key tiles in the
 // order of their use; one thread issues the MMAs. TMEM: Q hi | lo (128 columns, the A operand of S: read from there, the
-// shared memory has only K to deliver), per team S (64 columns, overwritten by the weights hi | lo, the A operand of O) and
-// O (128). V lies [key][dimension] as in the page and is a B operand with N along the rows.
-// A tile's 64 keys take 1024 (F16) or 1536 (pairs) clocks of the tensor pipe.
+// shared memory has only K to deliver), per team S (128 columns, overwritten by the weights hi | lo, the A operand of O) and one
+// O (128): a team takes it into its registers while the tensor core forms the next S. V lies [key][dimension] as in the page and is a B operand with N along the rows.
+// A tile's 128 keys take 2048 (F16) or 3 * 1024 (pairs) clocks of the tensor pipe. (64-key tiles: an MMA with N = 64 took 51
+// clocks instead of 32, and the whole 1860 a tile.)
 //
 // Behind the last visible key the weights are 0, but 0 * NaN is not: the PV product stops at the last 16 keys, and the rows of
 // V behind the last key are emptied in shared memory. In the few tiles that only some rows see, V is searched for infinities and
@@ -28,22 +29,22 @@ namespace elb {
 
 namespace {
 
-constexpr int KT_ROWS = 128, KT_KEYS = 64, KT_THREADS = 384, KT_MAXEDGE = 4;
-constexpr unsigned KT_SPIN = 1u << 24;
+constexpr int KT_ROWS = 128, KT_KEYS = 128, KT_THREADS = 384, KT_MAXEDGE = 4;
+constexpr unsigned KT_SPIN = 1u << 21;
 constexpr int KT_LD = KV_D + 4;  // floats per row when the teams meet
 
 template <int PL> struct TileShape {
-    static constexpr int HALF = KT_KEYS * 128;           // 64 rows of 64 values
-    static constexpr int PLANE = 2 * HALF;               // 64 keys of one plane
+    static constexpr int HALF = KT_KEYS * 128;           // 64 of the 128 values of every key
+    static constexpr int PLANE = 2 * HALF;               // one plane
     static constexpr int SLOT = PL * PLANE;              // keys or values of a tile
-    static constexpr int SLOTS = 12 / PL;
+    static constexpr int SLOTS = 6 / PL;
     static constexpr int RING = SLOTS * SLOT;
     static constexpr int SMEM = RING + 4096 + 1024;
     static_assert(RING >= KT_ROWS * KT_LD * 4, "the teams' sums take the place of the ring");
 };
 
 struct TileBars {
-    uint64_t full[12], empty[12], s_full[2], p_full[2], o_full[2], q_full, edge[KT_MAXEDGE];
+    uint64_t full[6], empty[6], s_full[2], p_full[2], o_full[2], o_free, q_full, edge[KT_MAXEDGE];
     uint32_t tmem;
     int odd[KT_MAXEDGE];  // edge tile k has infinities or NaN among its values
     int fail;
@@ -113,10 +114,16 @@ __device__ __forceinline__ void tm_st16(uint32_t a, const uint32_t (&r)[16]) {
 __device__ __forceinline__ uint32_t tm_ld1(uint32_t a) {
     uint32_t r;
     asm volatile("tcgen05.ld.sync.aligned.32x32b.x1.b32 {%0}, [%1];" : "=r"(r) : "r"(a) : "memory");
-    asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+    asm volatile("tcgen05.wait::ld.sync.aligned;" : "+r"(r)::"memory");
     return r;
 }
-__device__ __forceinline__ void tm_wait_ld() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
+// Loads return at once; what they bring is there behind the wait. It takes the registers as operands, so that nothing that reads
+// them can be moved in front of it.
+#define KT_W8(r, o) "+r"(r[o]), "+r"(r[o + 1]), "+r"(r[o + 2]), "+r"(r[o + 3]), "+r"(r[o + 4]), "+r"(r[o + 5]), "+r"(r[o + 6]), "+r"(r[o + 7])
+__device__ __forceinline__ void tm_wait(uint32_t (&r)[16]) { asm volatile("tcgen05.wait::ld.sync.aligned;" : KT_W8(r, 0), KT_W8(r, 8)::"memory"); }
+__device__ __forceinline__ void tm_wait(uint32_t (&r)[32]) {
+    asm volatile("tcgen05.wait::ld.sync.aligned;" : KT_W8(r, 0), KT_W8(r, 8), KT_W8(r, 16), KT_W8(r, 24)::"memory");
+}
 __device__ __forceinline__ void tm_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 __device__ __forceinline__ void tm_st32(uint32_t a, const uint32_t (&r)[32]) {
     asm volatile(
@@ -173,7 +180,7 @@ template <bool EDGE> __device__ __forceinline__ float tile_weights(uint32_t sp, 
     for (int h = 0; h < KT_KEYS; h += 32) {
         uint32_t x[32];
         tm_ld32(sp + h, x);
-        tm_wait_ld();
+        tm_wait(x);
         float u[4] = {mx, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
         for (int i = 0; i < 32; i += 2) {
@@ -188,11 +195,8 @@ template <bool EDGE> __device__ __forceinline__ float tile_weights(uint32_t sp, 
     m = mx;
     const Two ff = two(f, f), nb = two(-base, -base), minus = two(-1.f, -1.f);
     Two sum = two(0.f, 0.f), sum_b = sum;
-#pragma unroll 1
-    for (int h = 0; h < KT_KEYS; h += 16) {
-        uint32_t x[16], p[16];
-        tm_ld16(sp + h, x);
-        tm_wait_ld();
+    auto weigh = [&](const uint32_t (&x)[16], int h) {
+        uint32_t p[16];
 #pragma unroll
         for (int i = 0; i < 16; i += 2) {
             const float2 y = parts(fma2(two(x[i], x[i + 1]), ff, nb));
@@ -212,6 +216,24 @@ template <bool EDGE> __device__ __forceinline__ float tile_weights(uint32_t sp, 
             p[8 + i / 2] = *reinterpret_cast<const uint32_t*>(&lo);
         }
         tm_st16(sp + h, p);
+    };
+    // The next 16 scores are on their way while 16 are worked on. No load is under way where the loop turns: what a loop
+    // carries may be copied there, before the load has come in.
+#pragma unroll 1
+    for (int h = 0; h < KT_KEYS; h += 64) {
+        uint32_t xa[16], xb[16], xc[16], xd[16];
+        tm_ld16(sp + h, xa);
+        tm_wait(xa);
+        tm_ld16(sp + h + 16, xb);
+        weigh(xa, h);
+        tm_wait(xb);
+        tm_ld16(sp + h + 32, xc);
+        weigh(xb, h + 16);
+        tm_wait(xc);
+        tm_ld16(sp + h + 48, xd);
+        weigh(xc, h + 32);
+        tm_wait(xd);
+        weigh(xd, h + 48);
     }
     const float2 t = parts(add2(sum, sum_b));
     l = l * corr + (t.x + t.y);
@@ -325,7 +347,7 @@ __global__ void __launch_bounds__(KT_THREADS, 1) k_kv_attn_tile(const __grid_con
                     if (!ok) break;
                 }
                 const int key0 = b.kb + n * KT_KEYS;
-                const int box = min(a.rows.page, KT_KEYS), boxes = (min(KT_KEYS, b.vis - key0) + box - 1) / box;  // pages with visible keys
+                const int box = min(a.rows.page, 64), boxes = (min(KT_KEYS, b.vis - key0) + box - 1) / box;  // pages with visible keys
                 if (lane == 0) bar_expect(bars->full + slot, uint32_t(boxes * box * 128 * 2 * PL));
                 __syncwarp();
                 if (lane < boxes * 2 * PL) {  // a lane per (page, half, plane)
@@ -356,7 +378,7 @@ __global__ void __launch_bounds__(KT_THREADS, 1) k_kv_attn_tile(const __grid_con
                 if (ok) ok = warp_wait(bars->full + slot, phase, bars);
                 if (!ok) return;
                 after_sync();
-                const uint32_t d = 128 + (n & 1) * 64, k = ring_k + slot * (S::SLOT >> 4);
+                const uint32_t d = 128 + (n & 1) * 128, k = ring_k + slot * (S::SLOT >> 4);
                 if (elect()) {
 #pragma unroll
                     for (int ks = 0; ks < 8; ++ks) {
@@ -379,9 +401,10 @@ __global__ void __launch_bounds__(KT_THREADS, 1) k_kv_attn_tile(const __grid_con
                 const int w = n & 1;
                 ok = warp_wait(bars->p_full + w, (n >> 1) & 1, bars) && warp_wait(bars->full + slot, phase, bars);
                 if (ok && n >= edge0) ok = warp_wait(bars->edge + (n - edge0), 0, bars);
+                if (ok && n > 0) ok = warp_wait(&bars->o_free, (n - 1) & 1, bars);
                 if (!ok) break;
                 after_sync();
-                const uint32_t d = 256 + w * 128, p = 128 + w * 64, v = ring_v + slot * (S::SLOT >> 4);
+                const uint32_t d = 384, p = 128 + w * 128, v = ring_v + slot * (S::SLOT >> 4);
                 const int steps = min(KT_KEYS / 16, (b.vis - (b.kb + n * KT_KEYS) + 15) / 16);
                 if (elect()) {
 #pragma unroll
@@ -417,6 +440,7 @@ __global__ void __launch_bounds__(KT_THREADS, 1) k_kv_attn_tile(const __grid_con
         if (tid == 0) {
             for (int s = 0; s < S::SLOTS; ++s) { bar_init(bars->full + s, 1); bar_init(bars->empty + s, 1); }
             for (int w = 0; w < 2; ++w) { bar_init(bars->s_full + w, 1); bar_init(bars->p_full + w, 4); bar_init(bars->o_full + w, 1); }
+            bar_init(&bars->o_free, 4);
             bar_init(&bars->q_full, 8);
             for (int k = 0; k < KT_MAXEDGE; ++k) bar_init(bars->edge + k, 1);
             asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -462,7 +486,7 @@ __global__ void __launch_bounds__(KT_THREADS, 1) k_kv_attn_tile(const __grid_con
             float m = -INFINITY, l = 0.f;
 #pragma unroll
             for (int d = 0; d < KV_D / 2; ++d) O[d] = two(0.f, 0.f);
-            const uint32_t sp = mine + 128 + team * 64, so = mine + 256 + team * 128;
+            const uint32_t sp = mine + 128 + team * 128, so = mine + 384;
 #pragma unroll 1
             for (int n = team; n < N; n += 2) {
                 ok = warp_wait(bars->s_full + team, (n >> 1) & 1, bars);
@@ -510,7 +534,7 @@ __global__ void __launch_bounds__(KT_THREADS, 1) k_kv_attn_tile(const __grid_con
                 before_sync();
                 __syncwarp();
                 if (lane == 0) bar_arrive(bars->p_full + team);
-                ok = warp_wait(bars->o_full + team, (n >> 1) & 1, bars);
+                ok = warp_wait(bars->o_full + team, (n >> 1) & 1, bars);  // (a barrier per team: a wait that skips phases would take an old one for its own)
                 if (!ok) break;
                 after_sync();
                 if (!odd) {  // the next 32 sums are on their way while these are added
@@ -519,13 +543,15 @@ __global__ void __launch_bounds__(KT_THREADS, 1) k_kv_attn_tile(const __grid_con
                     tm_ld32(so, x[0]);
 #pragma unroll
                     for (int h = 0; h < 4; ++h) {
-                        tm_wait_ld();
+                        tm_wait(x[h & 1]);
                         if (h < 3) tm_ld32(so + h * 32 + 32, x[(h + 1) & 1]);
 #pragma unroll
                         for (int i = 0; i < 32; i += 2) O[h * 16 + i / 2] = fma2(O[h * 16 + i / 2], cc, two(x[h & 1][i], x[h & 1][i + 1]));
                     }
                 }
                 before_sync();
+                __syncwarp();
+                if (lane == 0) bar_arrive(&bars->o_free);
             }
             // the teams' results: through shared memory (the ring is used up once both are here)
             ex[256 + (team * 128 + r) * 2] = m;
@@ -573,6 +599,7 @@ __global__ void __launch_bounds__(KT_THREADS, 1) k_kv_attn_tile(const __grid_con
         if (tid == 0) {
             for (int s = 0; s < S::SLOTS; ++s) { bar_inval(bars->full + s); bar_inval(bars->empty + s); }
             for (int w = 0; w < 2; ++w) { bar_inval(bars->s_full + w); bar_inval(bars->p_full + w); bar_inval(bars->o_full + w); }
+            bar_inval(&bars->o_free);
             bar_inval(&bars->q_full);
             for (int k = 0; k < KT_MAXEDGE; ++k) bar_inval(bars->edge + k);
         }
