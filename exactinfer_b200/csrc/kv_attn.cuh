@@ -33,6 +33,10 @@ __device__ __forceinline__ float ex2(float x) {
     return y;
 }
 
+__device__ __forceinline__ void cp16z(uint32_t dst, const void* src, bool on) {  // zeros when off
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(on ? 16 : 0) : "memory");
+}
+
 // (x, y) -> two packed fp16 and what they leave, packed; a remainder of an infinity is 0
 __device__ __forceinline__ void half_pair(float x, float y, uint32_t& hi, uint32_t& lo) {
     const __half2 h = __floats2half2_rn(x, y);

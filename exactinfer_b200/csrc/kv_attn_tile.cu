@@ -40,11 +40,12 @@ template <int PL> struct TileShape {
     static constexpr int SLOTS = 6 / PL;
     static constexpr int RING = SLOTS * SLOT;
     static constexpr int SMEM = RING + 4096 + 1024;
-    static_assert(RING >= KT_ROWS * KT_LD * 4, "the teams' sums take the place of the ring");
+    static constexpr int Q_STAGE = RING - KT_ROWS * KT_LD * 4;  // the queries pass through the end of the ring
+    static_assert(RING >= 2 * KT_ROWS * KT_LD * 4, "the teams' sums take the place of the ring");
 };
 
 struct TileBars {
-    uint64_t full[6], empty[6], s_full[2], p_full[2], o_full[2], o_free, q_full, edge[KT_MAXEDGE];
+    uint64_t full[6], empty[6], s_full[2], pv_ready[2], o_full[2], q_full, edge[KT_MAXEDGE];
     uint32_t tmem;
     int odd[KT_MAXEDGE];  // edge tile k has infinities or NaN among its values
     int fail;
@@ -87,6 +88,8 @@ template <bool ADD> __device__ __forceinline__ void mma_ts(uint32_t d, uint32_t 
                  " tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], db, %4, p;\n}\n"
                  ::"r"(d), "r"(a), "r"(b), "r"(b_hi), "r"(idesc), "n"(int(ADD)) : "memory");
 }
+// a value that every lane of a warp has: the compiler then knows, and keeps loops and MMA operands in uniform registers
+__device__ __forceinline__ int uniform(int x) { return __shfl_sync(0xffffffffu, x, 0); }
 __device__ __forceinline__ bool elect() {
     uint32_t p;
     asm volatile("{\n .reg .pred p;\n elect.sync _|p, 0xffffffff;\n selp.u32 %0, 1, 0, p;\n}\n" : "=r"(p));
@@ -157,6 +160,11 @@ __device__ __forceinline__ float2 parts(Two x) {
 __device__ __forceinline__ Two fma2(Two a, Two b, Two c) {
     Two r;
     asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+    return r;
+}
+__device__ __forceinline__ Two mul2(Two a, Two b) {
+    Two r;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
     return r;
 }
 __device__ __forceinline__ Two add2(Two a, Two b) {
@@ -241,6 +249,16 @@ template <bool EDGE> __device__ __forceinline__ float tile_weights(uint32_t sp, 
     return corr;
 }
 
+// consecutive rows of a tile: row, its token and its head among the group's (one division for all of them)
+struct RowWalk {
+    int row, token, head;
+    __device__ __forceinline__ RowWalk(int r, int group) : row(r), token(r / group), head(r % group) {}
+    __device__ __forceinline__ void step(int group) {
+        ++row;
+        if (++head == group) { head = 0; ++token; }
+    }
+};
+
 // What a CTA works on
 struct TileJob {
     int s, j, i, c, kb, ke, vis, vis_min, tiles, edge0;
@@ -256,7 +274,7 @@ __global__ void __launch_bounds__(KT_THREADS, 1) k_kv_attn_tile(const __grid_con
     uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(tile_raw) + 1023) & ~uintptr_t(1023));
     TileBars* bars = reinterpret_cast<TileBars*>(smem + S::RING);
     float* ex = reinterpret_cast<float*>(smem + S::RING + 1024);  // [2][128] x 2 words between the teams
-    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    const int tid = threadIdx.x, warp = uniform(tid >> 5), lane = tid & 31;
     TileJob b;
     {   // block -> (tile, sequence, key head, split): the last tiles, which see most, first; splits fastest
         int64_t x = blockIdx.x;
@@ -268,7 +286,7 @@ __global__ void __launch_bounds__(KT_THREADS, 1) k_kv_attn_tile(const __grid_con
         b.i = a.tiles_max - 1 - int(x / a.rows.n_seq);
     }
     b.sq = kv_seq(a.rows, b.s);
-    const int nrows = b.sq.nq * a.group;
+    const int nrows = uniform(b.sq.nq * a.group);
     if (b.i * KT_ROWS >= nrows) return;
     if (warp == 9) {
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(su32(&bars->tmem)) : "memory");
@@ -282,14 +300,14 @@ __global__ void __launch_bounds__(KT_THREADS, 1) k_kv_attn_tile(const __grid_con
             if (b.i * KT_ROWS >= nrows) return false;
             b.cut = a.splits > 1 && b.i < a.tiles_max;
             if (!b.cut && b.c) return false;
-            b.vis = kv_visible(a.rows, b.sq, min(((b.i + 1) * KT_ROWS - 1) / a.group, b.sq.nq - 1));
-            b.vis_min = kv_visible(a.rows, b.sq, b.i * KT_ROWS / a.group);
+            b.vis = uniform(kv_visible(a.rows, b.sq, min(((b.i + 1) * KT_ROWS - 1) / a.group, b.sq.nq - 1)));
+            b.vis_min = uniform(kv_visible(a.rows, b.sq, b.i * KT_ROWS / a.group));
             b.kb = b.cut ? b.c * a.chunk : 0;
             b.ke = b.cut && b.c < a.splits - 1 ? min(b.vis, b.kb + a.chunk) : b.vis;
             if (b.c && b.kb >= b.ke) continue;  // nothing here; the join does not look at it
-            b.tiles = max(0, (b.ke - b.kb + KT_KEYS - 1) / KT_KEYS);
+            b.tiles = uniform(max(0, (b.ke - b.kb + KT_KEYS - 1) / KT_KEYS));
             // edge tiles: those with keys that not every row sees, and a last one that ends inside (at most 3)
-            b.edge0 = max(0, min(b.vis_min, b.vis / KT_KEYS * KT_KEYS) - b.kb) / KT_KEYS;
+            b.edge0 = uniform(max(0, min(b.vis_min, b.vis / KT_KEYS * KT_KEYS) - b.kb) / KT_KEYS);
             return true;
         }
     };
@@ -341,6 +359,10 @@ __global__ void __launch_bounds__(KT_THREADS, 1) k_kv_attn_tile(const __grid_con
                 const int n = is_v ? (e == 2 * N - 1 ? N - 1 : e / 2 - 1) : (e + 1) / 2;
                 const int slot = e % S::SLOTS;
                 const uint32_t parity = ((e / S::SLOTS) & 1) ^ 1;
+                if (e < S::SLOTS && (slot + 1) * S::SLOT > S::Q_STAGE) {  // the queries pass through here first
+                    ok = warp_wait(&bars->q_full, 0, bars);
+                    if (!ok) break;
+                }
                 if (!__all_sync(0xffffffffu, bar_try(bars->empty + slot, parity))) {
                     search(min(v_issued, N));  // the slot may be waiting for this
                     if (ok) ok = warp_wait(bars->empty + slot, parity, bars);
@@ -375,9 +397,6 @@ __global__ void __launch_bounds__(KT_THREADS, 1) k_kv_attn_tile(const __grid_con
             };
             ok = warp_wait(&bars->q_full, 0, bars);
             auto scores = [&](int n) {
-                if (ok) ok = warp_wait(bars->full + slot, phase, bars);
-                if (!ok) return;
-                after_sync();
                 const uint32_t d = 128 + (n & 1) * 128, k = ring_k + slot * (S::SLOT >> 4);
                 if (elect()) {
 #pragma unroll
@@ -395,13 +414,20 @@ __global__ void __launch_bounds__(KT_THREADS, 1) k_kv_attn_tile(const __grid_con
                 __syncwarp();
                 next();
             };
-            scores(0);
-            if (N > 1) scores(1);
+            for (int n = 0; n < min(N, 2) && ok; ++n) {
+                ok = warp_wait(bars->full + slot, phase, bars);
+                after_sync();
+                if (ok) scores(n);
+            }
+            // An MMA is issued about when it starts, so every wait between two of them is time that the tensor core stands still: what
+            // can be waited for ahead is, and the last wait before a product is a single one, for the weights and for O being free.
             for (int n = 0; n < N && ok; ++n) {
                 const int w = n & 1;
-                ok = warp_wait(bars->p_full + w, (n >> 1) & 1, bars) && warp_wait(bars->full + slot, phase, bars);
+                const bool more = n + 2 < N;
+                ok = warp_wait(bars->full + slot, phase, bars);
+                if (ok && PL == 1 && more) ok = warp_wait(bars->full + (slot + 1 == S::SLOTS ? 0 : slot + 1), slot + 1 == S::SLOTS ? phase ^ 1 : phase, bars);
                 if (ok && n >= edge0) ok = warp_wait(bars->edge + (n - edge0), 0, bars);
-                if (ok && n > 0) ok = warp_wait(&bars->o_free, (n - 1) & 1, bars);
+                if (ok) ok = warp_wait(bars->pv_ready + w, (n >> 1) & 1, bars);
                 if (!ok) break;
                 after_sync();
                 const uint32_t d = 384, p = 128 + w * 128, v = ring_v + slot * (S::SLOT >> 4);
@@ -424,7 +450,13 @@ __global__ void __launch_bounds__(KT_THREADS, 1) k_kv_attn_tile(const __grid_con
                 }
                 __syncwarp();
                 next();
-                if (n + 2 < N) scores(n + 2);
+                if (more) {
+                    if (PL == 2) {  // (three slots: its load has waited for the product before this one)
+                        ok = warp_wait(bars->full + slot, phase, bars);
+                        after_sync();
+                    }
+                    if (ok) scores(n + 2);
+                }
             }
         }
         __syncwarp();
@@ -439,8 +471,7 @@ __global__ void __launch_bounds__(KT_THREADS, 1) k_kv_attn_tile(const __grid_con
         const int N = b.tiles, edge0 = b.edge0;
         if (tid == 0) {
             for (int s = 0; s < S::SLOTS; ++s) { bar_init(bars->full + s, 1); bar_init(bars->empty + s, 1); }
-            for (int w = 0; w < 2; ++w) { bar_init(bars->s_full + w, 1); bar_init(bars->p_full + w, 4); bar_init(bars->o_full + w, 1); }
-            bar_init(&bars->o_free, 4);
+            for (int w = 0; w < 2; ++w) { bar_init(bars->s_full + w, 1); bar_init(bars->pv_ready + w, 8); bar_init(bars->o_full + w, 1); }
             bar_init(&bars->q_full, 8);
             for (int k = 0; k < KT_MAXEDGE; ++k) bar_init(bars->edge + k, 1);
             asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -452,41 +483,58 @@ __global__ void __launch_bounds__(KT_THREADS, 1) k_kv_attn_tile(const __grid_con
             const int team = warp >> 2, r = (warp & 3) * 32 + lane, row = b.i * KT_ROWS + r;
             const uint32_t mine = uint32_t((warp & 3) * 32) << 16;  // (all 512 columns are this CTA's: they start at 0)
             const bool real = row < nrows;
-            const int token = real ? row / a.group : 0, head = b.j * a.group + row % a.group;
-            const int see = real ? kv_visible(a.rows, b.sq, token) : b.vis;
+            const int see = real ? kv_visible(a.rows, b.sq, row / a.group) : b.vis;
+            // queries: a warp copies 16 whole rows into the end of the ring, then every thread takes half of its row to tensor
+            // memory as hi | lo (a thread per row straight from global memory: 10000 clocks)
+            const RowWalk first(b.i * KT_ROWS + warp * 16, a.group);
+            float* qs = reinterpret_cast<float*>(smem + S::Q_STAGE);  // [row][KT_LD]
+            {
+                RowWalk w = first;
+#pragma unroll 4
+                for (int q = 0; q < 16; ++q, w.step(a.group)) {
+                    const bool on = w.row < nrows;
+                    cp16z(su32(qs + (warp * 16 + q) * KT_LD + lane * 4),
+                          on ? a.q + (b.sq.row0 + w.token) * a.ldq + (b.j * a.group + w.head) * KV_D + lane * 4 : a.q, on);
+                }
+                asm volatile("cp.async.commit_group;\n cp.async.wait_group 0;" ::: "memory");
+            }
+            asm volatile("bar.sync 1, 256;" ::: "memory");
             float f;
-            {   // queries: this team brings 64 of the 128 values of every row
-                float4 q[16];
-                const float4* src = reinterpret_cast<const float4*>(a.q + (b.sq.row0 + token) * a.ldq + head * KV_D + team * 64);
-                float m = 0.f;
+            {
+                float4 x[16];
+                float mx = 0.f;
 #pragma unroll
                 for (int u = 0; u < 16; ++u) {
-                    q[u] = real ? __ldg(src + u) : make_float4(0.f, 0.f, 0.f, 0.f);
-                    m = fmaxf(m, fmaxf(fmaxf(fabsf(q[u].x), fabsf(q[u].y)), fmaxf(fabsf(q[u].z), fabsf(q[u].w))));
+                    x[u] = *reinterpret_cast<const float4*>(qs + r * KT_LD + team * 64 + 4 * u);
+                    mx = max3(mx, max3(fabsf(x[u].x), fabsf(x[u].y), fabsf(x[u].z)), fabsf(x[u].w));
                 }
-                ex[team * 128 + r] = m;
+                ex[team * 128 + r] = mx;
                 asm volatile("bar.sync 1, 256;" ::: "memory");
                 const RowScale rs = row_scale(fmaxf(ex[r], ex[128 + r]), fabsf(a.scale2));  // (a negative scale goes into the queries)
                 f = rs.f;
-                const float sg = a.scale2 < 0.f ? -1.f : 1.f;
+                const float s1 = a.scale2 < 0.f ? -rs.up.s1 : rs.up.s1;
+                const Two k1 = two(s1, s1), k2 = two(rs.up.s2, rs.up.s2);
                 uint32_t hi[32], lo[32];
 #pragma unroll
                 for (int u = 0; u < 16; ++u) {
-                    half_pair(q[u].x * sg * rs.up.s1 * rs.up.s2, q[u].y * sg * rs.up.s1 * rs.up.s2, hi[2 * u], lo[2 * u]);
-                    half_pair(q[u].z * sg * rs.up.s1 * rs.up.s2, q[u].w * sg * rs.up.s1 * rs.up.s2, hi[2 * u + 1], lo[2 * u + 1]);
+                    const float2 y = parts(mul2(mul2(two(x[u].x, x[u].y), k1), k2)), z = parts(mul2(mul2(two(x[u].z, x[u].w), k1), k2));
+                    half_pair_finite(y.x, y.y, hi[2 * u], lo[2 * u]);  // (an infinity becomes infinity and NaN: its row is NaN either way)
+                    half_pair_finite(z.x, z.y, hi[2 * u + 1], lo[2 * u + 1]);
                 }
                 tm_st32(mine + team * 32, hi);
                 tm_st32(mine + 64 + team * 32, lo);
-                tm_wait_st();
-                before_sync();
-                __syncwarp();
-                if (lane == 0) bar_arrive(&bars->q_full);
             }
+            tm_wait_st();
+            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");  // TMA may write here now
+            before_sync();
+            __syncwarp();
+            if (lane == 0) bar_arrive(&bars->q_full);
             Two O[KV_D / 2];
             float m = -INFINITY, l = 0.f;
 #pragma unroll
             for (int d = 0; d < KV_D / 2; ++d) O[d] = two(0.f, 0.f);
             const uint32_t sp = mine + 128 + team * 128, so = mine + 384;
+            if (team == 1 && lane == 0) bar_arrive(bars->pv_ready);  // O is free at first
 #pragma unroll 1
             for (int n = team; n < N; n += 2) {
                 ok = warp_wait(bars->s_full + team, (n >> 1) & 1, bars);
@@ -533,7 +581,7 @@ __global__ void __launch_bounds__(KT_THREADS, 1) k_kv_attn_tile(const __grid_con
                 }
                 before_sync();
                 __syncwarp();
-                if (lane == 0) bar_arrive(bars->p_full + team);
+                if (lane == 0) bar_arrive(bars->pv_ready + team);
                 ok = warp_wait(bars->o_full + team, (n >> 1) & 1, bars);  // (a barrier per team: a wait that skips phases would take an old one for its own)
                 if (!ok) break;
                 after_sync();
@@ -551,7 +599,7 @@ __global__ void __launch_bounds__(KT_THREADS, 1) k_kv_attn_tile(const __grid_con
                 }
                 before_sync();
                 __syncwarp();
-                if (lane == 0) bar_arrive(&bars->o_free);
+                if (lane == 0) bar_arrive(bars->pv_ready + (team ^ 1));  // O is free for the other team's next product
             }
             // the teams' results: through shared memory (the ring is used up once both are here)
             ex[256 + (team * 128 + r) * 2] = m;
@@ -562,34 +610,28 @@ __global__ void __launch_bounds__(KT_THREADS, 1) k_kv_attn_tile(const __grid_con
             const float den = k0 * l0 + k1 * l1, k = team ? k1 : k0;
             const bool final_here = !b.cut || b.vis <= a.chunk;
             const float inv = final_here ? (den == 0.f ? 0.f : 1.f / den) : 1.f;
-            float4* stage = reinterpret_cast<float4*>(reinterpret_cast<float*>(smem) + r * KT_LD);
-            if (team == 1) {
+            float* stage = reinterpret_cast<float*>(smem);  // [team][row][KT_LD]
+            float4* own_row = reinterpret_cast<float4*>(stage + (team * KT_ROWS + r) * KT_LD);
+            const float ki = k * inv;
 #pragma unroll
-                for (int d = 0; d < KV_D; d += 4) {
-                    const float2 x = parts(O[d / 2]), y = parts(O[d / 2 + 1]);
-                    stage[d / 4] = make_float4(x.x * k, x.y * k, y.x * k, y.y * k);
-                }
-            }
-            asm volatile("bar.sync 1, 256;" ::: "memory");
-            if (team == 0) {
-#pragma unroll
-                for (int d = 0; d < KV_D; d += 4) {
-                    const float4 u = stage[d / 4];
-                    const float2 x = parts(O[d / 2]), y = parts(O[d / 2 + 1]);
-                    stage[d / 4] = make_float4((x.x * k + u.x) * inv, (x.y * k + u.y) * inv, (y.x * k + u.z) * inv, (y.y * k + u.w) * inv);
-                }
+            for (int d = 0; d < KV_D; d += 4) {
+                const float2 x = parts(O[d / 2]), y = parts(O[d / 2 + 1]);
+                own_row[d / 4] = make_float4(x.x * ki, x.y * ki, y.x * ki, y.y * ki);
             }
             const int64_t slot = ((int64_t(b.s) * a.tiles_max + b.i) * a.HKV + b.j) * a.splits + b.c;
             float* part = a.part + slot * KT_ROWS * (KV_D + 2);
             if (!final_here && team == 0) { part[KT_ROWS * KV_D + r] = M; part[KT_ROWS * (KV_D + 1) + r] = den; }
             asm volatile("bar.sync 1, 256;" ::: "memory");
-            if (ok)
-                for (int q = warp; q < KT_ROWS && b.i * KT_ROWS + q < nrows; q += 8) {
-                    const int rw = b.i * KT_ROWS + q;
-                    const float4 u = *reinterpret_cast<const float4*>(reinterpret_cast<float*>(smem) + q * KT_LD + lane * 4);
-                    float* dst = final_here ? a.out + (b.sq.row0 + rw / a.group) * a.ldo + (b.j * a.group + rw % a.group) * KV_D : part + q * KV_D;
-                    *reinterpret_cast<float4*>(dst + lane * 4) = u;
+            if (ok) {
+                RowWalk w = first;
+#pragma unroll 4
+                for (int q = warp * 16; q < warp * 16 + 16; ++q, w.step(a.group)) {
+                    const float4 x = *reinterpret_cast<const float4*>(stage + q * KT_LD + lane * 4);
+                    const float4 y = *reinterpret_cast<const float4*>(stage + (KT_ROWS + q) * KT_LD + lane * 4);
+                    float* dst = final_here ? a.out + (b.sq.row0 + w.token) * a.ldo + (b.j * a.group + w.head) * KV_D : part + q * KV_D;
+                    if (w.row < nrows) *reinterpret_cast<float4*>(dst + lane * 4) = make_float4(x.x + y.x, x.y + y.y, x.z + y.z, x.w + y.w);
                 }
+            }
         }
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");  // the ring is written by TMA again
         before_sync();
@@ -598,8 +640,7 @@ __global__ void __launch_bounds__(KT_THREADS, 1) k_kv_attn_tile(const __grid_con
         if (bars->fail) break;
         if (tid == 0) {
             for (int s = 0; s < S::SLOTS; ++s) { bar_inval(bars->full + s); bar_inval(bars->empty + s); }
-            for (int w = 0; w < 2; ++w) { bar_inval(bars->s_full + w); bar_inval(bars->p_full + w); bar_inval(bars->o_full + w); }
-            bar_inval(&bars->o_free);
+            for (int w = 0; w < 2; ++w) { bar_inval(bars->s_full + w); bar_inval(bars->pv_ready + w); bar_inval(bars->o_full + w); }
             bar_inval(&bars->q_full);
             for (int k = 0; k < KT_MAXEDGE; ++k) bar_inval(bars->edge + k);
         }
