@@ -12,7 +12,7 @@
 // Two teams of four warps work on alternate key tiles, a thread per query row (= TMEM lane), each with its own running
 // maximum, denominator and 128 sums, joined once at the end: while one team forms its weights, the tensor core
 // multiplies for the other. One warp brings keys and values by TMA, page by page, into a ring of 128-key tiles in the
-// order of their use; one thread issues the MMAs. TMEM: Q hi | lo (128 columns, the A operand of S: read from there, the
+// order of their use; two warps issue the MMAs, one searches the values. TMEM: Q hi | lo (128 columns, the A operand of S: read from there, the
 // shared memory has only K to deliver), per team S (128 columns, overwritten by the weights hi | lo, the A operand of O) and one
 // O (128): a team takes it into its registers while the tensor core forms the next S. V lies [key][dimension] as in the page and is a B operand with N along the rows.
 // A tile's 128 keys take 2048 (F16) or 3 * 1024 (pairs) clocks of the tensor pipe. (64-key tiles: an MMA with N = 64 took 51
@@ -45,7 +45,7 @@ template <int PL> struct TileShape {
 };
 
 struct TileBars {
-    uint64_t full[6], empty[6], s_full[2], pv_ready[2], o_full[2], q_full, edge[KT_MAXEDGE];
+    uint64_t full[6], empty[6], s_full[2], pv_ready[2], o_full[2], q_full, go[KT_MAXEDGE], edge[KT_MAXEDGE];
     uint32_t tmem;
     int odd[KT_MAXEDGE];  // edge tile k has infinities or NaN among its values
     int fail;
@@ -192,13 +192,13 @@ template <bool EDGE> __device__ __forceinline__ float tile_weights(uint32_t sp, 
         float u[4] = {mx, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
         for (int i = 0; i < 32; i += 2) {
-            const float x0 = EDGE && h + i >= left ? -INFINITY : __uint_as_float(x[i]);
-            const float x1 = EDGE && h + i + 1 >= left ? -INFINITY : __uint_as_float(x[i + 1]);
+            const float x0 = EDGE && i >= left - h ? -INFINITY : __uint_as_float(x[i]);
+            const float x1 = EDGE && i + 1 >= left - h ? -INFINITY : __uint_as_float(x[i + 1]);
             u[(i >> 1) & 3] = max3(u[(i >> 1) & 3], x0, x1);
         }
         mx = fmaxf(max3(u[0], u[1], u[2]), u[3]);
     }
-    mx = fmaxf(m, mx == -INFINITY ? -INFINITY : mx * f);
+    mx = fmaxf(m, mx * f);
     const float corr = mx == -INFINITY ? 1.f : ex2(m - mx), base = mx == -INFINITY ? 0.f : mx - KA_P;
     m = mx;
     const Two ff = two(f, f), nb = two(-base, -base), minus = two(-1.f, -1.f);
@@ -207,12 +207,9 @@ template <bool EDGE> __device__ __forceinline__ float tile_weights(uint32_t sp, 
         uint32_t p[16];
 #pragma unroll
         for (int i = 0; i < 16; i += 2) {
-            const float2 y = parts(fma2(two(x[i], x[i + 1]), ff, nb));
-            float p0 = ex2(y.x), p1 = ex2(y.y);
-            if (EDGE) {
-                p0 = h + i < left && __uint_as_float(x[i]) != -INFINITY ? p0 : 0.f;
-                p1 = h + i + 1 < left && __uint_as_float(x[i + 1]) != -INFINITY ? p1 : 0.f;
-            }
+            const uint32_t x0 = EDGE && i >= left - h ? 0xff800000u : x[i], x1 = EDGE && i + 1 >= left - h ? 0xff800000u : x[i + 1];
+            const float2 y = parts(fma2(two(x0, x1), ff, nb));
+            const float p0 = ex2(y.x), p1 = ex2(y.y);
             const Two pp = two(p0, p1);
             if (i & 2) sum_b = add2(sum_b, pp);
             else sum = add2(sum, pp);
@@ -312,8 +309,9 @@ __global__ void __launch_bounds__(KT_THREADS, 1) k_kv_attn_tile(const __grid_con
         }
     };
     auto all_here = [] { asm volatile("bar.sync 0, %0;" ::"n"(KT_THREADS) : "memory"); };
-    // Ring elements in the order of use: K0, K1, V0, K2, V1, K3, V2, ...: V of tile n is element 2n + 2
+    // Ring elements in the order of use: K0, K1, V0, K2, V1, K3, V2, ...: K of tile n is element 2n - 1 (K0: 0), V is 2n + 2
     // (the last tile's one earlier: no K comes before it)
+    auto k_elem = [](int n) { return n == 0 ? 0 : 2 * n - 1; };
     auto v_elem = [&](int n) { return n == b.tiles - 1 ? 2 * n + 1 : 2 * n + 2; };
 
     if (warp >= 8) {
@@ -325,35 +323,7 @@ __global__ void __launch_bounds__(KT_THREADS, 1) k_kv_attn_tile(const __grid_con
         all_here();
         after_sync();
         if (warp == 8) {  // ---- keys and values
-            int searched = edge0;  // edge tiles before this one are done with
-            auto search = [&](int upto) {  // V of the edge tiles below `upto`: their loads are under way
-                for (; searched < upto && ok; ++searched) {
-                    const int e = v_elem(searched), key0 = b.kb + searched * KT_KEYS;
-                    ok = warp_wait(bars->full + e % S::SLOTS, (e / S::SLOTS) & 1, bars);
-                    if (!ok) break;
-                    uint8_t* v = smem + (e % S::SLOTS) * S::SLOT;
-                    const int have = min(KT_KEYS, b.vis - key0), up = (have + 15) / 16 * 16;
-                    for (int w = lane; w < (up - have) * 8 * 2 * PL; w += 32) {  // rows behind the last key
-                        const int part = w / ((up - have) * 8), rest = w % ((up - have) * 8);
-                        *reinterpret_cast<uint4*>(v + part * S::HALF + have * 128 + rest * 16) = make_uint4(0, 0, 0, 0);
-                    }
-                    uint32_t any = 0;
-                    if (b.vis_min < b.vis)
-                        for (int w = lane; w < have * 8 * 2 * PL; w += 32) {
-                            const int part = w / (have * 8), rest = w % (have * 8);
-                            const uint4 u = *reinterpret_cast<const uint4*>(v + part * S::HALF + rest * 16);
-                            for (uint32_t h : {u.x, u.y, u.z, u.w}) any |= uint32_t((h & 0x7c00u) == 0x7c00u) | uint32_t((h & 0x7c000000u) == 0x7c000000u);
-                        }
-                    const bool odd = __any_sync(0xffffffffu, any != 0);
-                    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-                    __syncwarp();
-                    if (lane == 0) {
-                        bars->odd[searched - edge0] = odd;
-                        bar_arrive(bars->edge + (searched - edge0));
-                    }
-                }
-            };
-            int v_issued = 0, issued = 0;
+            int issued = 0;
             for (int e = 0; e < 2 * N && ok; ++e) {
                 const bool is_v = e == 2 * N - 1 || (e >= 2 && e % 2 == 0);
                 const int n = is_v ? (e == 2 * N - 1 ? N - 1 : e / 2 - 1) : (e + 1) / 2;
@@ -363,11 +333,8 @@ __global__ void __launch_bounds__(KT_THREADS, 1) k_kv_attn_tile(const __grid_con
                     ok = warp_wait(&bars->q_full, 0, bars);
                     if (!ok) break;
                 }
-                if (!__all_sync(0xffffffffu, bar_try(bars->empty + slot, parity))) {
-                    search(min(v_issued, N));  // the slot may be waiting for this
-                    if (ok) ok = warp_wait(bars->empty + slot, parity, bars);
-                    if (!ok) break;
-                }
+                ok = warp_wait(bars->empty + slot, parity, bars);
+                if (!ok) break;
                 const int key0 = b.kb + n * KT_KEYS;
                 const int box = min(a.rows.page, 64), boxes = (min(KT_KEYS, b.vis - key0) + box - 1) / box;  // pages with visible keys
                 if (lane == 0) bar_expect(bars->full + slot, uint32_t(boxes * box * 128 * 2 * PL));
@@ -381,78 +348,108 @@ __global__ void __launch_bounds__(KT_THREADS, 1) k_kv_attn_tile(const __grid_con
                     tma_rows(su32(smem + slot * S::SLOT + pl * S::PLANE + half * S::HALF + q * box * 128), &map, half * 64, y, bars->full + slot);
                 }
                 ++issued;
-                if (is_v) v_issued = n + 1;
+                if (is_v && n >= edge0) {
+                    __syncwarp();
+                    if (lane == 0) bar_arrive(bars->go + (n - edge0));
+                }
             }
-            search(N);
             if (!ok)  // nothing may still be arriving when the CTA ends
                 for (int e = max(0, issued - S::SLOTS); e < issued; ++e)
                     for (unsigned it = 0; it < KT_SPIN && !bar_try(bars->full + e % S::SLOTS, (e / S::SLOTS) & 1); ++it) {}
-        } else if (warp == 9 && N > 0) {  // ---- MMA issuer: the whole warp walks the tiles, one lane issues
-            // (with all of it inside `if (lane == 0)` every operand went through a vector register: 100 clocks per MMA)
+        } else if (warp == 11) {  // ---- values of the edge tiles
+            for (int n = edge0; n < N && ok; ++n) {
+                const int e = v_elem(n), have = min(KT_KEYS, b.vis - (b.kb + n * KT_KEYS)), up = (have + 15) / 16 * 16;
+                // (a parity tells a phase from the one before it only: the slot's turn has come once its load is issued)
+                ok = warp_wait(bars->go + (n - edge0), 0, bars) && warp_wait(bars->full + e % S::SLOTS, (e / S::SLOTS) & 1, bars);
+                if (!ok) break;
+                uint8_t* v = smem + (e % S::SLOTS) * S::SLOT;
+                for (int part = 0; part < 2 * PL; ++part)  // rows behind the last key
+                    for (int w = lane; w < (up - have) * 8; w += 32) *reinterpret_cast<uint4*>(v + part * S::HALF + have * 128 + w * 16) = make_uint4(0, 0, 0, 0);
+                uint32_t any = 0;
+                if (b.vis_min < b.vis)
+                    for (int part = 0; part < 2 * PL; ++part)
+#pragma unroll 8
+                        for (int w = lane; w < KT_KEYS * 8; w += 32) {  // an exponent of all ones carries into the sign's place
+                            const uint4 u = *reinterpret_cast<const uint4*>(v + part * S::HALF + w * 16);
+                            const uint32_t c = (((u.x & 0x7c007c00u) + 0x04000400u) | ((u.y & 0x7c007c00u) + 0x04000400u) |
+                                                ((u.z & 0x7c007c00u) + 0x04000400u) | ((u.w & 0x7c007c00u) + 0x04000400u)) & 0x80008000u;
+                            any |= w < have * 8 ? c : 0u;
+                        }
+                const bool odd = __any_sync(0xffffffffu, any != 0);
+                asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+                __syncwarp();
+                if (lane == 0) {
+                    bars->odd[n - edge0] = odd;
+                    bar_arrive(bars->edge + (n - edge0));
+                }
+            }
+        } else {  // ---- MMA issuers, one per team: the whole warp walks the team's tiles, one lane issues
+            // (with all of it inside `if (lane == 0)` every operand went through a vector register: 100 clocks per MMA). An MMA is
+            // issued about when it starts, so a wait between two of them is time that the tensor core stands still: with an
+            // issuer per team one waits while the other's products run. O(n) and S(n + 2) follow one another without a wait.
             constexpr uint32_t id_s = idesc_f16(KT_KEYS, false), id_o = idesc_f16(KV_D, true);
+            const int w = warp - 9;
             const uint32_t ring_k = desc_lo(su32(smem), 0), ring_v = desc_lo(su32(smem), S::HALF);
-            uint32_t slot = 0, phase = 0;
-            auto next = [&]() {
-                if (++slot == S::SLOTS) { slot = 0; phase ^= 1; }
-            };
-            ok = warp_wait(&bars->q_full, 0, bars);
+            const uint32_t s_at = 128 + w * 128, o_at = 384;
             auto scores = [&](int n) {
-                const uint32_t d = 128 + (n & 1) * 128, k = ring_k + slot * (S::SLOT >> 4);
+                const int slot = k_elem(n) % S::SLOTS;
+                const uint32_t k = ring_k + slot * (S::SLOT >> 4);
                 if (elect()) {
 #pragma unroll
                     for (int ks = 0; ks < 8; ++ks) {
                         const uint32_t at = k + (ks >> 2) * (S::HALF >> 4) + (ks & 3) * 2;
-                        if (ks == 0) mma_ts<false>(d, 64, at, KT_DESC_HI, id_s);
-                        else mma_ts<true>(d, 64 + ks * 8, at, KT_DESC_HI, id_s);
-                        if (PL == 2) mma_ts<true>(d, ks * 8, at + (S::PLANE >> 4), KT_DESC_HI, id_s);
+                        if (ks == 0) mma_ts<false>(s_at, 64, at, KT_DESC_HI, id_s);
+                        else mma_ts<true>(s_at, 64 + ks * 8, at, KT_DESC_HI, id_s);
+                        if (PL == 2) mma_ts<true>(s_at, ks * 8, at + (S::PLANE >> 4), KT_DESC_HI, id_s);
                     }
 #pragma unroll
-                    for (int ks = 0; ks < 8; ++ks) mma_ts<true>(d, ks * 8, k + (ks >> 2) * (S::HALF >> 4) + (ks & 3) * 2, KT_DESC_HI, id_s);
+                    for (int ks = 0; ks < 8; ++ks) mma_ts<true>(s_at, ks * 8, k + (ks >> 2) * (S::HALF >> 4) + (ks & 3) * 2, KT_DESC_HI, id_s);
                     commit(bars->empty + slot);
-                    commit(bars->s_full + (n & 1));
+                    commit(bars->s_full + w);
                 }
                 __syncwarp();
-                next();
             };
-            for (int n = 0; n < min(N, 2) && ok; ++n) {
-                ok = warp_wait(bars->full + slot, phase, bars);
+            auto k_wait = [&](int n) {
+                const int e = k_elem(n);
+                return warp_wait(bars->full + e % S::SLOTS, (e / S::SLOTS) & 1, bars);
+            };
+            if (w < N) {
+                ok = warp_wait(&bars->q_full, 0, bars) && k_wait(w);
                 after_sync();
-                if (ok) scores(n);
+                if (ok) scores(w);
             }
-            // An MMA is issued about when it starts, so every wait between two of them is time that the tensor core stands still: what
-            // can be waited for ahead is, and the last wait before a product is a single one, for the weights and for O being free.
-            for (int n = 0; n < N && ok; ++n) {
-                const int w = n & 1;
+            for (int n = w; n < N && ok; n += 2) {
                 const bool more = n + 2 < N;
-                ok = warp_wait(bars->full + slot, phase, bars);
-                if (ok && PL == 1 && more) ok = warp_wait(bars->full + (slot + 1 == S::SLOTS ? 0 : slot + 1), slot + 1 == S::SLOTS ? phase ^ 1 : phase, bars);
+                const int e = v_elem(n), slot = e % S::SLOTS;
+                // A wait for a slot is good only when the load before it in that slot is known to have come in (a parity tells two
+                // neighbouring phases apart, no more). The weights being ready says so of every tile before this one.
+                ok = warp_wait(bars->pv_ready + w, (n >> 1) & 1, bars) && warp_wait(bars->full + slot, (e / S::SLOTS) & 1, bars);
+                if (ok && PL == 1 && more) ok = k_wait(n + 2);
                 if (ok && n >= edge0) ok = warp_wait(bars->edge + (n - edge0), 0, bars);
-                if (ok) ok = warp_wait(bars->pv_ready + w, (n >> 1) & 1, bars);
                 if (!ok) break;
                 after_sync();
-                const uint32_t d = 384, p = 128 + w * 128, v = ring_v + slot * (S::SLOT >> 4);
+                const uint32_t v = ring_v + slot * (S::SLOT >> 4);
                 const int steps = min(KT_KEYS / 16, (b.vis - (b.kb + n * KT_KEYS) + 15) / 16);
                 if (elect()) {
 #pragma unroll
                     for (int ks = 0; ks < KT_KEYS / 16; ++ks) {  // weights of 16 keys: 8 columns of hi, 8 of lo
                         if (ks >= steps) break;
-                        if (ks == 0) mma_ts<false>(d, p + 8, v, KT_DESC_HI, id_o);
-                        else mma_ts<true>(d, p + ks * 16 + 8, v + ks * 128, KT_DESC_HI, id_o);
-                        if (PL == 2) mma_ts<true>(d, p + ks * 16, v + (S::PLANE >> 4) + ks * 128, KT_DESC_HI, id_o);
+                        if (ks == 0) mma_ts<false>(o_at, s_at + 8, v, KT_DESC_HI, id_o);
+                        else mma_ts<true>(o_at, s_at + ks * 16 + 8, v + ks * 128, KT_DESC_HI, id_o);
+                        if (PL == 2) mma_ts<true>(o_at, s_at + ks * 16, v + (S::PLANE >> 4) + ks * 128, KT_DESC_HI, id_o);
                     }
 #pragma unroll
                     for (int ks = 0; ks < KT_KEYS / 16; ++ks) {
                         if (ks >= steps) break;
-                        mma_ts<true>(d, p + ks * 16, v + ks * 128, KT_DESC_HI, id_o);
+                        mma_ts<true>(o_at, s_at + ks * 16, v + ks * 128, KT_DESC_HI, id_o);
                     }
                     commit(bars->empty + slot);
                     commit(bars->o_full + w);
                 }
                 __syncwarp();
-                next();
                 if (more) {
                     if (PL == 2) {  // (three slots: its load has waited for the product before this one)
-                        ok = warp_wait(bars->full + slot, phase, bars);
+                        ok = k_wait(n + 2);
                         after_sync();
                     }
                     if (ok) scores(n + 2);
@@ -473,7 +470,7 @@ __global__ void __launch_bounds__(KT_THREADS, 1) k_kv_attn_tile(const __grid_con
             for (int s = 0; s < S::SLOTS; ++s) { bar_init(bars->full + s, 1); bar_init(bars->empty + s, 1); }
             for (int w = 0; w < 2; ++w) { bar_init(bars->s_full + w, 1); bar_init(bars->pv_ready + w, 8); bar_init(bars->o_full + w, 1); }
             bar_init(&bars->q_full, 8);
-            for (int k = 0; k < KT_MAXEDGE; ++k) bar_init(bars->edge + k, 1);
+            for (int k = 0; k < KT_MAXEDGE; ++k) { bar_init(bars->go + k, 1); bar_init(bars->edge + k, 1); }
             asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
         }
         before_sync();
@@ -511,7 +508,7 @@ __global__ void __launch_bounds__(KT_THREADS, 1) k_kv_attn_tile(const __grid_con
                 ex[team * 128 + r] = mx;
                 asm volatile("bar.sync 1, 256;" ::: "memory");
                 const RowScale rs = row_scale(fmaxf(ex[r], ex[128 + r]), fabsf(a.scale2));  // (a negative scale goes into the queries)
-                f = rs.f;
+                f = fmaxf(rs.f, 1e-37f);  // (0 would make NaN of the masked scores, which are -infinity; scores are below 2^39)
                 const float s1 = a.scale2 < 0.f ? -rs.up.s1 : rs.up.s1;
                 const Two k1 = two(s1, s1), k2 = two(rs.up.s2, rs.up.s2);
                 uint32_t hi[32], lo[32];
@@ -642,7 +639,7 @@ __global__ void __launch_bounds__(KT_THREADS, 1) k_kv_attn_tile(const __grid_con
             for (int s = 0; s < S::SLOTS; ++s) { bar_inval(bars->full + s); bar_inval(bars->empty + s); }
             for (int w = 0; w < 2; ++w) { bar_inval(bars->s_full + w); bar_inval(bars->pv_ready + w); bar_inval(bars->o_full + w); }
             bar_inval(&bars->q_full);
-            for (int k = 0; k < KT_MAXEDGE; ++k) bar_inval(bars->edge + k);
+            for (int k = 0; k < KT_MAXEDGE; ++k) { bar_inval(bars->go + k); bar_inval(bars->edge + k); }
         }
         }
     }
