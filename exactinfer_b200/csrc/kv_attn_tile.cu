@@ -282,13 +282,12 @@ __global__ void __launch_bounds__(KT_THREADS, 1) k_kv_attn_tile(const __grid_con
         b.s = int(x % a.rows.n_seq);
         b.i = a.tiles_max - 1 - int(x / a.rows.n_seq);
     }
-    b.sq = kv_seq(a.rows, b.s);
-    const int nrows = uniform(b.sq.nq * a.group);
-    if (b.i * KT_ROWS >= nrows) return;
     if (warp == 9) {
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(su32(&bars->tmem)) : "memory");
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
     }
+    b.sq = kv_seq(a.rows, b.s);
+    const int nrows = uniform(b.sq.nq * a.group);
     if (tid == 0) bars->fail = 0;
     bool ok = true;
     // the next tile of query rows of this CTA (more than one only when there are more rows than announced)
@@ -421,11 +420,18 @@ __global__ void __launch_bounds__(KT_THREADS, 1) k_kv_attn_tile(const __grid_con
             for (int n = w; n < N && ok; n += 2) {
                 const bool more = n + 2 < N;
                 const int e = v_elem(n), slot = e % S::SLOTS;
-                // A wait for a slot is good only when the load before it in that slot is known to have come in (a parity tells two
-                // neighbouring phases apart, no more). The weights being ready says so of every tile before this one.
-                ok = warp_wait(bars->pv_ready + w, (n >> 1) & 1, bars) && warp_wait(bars->full + slot, (e / S::SLOTS) & 1, bars);
-                if (ok && PL == 1 && more) ok = k_wait(n + 2);
-                if (ok && n >= edge0) ok = warp_wait(bars->edge + (n - edge0), 0, bars);
+                // Weights, values and (F16) the keys behind them in one wait, a lane each: a wait costs 200 clocks even when all
+                // is there. A wait for a slot is good only when the load before it in that slot is known to have come in (a parity
+                // tells two neighbouring phases apart, no more); the weights being ready says so, hence the second look at all.
+                {
+                    const int ek = k_elem(n + 2);
+                    uint64_t* bar = bars->pv_ready + w;
+                    uint32_t par = uint32_t(n >> 1) & 1;
+                    if (lane & 1) { bar = bars->full + slot; par = (e / S::SLOTS) & 1; }
+                    if (PL == 1 && more && (lane & 2)) { bar = bars->full + ek % S::SLOTS; par = (ek / S::SLOTS) & 1; }
+                    if (n >= edge0 && lane >= 16) { bar = bars->edge + (n - edge0); par = 0; }
+                    ok = warp_wait(bar, par, bars) && warp_wait(bar, par, bars);
+                }
                 if (!ok) break;
                 after_sync();
                 const uint32_t v = ring_v + slot * (S::SLOT >> 4);
@@ -466,6 +472,19 @@ __global__ void __launch_bounds__(KT_THREADS, 1) k_kv_attn_tile(const __grid_con
         asm volatile("setmaxnreg.inc.sync.aligned.u32 224;");
         for (; take(); b.i += a.tiles_max) {
         const int N = b.tiles, edge0 = b.edge0;
+            // queries: a warp copies 16 whole rows into the end of the ring, then every thread takes half of its row to tensor
+            // memory as hi | lo (a thread per row straight from global memory: 10000 clocks)
+            const RowWalk first(b.i * KT_ROWS + warp * 16, a.group);
+            float* qs = reinterpret_cast<float*>(smem + S::Q_STAGE);  // [row][KT_LD]
+            {
+                RowWalk w = first;
+#pragma unroll 4
+                for (int q = 0; q < 16; ++q, w.step(a.group)) {
+                    const bool on = w.row < nrows;
+                    cp16z(su32(qs + (warp * 16 + q) * KT_LD + lane * 4),
+                          on ? a.q + (b.sq.row0 + w.token) * a.ldq + (b.j * a.group + w.head) * KV_D + lane * 4 : a.q, on);
+                }
+            }
         if (tid == 0) {
             for (int s = 0; s < S::SLOTS; ++s) { bar_init(bars->full + s, 1); bar_init(bars->empty + s, 1); }
             for (int w = 0; w < 2; ++w) { bar_init(bars->s_full + w, 1); bar_init(bars->pv_ready + w, 8); bar_init(bars->o_full + w, 1); }
@@ -481,20 +500,7 @@ __global__ void __launch_bounds__(KT_THREADS, 1) k_kv_attn_tile(const __grid_con
             const uint32_t mine = uint32_t((warp & 3) * 32) << 16;  // (all 512 columns are this CTA's: they start at 0)
             const bool real = row < nrows;
             const int see = real ? kv_visible(a.rows, b.sq, row / a.group) : b.vis;
-            // queries: a warp copies 16 whole rows into the end of the ring, then every thread takes half of its row to tensor
-            // memory as hi | lo (a thread per row straight from global memory: 10000 clocks)
-            const RowWalk first(b.i * KT_ROWS + warp * 16, a.group);
-            float* qs = reinterpret_cast<float*>(smem + S::Q_STAGE);  // [row][KT_LD]
-            {
-                RowWalk w = first;
-#pragma unroll 4
-                for (int q = 0; q < 16; ++q, w.step(a.group)) {
-                    const bool on = w.row < nrows;
-                    cp16z(su32(qs + (warp * 16 + q) * KT_LD + lane * 4),
-                          on ? a.q + (b.sq.row0 + w.token) * a.ldq + (b.j * a.group + w.head) * KV_D + lane * 4 : a.q, on);
-                }
-                asm volatile("cp.async.commit_group;\n cp.async.wait_group 0;" ::: "memory");
-            }
+            asm volatile("cp.async.wait_all;" ::: "memory");
             asm volatile("bar.sync 1, 256;" ::: "memory");
             float f;
             {
@@ -666,8 +672,10 @@ TilePlan tile_plan(const Kv* kv, const elb_kv_batch* b, int n_head) {
     p.tiles = int((rows + KT_ROWS - 1) / KT_ROWS);
     const int64_t base = int64_t(b->n_seq) * kv->HKV * p.tiles;
     const int len = std::max(b->max_len, 1);
-    int64_t want = base >= 2 * kv->sm_count ? 1 : std::max<int64_t>(1, (int64_t(kv->sm_count) * (b->n_seq > 1 ? 4 : 1)) / base);
-    want = std::min<int64_t>(want, (len + 255) / 256);
+    // A CTA's start and end cost as much as 5 tiles of keys: one wave of long ranges when all sequences are alike, two when they may
+    // not be, and at least 4 tiles each (nine turns behind 203-4100 keys: four waves 90 us, two 60)
+    int64_t want = base >= 2 * kv->sm_count ? 1 : std::max<int64_t>(1, int64_t(kv->sm_count) * (b->n_seq > 1 ? 2 : 1) / base);
+    want = std::min<int64_t>(want, (len + 4 * KT_KEYS - 1) / (4 * KT_KEYS));
     p.chunk = int((len + want - 1) / want + KT_KEYS - 1) / KT_KEYS * KT_KEYS;
     p.splits = (len + p.chunk - 1) / p.chunk;
     return p;
