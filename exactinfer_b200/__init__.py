@@ -180,7 +180,7 @@ class Rope:
         self.config = rope_config(head_dim, **config)
         self.head_dim, h = head_dim, C.c_void_p()
         check(lib().elb_rope_create(device, C.byref(self.config), C.byref(h)))
-        self._h = h
+        self._h, self._destroy = h, lib().elb_rope_destroy
 
     def apply(self, x, pos, y, n: int, heads: int, ldx: int | None = None, ldy: int | None = None, norm=None, eps: float = 0.0, stream: int = 0):
         """y[n][heads] = x rotated at the positions pos[n] (elb_rope_dev); strides in floats, default the row's width."""
@@ -190,7 +190,7 @@ class Rope:
 
     def close(self):
         if getattr(self, "_h", None):
-            lib().elb_rope_destroy(self._h)
+            self._destroy(self._h)
             self._h = None
 
     def __del__(self):
@@ -214,7 +214,7 @@ class KvCache:
         h = C.c_void_p()
         self._mem, self.head_dim, self.n_head_kv = mem, head_dim, n_head_kv
         check(lib().elb_kv_create(device, n_layer, n_head_kv, head_dim, page, n_pages, type, _ptr(mem), C.byref(h)))
-        self._h = h
+        self._h, self._destroy = h, lib().elb_kv_destroy
 
     @staticmethod
     def bytes(n_layer: int, n_head_kv: int, page: int, n_pages: int, type: int = KV_F16, head_dim: int = 128) -> int:
@@ -249,7 +249,7 @@ class KvCache:
 
     def close(self):
         if getattr(self, "_h", None):
-            lib().elb_kv_destroy(self._h)
+            self._destroy(self._h)
             self._h = self._mem = None
 
     def __del__(self):

@@ -17,7 +17,7 @@ namespace elb {
 
 namespace {
 
-constexpr int RP_THREADS = 256, RP_TOKENS = 4, RP_MAXHALF = 128;
+constexpr int RP_THREADS = 256, RP_TOKENS = 4, RP_MAXHALF = 128, RP_BATCH = 4;
 
 struct RopeArgs {
     const double* turns;  // [half] or null: no rotation
@@ -109,66 +109,92 @@ __device__ __forceinline__ void fill_angles(const RopeArgs& a, int tokens, const
     }
 }
 
-// head_dim 32, 64, 128 or 256, dim a multiple of 8, rows on 16-byte boundaries; grid (token groups, head groups)
-__global__ void __launch_bounds__(RP_THREADS) k_rope(const RopeArgs a, int tokens, int heads_per_block) {
+// head_dim 32, 64, 128 or 256 (2^upt_log units), dim a multiple of 8, rows on 16-byte boundaries; grid (token groups, head groups).
+// Thread: unit u of every slots-th (token, head) pair of the block, RP_BATCH pairs at a time, whose loads go out together - the first
+// ones before the block knows its tokens.
+template <bool NORM>
+__global__ void __launch_bounds__(RP_THREADS) k_rope(const RopeArgs a, int tokens, int heads_per_block, int upt_log) {
     __shared__ float2 cs[RP_TOKENS][RP_MAXHALF];
     __shared__ Tok tok[RP_TOKENS];
     __shared__ int seq[RP_TOKENS];
     const int64_t t0 = int64_t(blockIdx.x) * tokens;
     const int heads = a.n_head + 2 * a.HKV, h0 = blockIdx.y * heads_per_block, nh = min(heads_per_block, heads - h0);
-    find_tokens(a, t0, tokens, tok, seq);
-    if (a.turns) fill_angles(a, tokens, tok, cs);
-    __syncthreads();
-    const int upt = a.head_dim / 8, total = tokens * nh * upt, half = a.dim / 2;
-    for (int i0 = 0; i0 < total; i0 += RP_THREADS) {  // (whole warps stay together for the reduction)
-        const int i = i0 + int(threadIdx.x), u = i % upt, hh = i / upt % nh, t = min(i / upt / nh, tokens - 1), h = h0 + hh;
-        const bool is_v = h >= a.n_head + a.HKV, is_k = !is_v && h >= a.n_head;
-        const bool on = i < total && tok[t].on && (!(is_k || is_v) || tok[t].row >= 0);
-        const int kh = h - a.n_head - (is_v ? a.HKV : 0);
-        const bool turn = a.turns && !is_v && 8 * u < a.dim, split = turn && a.layout == ELB_ROPE_HALF;
-        const int e0 = split ? 4 * u : 8 * u, e1 = split ? half + 4 * u : 8 * u + 4;
-        float v[8] = {};
-        if (on) {
-            const float* src = is_v ? a.v + (t0 + t) * a.ldv + kh * KV_D : is_k ? a.k + (t0 + t) * a.ldk + kh * KV_D : a.q + (t0 + t) * a.ldq + int64_t(h) * a.head_dim;
-            *reinterpret_cast<float4*>(v) = __ldcg(reinterpret_cast<const float4*>(src + e0));
-            *reinterpret_cast<float4*>(v + 4) = __ldcg(reinterpret_cast<const float4*>(src + e1));
+    const int upt = 1 << upt_log, u = threadIdx.x & (upt - 1), slot = threadIdx.x >> upt_log, slots = RP_THREADS >> upt_log;
+    const int pairs = tokens * nh, half = a.dim / 2;
+    const double part = 1.0 / double(1 << (upt_log + 3));  // 1 / head_dim, exact
+    const bool turned = a.turns && 8 * u < a.dim, apart = turned && a.layout == ELB_ROPE_HALF;
+    int th = slot, tt = 0;  // pair of the next load
+    while (th >= nh) { th -= nh; ++tt; }
+    for (int p0 = 0; p0 < pairs; p0 += RP_BATCH * slots) {  // (whole warps stay together for the reductions)
+        float v[RP_BATCH][8];
+        int ht[RP_BATCH], tk[RP_BATCH];
+#pragma unroll
+        for (int b = 0; b < RP_BATCH; ++b) {
+            const int h = h0 + th;
+            ht[b] = tt < tokens ? h : -1;
+            tk[b] = tt;
+            if (tt < tokens && t0 + tt < a.n) {
+                const bool is_v = h >= a.n_head + a.HKV, is_k = h >= a.n_head;
+                const int64_t t = t0 + tt;
+                const float* src = is_v ? a.v + t * a.ldv + (h - a.n_head - a.HKV) * KV_D : is_k ? a.k + t * a.ldk + (h - a.n_head) * KV_D
+                                                                                                  : a.q + t * a.ldq + int64_t(h) * a.head_dim;
+                const bool ap = apart && !is_v;
+                *reinterpret_cast<float4*>(v[b]) = __ldcg(reinterpret_cast<const float4*>(src + (ap ? 4 * u : 8 * u)));
+                *reinterpret_cast<float4*>(v[b] + 4) = __ldcg(reinterpret_cast<const float4*>(src + (ap ? half + 4 * u : 8 * u + 4)));
+            } else {
+#pragma unroll
+                for (int i = 0; i < 8; ++i) v[b][i] = 0.f;
+            }
+            th += slots;
+            while (th >= nh) { th -= nh; ++tt; }
         }
-        const float* w = is_v ? nullptr : is_k ? a.k_norm : a.q_norm;
-        if (a.q_norm || a.k_norm) {
-            double ss = 0.0;
+        if (p0 == 0) {
+            find_tokens(a, t0, tokens, tok, seq);
+            if (a.turns) fill_angles(a, tokens, tok, cs);
+            __syncthreads();
+        }
 #pragma unroll
-            for (int j = 0; j < 8; ++j) ss += double(v[j]) * double(v[j]);
-            for (int o = upt / 2; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
-            if (w) {
-                const float inv = inv_rms(ss / a.head_dim + double(a.eps));
+        for (int b = 0; b < RP_BATCH; ++b) {
+            const int h = ht[b], t = min(tk[b], tokens - 1);
+            const bool is_v = h >= a.n_head + a.HKV, is_k = !is_v && h >= a.n_head, turn = turned && !is_v, ap = apart && !is_v;
+            const int e0 = ap ? 4 * u : 8 * u, e1 = ap ? half + 4 * u : 8 * u + 4;
+            if (NORM && __any_sync(0xffffffffu, h >= 0 && !is_v)) {
+                double ss = 0.0;
 #pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    v[j] = __fmul_rn(__fmul_rn(v[j], inv), w[e0 + j]);
-                    v[j + 4] = __fmul_rn(__fmul_rn(v[j + 4], inv), w[e1 + j]);
+                for (int i = 0; i < 8; ++i) ss += double(v[b][i]) * double(v[b][i]);
+                for (int o = upt / 2; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
+                const float* w = is_v ? nullptr : is_k ? a.k_norm : a.q_norm;
+                if (w && h >= 0) {
+                    const float inv = inv_rms(ss * part + double(a.eps));
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        v[b][i] = __fmul_rn(__fmul_rn(v[b][i], inv), w[e0 + i]);
+                        v[b][i + 4] = __fmul_rn(__fmul_rn(v[b][i + 4], inv), w[e1 + i]);
+                    }
                 }
             }
-        }
-        if (turn) {
+            if (turn) {
 #pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                const float2 c = cs[t][4 * u + j];
-                float& x = split ? v[j] : v[2 * j];
-                float& y = split ? v[j + 4] : v[2 * j + 1];
-                const float x0 = x, y0 = y;
-                x = x0 * c.x - y0 * c.y;
-                y = x0 * c.y + y0 * c.x;
+                for (int i = 0; i < 4; ++i) {
+                    const float2 c = cs[t][4 * u + i];
+                    const float x0 = ap ? v[b][i] : v[b][2 * i], y0 = ap ? v[b][i + 4] : v[b][2 * i + 1];
+                    const float x = x0 * c.x - y0 * c.y, y = x0 * c.y + y0 * c.x;
+                    if (ap) { v[b][i] = x; v[b][i + 4] = y; }
+                    else { v[b][2 * i] = x; v[b][2 * i + 1] = y; }
+                }
             }
-        }
-        if (!on) continue;
-        if (is_k || is_v) {
-            const int64_t plane = int64_t(a.rows.page) * KV_D;
-            __half* dst = a.pool + tok[t].row + (int64_t(is_v) * a.HKV + kh) * a.planes * plane;
-            store4(dst + e0, a.planes, plane, v);
-            store4(dst + e1, a.planes, plane, v + 4);
-        } else {
-            float* dst = a.q_out + (t0 + t) * a.ldqo + int64_t(h) * a.head_dim;
-            *reinterpret_cast<float4*>(dst + e0) = *reinterpret_cast<const float4*>(v);
-            *reinterpret_cast<float4*>(dst + e1) = *reinterpret_cast<const float4*>(v + 4);
+            if (h < 0 || !tok[t].on) continue;
+            if (is_k || is_v) {
+                if (tok[t].row < 0) continue;
+                const int64_t plane = int64_t(a.rows.page) * KV_D;
+                __half* dst = a.pool + tok[t].row + (int64_t(is_v) * a.HKV + h - a.n_head - (is_v ? a.HKV : 0)) * a.planes * plane;
+                store4(dst + e0, a.planes, plane, v[b]);
+                store4(dst + e1, a.planes, plane, v[b] + 4);
+            } else {
+                float* dst = a.q_out + (t0 + t) * a.ldqo + int64_t(h) * a.head_dim;
+                *reinterpret_cast<float4*>(dst + e0) = *reinterpret_cast<const float4*>(v[b]);
+                *reinterpret_cast<float4*>(dst + e1) = *reinterpret_cast<const float4*>(v[b] + 4);
+            }
         }
     }
 }
@@ -207,14 +233,17 @@ __global__ void __launch_bounds__(RP_THREADS) k_rope_any(const RopeArgs a) {
 bool aligned16(const void* p, int64_t ld) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0 && ld % 4 == 0; }
 
 int rope_run(RopeArgs& a, cudaStream_t s) {
-    // one token per block until there are enough of them to fill the GPU; then four share the block's start-up. Heads are cut
-    // over blocks while the grid is small
-    const int heads = a.n_head + 2 * a.HKV, tokens = a.n >= 2048 ? RP_TOKENS : 1;
+    // tokens of a block share its start-up (angles in double): four when there are enough tokens to fill the GPU all the same.
+    // Heads are cut over blocks while the grid is small
+    const int heads = a.n_head + 2 * a.HKV, tokens = a.n >= 1024 ? 4 : a.n >= 512 ? 2 : 1;
     const int64_t groups = (a.n + tokens - 1) / tokens;
     int per = heads;
-    while (per > 8 && groups * ((heads + per - 1) / per) < 592) per = (per + 1) / 2;
-    if (groups > 0x7fffffff) return fail(ELB_ERR_UNSUPPORTED, "rope: too many rows");
-    k_rope<<<dim3(unsigned(groups), unsigned((heads + per - 1) / per)), RP_THREADS, 0, s>>>(a, tokens, per);
+    while (per > 16 && groups * ((heads + per - 1) / per) < 296) per = (per + 1) / 2;
+    int upt_log = 2;
+    while ((8 << upt_log) < a.head_dim) ++upt_log;
+    const dim3 grid{unsigned(groups), unsigned((heads + per - 1) / per)};
+    if (a.q_norm || a.k_norm) k_rope<true><<<grid, RP_THREADS, 0, s>>>(a, tokens, per, upt_log);
+    else k_rope<false><<<grid, RP_THREADS, 0, s>>>(a, tokens, per, upt_log);
     ELB_CUDA(cudaGetLastError());
     return ELB_OK;
 }
