@@ -1,14 +1,15 @@
 // Beam search's selection (elb_beam_select_dev): of the candidates (row b, token t) of a group, scored
 // d_scores[b] + (x_bt - log sum_u exp x_bu) in double precision, the k best.
 //
-// Bound by memory: the logits are read once. A row is cut into chunks of 4096 over many blocks; a block leaves its chunk's maximum,
-// its sum of exponentials behind that maximum and the chunk's k best logits in order. A second launch, one block per group and
-// a warp per row, joins the sums in chunk order, merges the lists, and picks over the rows.
+// Bound by memory: the logits are read once, by k_beam_segments: a warp per segment of 512 logits leaves its maximum, its sum of
+// exponentials behind that maximum and the largest logit that may be picked. Everything else works on these: k_beam_pick,
+// a block per row, joins the sums, takes a bound that k logits reach from the segments' largest, and reads again only the
+// segments that reach it (the order of equal logits needs no care: all at the bound are looked at); the block of a group that comes
+// last picks over the rows. (The k best of every 4096 logits, found where they were read, were 2.4 times the instructions.)
+// Places are found by counting the larger ones.
 //
 // Exponentials are the work beside the loads: double precision, e^y = 2^(i/64) 2^n e^r with y = (64 n + i) ln 2 / 64 + r, |r| <=
-// ln 2 / 128 and the Taylor sum of e^r to r^4 / 24 (4e-14 off at most), nine double operations a logit. The k best: of k groups
-// of threads each has a largest logit; the smallest of these is a bound that at least k logits reach and, on logits that
-// are spread at all, few more. Those are listed and each finds its place by counting the larger ones.
+// ln 2 / 128 and the Taylor sum of e^r to r^4 / 24 (4e-14 off at most), nine double operations a logit.
 #include <algorithm>
 #include <cmath>
 
@@ -18,11 +19,12 @@ namespace elb {
 
 namespace {
 
-constexpr int BS_THREADS = 256, BS_WARPS = 8, BS_PER = 16, BS_CHUNK = BS_THREADS * BS_PER, BS_MAXK = 64;
-constexpr int BS_LIST = 1024;  // logits of a chunk that may reach its bound before the slow way is taken
-constexpr int BJ_STAGE = 512;  // candidates of a row that are merged in shared memory
+constexpr int BS_THREADS = 256, BS_WARPS = 8, BS_PER = 16, BS_SEG = 32 * BS_PER, BS_MAXK = 64;
+constexpr int BS_MAXSEG = 2048;  // segments of a row; longer rows have longer ones
+constexpr int BP_THREADS = 128, BP_LIST = 1024, BP_SEGS = 8;
 
-struct BeamChunk { double sum; float mx; int pad; };
+struct BeamSeg { double sum; float mx; unsigned top; };  // top: beam_key of the largest logit that may be picked
+struct BeamBest { unsigned long long score; int token, pad; };  // score: beam_order
 
 // order of a logit as an unsigned number; 0: not a candidate (-infinity or NaN)
 __device__ __forceinline__ unsigned beam_key(float x) {
@@ -60,222 +62,282 @@ __device__ __forceinline__ float max_nan(float a, float b) {
     return r;
 }
 
-// VEC: rows start on 16-byte boundaries
+// order of a finite score as an unsigned number (0: none)
+__device__ __forceinline__ unsigned long long beam_order(double x) {
+    const unsigned long long bits = static_cast<unsigned long long>(__double_as_longlong(x + 0.0));  // (-0 and 0 are equal scores)
+    return x > -INFINITY && x < INFINITY ? (bits >> 63 ? ~bits : bits | 0x8000000000000000ull) : 0ull;
+}
+
+// grid (segments / 8, rows); VEC: rows start on 16-byte boundaries. `steps` times 512 logits per segment.
 template <bool VEC>
-__global__ void __launch_bounds__(BS_THREADS) k_beam_chunks(const float* __restrict__ logits, int64_t ld, int n, int k, int groups_log,
-                                                            const uint32_t* __restrict__ allowed, int64_t allowed_ld,
-                                                            BeamChunk* __restrict__ parts, unsigned long long* __restrict__ cand) {
-    __shared__ unsigned long long list[BS_LIST];  // (the slow way: [warp][k])
+__global__ void __launch_bounds__(BS_THREADS, 5) k_beam_segments(const float* __restrict__ logits, int64_t ld, int n, int segs, int steps, int beams,
+                                                                 const uint32_t* __restrict__ allowed, int64_t allowed_ld,
+                                                                 BeamSeg* __restrict__ parts, unsigned* __restrict__ arrived) {
     __shared__ double tab[64];
-    __shared__ float red_f[BS_WARPS], red_b[BS_WARPS];
-    __shared__ double red_d[BS_WARPS];
-    __shared__ int count;
     pdl_launch_dependents();
-    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, chunks = gridDim.x;
-    const int64_t row = blockIdx.y, slot = row * chunks + blockIdx.x;
+    const int tid = threadIdx.x, lane = tid & 31, seg = int(blockIdx.x) * BS_WARPS + (tid >> 5);
+    const int64_t row = blockIdx.y;
     const float* x = logits + row * ld;
     const uint32_t* mask = allowed ? allowed + row * allowed_ld : nullptr;
-    const int base = int(blockIdx.x) * BS_CHUNK;
-    auto token = [&](int j) { return base + 4 * (BS_THREADS * (j / 4) + tid) + (j & 3); };  // of a thread's j-th logit
-    float v[BS_PER];
-#pragma unroll
-    for (int q = 0; q < BS_PER / 4; ++q) {
-        const int i = token(4 * q);
-        if (VEC && i + 3 < n) {
-            *reinterpret_cast<float4*>(v + 4 * q) = __ldcg(reinterpret_cast<const float4*>(x + i));
-        } else {
-#pragma unroll
-            for (int c = 0; c < 4; ++c) v[4 * q + c] = i + c < n ? __ldcg(x + i + c) : -INFINITY;
-        }
-    }
-    unsigned off = 0;  // bit j: logit j may not be picked
-    if (mask) {
+    if (blockIdx.x == 0 && tid == 0 && row % beams == 0) arrived[row / beams] = 0;  // for the second launch
+    float mx = -INFINITY;
+    double sum = 0.0;
+    unsigned top = 0;
+    for (int st = 0; st < steps; ++st) {
+        const int base = (seg * steps + st) * BS_SEG;
+        float v[BS_PER];
 #pragma unroll
         for (int q = 0; q < BS_PER / 4; ++q) {
-            const int i = token(4 * q);
-            off |= (i < n ? ~(mask[i >> 5] >> (i & 31)) & 15u : 15u) << (4 * q);
-        }
-    }
-    if (tid < 64) tab[tid] = exp2(tid / 64.0);
-    if (tid == 0) count = 0;
-    float mx = -INFINITY;  // (NaN is passed over here and spoils the sum below)
+            const int i = base + 128 * q + 4 * lane;
+            if (VEC && i + 3 < n) {
+                *reinterpret_cast<float4*>(v + 4 * q) = __ldcg(reinterpret_cast<const float4*>(x + i));
+            } else {
 #pragma unroll
-    for (int j = 0; j < BS_PER; ++j) mx = fmaxf(mx, v[j]);
-    float best = mx;  // the largest that may be picked
-    if (mask) {
-        best = -INFINITY;
-#pragma unroll
-        for (int j = 0; j < BS_PER; ++j) best = (off >> j) & 1u ? best : fmaxf(best, v[j]);
-    }
-    float bound = best;
-    for (int o = 1; o < 32 >> max(0, groups_log - 3); o <<= 1) bound = fmaxf(bound, __shfl_xor_sync(0xffffffffu, bound, o));  // of a group of threads
-    for (int o = 16; o > 0; o >>= 1) bound = fminf(bound, __shfl_xor_sync(0xffffffffu, bound, o));
-    mx = warp_max(mx);
-    if (lane == 0) { red_f[warp] = mx; red_b[warp] = bound; }
-    __syncthreads();
-    bound = red_b[0];
-#pragma unroll
-    for (int w = 0; w < BS_WARPS; ++w) { mx = fmaxf(mx, red_f[w]); bound = fminf(bound, red_b[w]); }
-    if (best >= bound && best > -INFINITY) {  // (the order of the list does not matter: places are counted)
-#pragma unroll
-        for (int j = 0; j < BS_PER; ++j)
-            if (v[j] >= bound && v[j] > -INFINITY && !((off >> j) & 1u)) {
-                const int at = atomicAdd(&count, 1);
-                if (at < BS_LIST) list[at] = beam_pack(beam_key(v[j]), token(j));
+                for (int c = 0; c < 4; ++c) v[4 * q + c] = i + c < n ? __ldcg(x + i + c) : -INFINITY;
             }
-    }
-    // Terms below e^-700 of the largest, and places behind the row's end, count as e^-700: nothing beside the largest's 1. A row
-    // with +infinity has no log-sum-exp.
-    double sum = mx < INFINITY ? 0.0 : double(NAN);
-    if (mx != -INFINITY) {
-        const float low = mx - 700.f;
-        const double from = mx;
+        }
+        unsigned off = 0;  // bit j: logit j may not be picked
+        if (mask) {
 #pragma unroll
-        for (int j = 0; j < BS_PER; ++j) sum = add_exp(sum, double(max_nan(v[j], low)) - from, tab);
-    } else {
+            for (int q = 0; q < BS_PER / 4; ++q) {
+                const int i = base + 128 * q + 4 * lane;
+                off |= (i < n ? ~(mask[i >> 5] >> (i & 31)) & 15u : 15u) << (4 * q);
+            }
+        }
+        if (st == 0) {
+            if (tid < 64) tab[tid] = exp2(tid / 64.0);
+            __syncthreads();
+        }
+        float here = v[0];  // (NaN is passed over here and spoils the sum below)
 #pragma unroll
-        for (int j = 0; j < BS_PER; ++j) sum = v[j] != v[j] ? double(NAN) : sum;
+        for (int j = 1; j < BS_PER; ++j) here = fmaxf(here, v[j]);
+        float best = here;
+        if (mask) {
+            best = -INFINITY;
+#pragma unroll
+            for (int j = 0; j < BS_PER; ++j) best = (off >> j) & 1u ? best : fmaxf(best, v[j]);
+        }
+        top = max(top, __reduce_max_sync(0xffffffffu, beam_key(best)));
+        const unsigned most = __reduce_max_sync(0xffffffffu, beam_key(here));
+        here = most ? beam_logit(most) : -INFINITY;
+        if (here > mx) {
+            sum = mx == -INFINITY ? sum : sum * exp(double(mx) - double(here));
+            mx = here;
+        }
+        // Terms below e^-700 of the largest, and places behind the row's end, count as e^-700: nothing beside the largest's 1
+        if (mx > -INFINITY) {
+            const float low = mx - 700.f;
+            const double from = mx;
+#pragma unroll
+            for (int j = 0; j < BS_PER; ++j) sum = add_exp(sum, double(max_nan(v[j], low)) - from, tab);
+        } else {
+#pragma unroll
+            for (int j = 0; j < BS_PER; ++j) sum = v[j] != v[j] ? double(NAN) : sum;
+        }
     }
     sum = warp_sum(sum);
-    if (lane == 0) red_d[warp] = sum;
-    __syncthreads();
-    const int have = count;
-    if (tid == 0) {
-        double t = 0.0;
-        for (int w = 0; w < BS_WARPS; ++w) t += red_d[w];
-        parts[slot].sum = t;
-        parts[slot].mx = mx;
+    if (lane == 0 && seg < segs) parts[row * segs + seg] = BeamSeg{mx < INFINITY ? sum : double(NAN), mx, top};  // (+infinity: no log-sum-exp)
+}
+
+// A block per row.
+__global__ void __launch_bounds__(BP_THREADS) k_beam_pick(const float* __restrict__ logits, int64_t ld, int n, int segs, int steps, int beams, int k, bool vec,
+                                                          const uint32_t* __restrict__ allowed, int64_t allowed_ld,
+                                                          const BeamSeg* __restrict__ parts, const double* __restrict__ scores,
+                                                          BeamBest* __restrict__ rows_best, unsigned* __restrict__ arrived,
+                                                          int* __restrict__ parent, int* __restrict__ token, double* __restrict__ score) {
+    constexpr int WARPS = BP_THREADS / 32;
+    __shared__ unsigned top[BS_MAXSEG], group_top[32];
+    __shared__ unsigned long long list[BP_LIST];
+    __shared__ __align__(16) float vals[BP_SEGS * BS_SEG];
+    __shared__ int chosen[BS_MAXSEG];
+    __shared__ float red_f[WARPS];
+    __shared__ double red_d[WARPS];
+    __shared__ unsigned long long red_k[WARPS];
+    __shared__ int count, some;
+    __shared__ bool last;
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    const int64_t row = blockIdx.x;
+    const float* x = logits + row * ld;
+    const uint32_t* mask = allowed ? allowed + row * allowed_ld : nullptr;
+    const double own = scores[row];  // (an input of the call: nothing in front of this kernel writes it)
+    pdl_wait();
+    const BeamSeg* p = parts + row * segs;
+    // segments: the row's maximum and sum, and the k with the largest logits, the lower of equal ones first
+    const BeamSeg none{0.0, -INFINITY, 0u};
+    BeamSeg mine[4];
+    float M = -INFINITY;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+        mine[j] = tid + j * BP_THREADS < segs ? p[tid + j * BP_THREADS] : none;
+        if (tid + j * BP_THREADS < segs) top[tid + j * BP_THREADS] = mine[j].top;
+        M = fmaxf(M, mine[j].mx);
     }
-    if (have <= BS_LIST) {  // a candidate's place: how many are larger
-        for (int c = tid; c < have; c += BS_THREADS) {
+    for (int i = tid + 4 * BP_THREADS; i < segs; i += BP_THREADS) {
+        top[i] = p[i].top;
+        M = fmaxf(M, p[i].mx);
+    }
+    M = warp_max(M);
+    if (lane == 0) red_f[warp] = M;
+    if (tid == 0) { count = 0; some = 0; }
+    __syncthreads();
+#pragma unroll
+    for (int w = 0; w < WARPS; ++w) M = fmaxf(M, red_f[w]);
+    auto term = [&](const BeamSeg& q) { return q.mx == -INFINITY ? q.sum : q.sum * exp(double(q.mx) - double(M)); };
+    double sum = 0.0;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) sum += term(mine[j]);
+    for (int i = tid + 4 * BP_THREADS; i < segs; i += BP_THREADS) sum += term(p[i]);
+    sum = warp_sum(sum);
+    if (lane == 0) red_d[warp] = sum;
+    // A bound that at least k logits reach: every thread has the largest of its segments; of 32 groups of threads the k-th largest
+    // of their maxima (sorted across a warp), for k > 32 the smallest of 64 pairs' maxima.
+    unsigned most = 0;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) most = max(most, mine[j].top);
+    for (int i = tid + 4 * BP_THREADS; i < segs; i += BP_THREADS) most = max(most, top[i]);
+    most = max(most, __shfl_xor_sync(0xffffffffu, most, 1));
+    if (k <= 32) {
+        most = max(most, __shfl_xor_sync(0xffffffffu, most, 2));
+        if ((lane & 3) == 0) group_top[tid / 4] = most;
+        __syncthreads();
+        unsigned v = group_top[lane];
+#pragma unroll 1
+        for (int size = 2; size <= 32; size *= 2)
+#pragma unroll 1
+            for (int d = size / 2; d > 0; d /= 2) {  // descending
+                const unsigned o = __shfl_xor_sync(0xffffffffu, v, d);
+                v = ((lane & d) == 0) == ((lane & size) == 0) ? max(v, o) : min(v, o);
+            }
+        most = __shfl_sync(0xffffffffu, v, k - 1);
+    } else {
+        most = __reduce_min_sync(0xffffffffu, most);
+        if (lane == 0) group_top[warp] = most;
+        __syncthreads();
+        for (int w = 0; w < WARPS; ++w) most = min(most, group_top[w]);
+    }
+    const unsigned bound = most;
+    for (int i = tid; i < segs; i += BP_THREADS) {
+        const unsigned u = top[i];
+        if (u && u >= bound) chosen[atomicAdd(&some, 1)] = i;
+    }
+    __syncthreads();
+    double lse = 0.0;
+    for (int w = 0; w < WARPS; ++w) lse += red_d[w];
+    lse = double(M) + log(lse);
+    const bool live = lse > -INFINITY && lse < INFINITY && own > -INFINITY && own < INFINITY;
+    // their logits once more, eight segments' step at a time
+    const int taken = live ? some : 0;
+    auto key_at = [&](int c, int st, int e) -> unsigned long long {  // element e of step st of chosen segment c, 0 when it is no candidate
+        const int i = (chosen[c] * steps + st) * BS_SEG + e;
+        const unsigned key = i < n && (!mask || ((mask[i >> 5] >> (i & 31)) & 1u)) ? beam_key(__ldcg(x + i)) : 0u;
+        return key >= bound ? beam_pack(key, i) : 0ull;
+    };
+    for (int st = 0; st < steps; ++st)
+        for (int c0 = 0; c0 < taken; c0 += BP_SEGS) {
+            const int here = min(BP_SEGS, taken - c0);
+            for (int e = 4 * tid; e < here * BS_SEG; e += 4 * BP_THREADS) {
+                const int i = (chosen[c0 + e / BS_SEG] * steps + st) * BS_SEG + e % BS_SEG;
+                if (vec && i + 3 < n) {
+                    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(uint32_t(__cvta_generic_to_shared(vals + e))), "l"(x + i) : "memory");
+                } else {
+                    for (int q = 0; q < 4; ++q) vals[e + q] = i + q < n ? __ldcg(x + i + q) : -INFINITY;
+                }
+            }
+            asm volatile("cp.async.wait_all;" ::: "memory");
+            const float low = bound ? beam_logit(bound) : -INFINITY;
+            for (int e = 4 * tid; e < here * BS_SEG; e += 4 * BP_THREADS) {  // (a thread's own)
+                const float4 v = *reinterpret_cast<const float4*>(vals + e);
+                const float most = fmaxf(fmaxf(v.x, v.y), fmaxf(v.z, v.w));
+                if (!(most >= low) || most == -INFINITY) continue;
+                for (int q = 0; q < 4; ++q) {
+                    const float w = vals[e + q];
+                    const int i = (chosen[c0 + e / BS_SEG] * steps + st) * BS_SEG + e % BS_SEG + q;
+                    if (!(w >= low) || w == -INFINITY || (mask && !((mask[i >> 5] >> (i & 31)) & 1u))) continue;
+                    const int at = atomicAdd(&count, 1);  // (the order does not matter: places are counted)
+                    if (at < BP_LIST) list[at] = beam_pack(beam_key(w), i);
+                }
+            }
+        }
+    __syncthreads();
+    BeamBest* mine_best = rows_best + row * k;
+    const int have = count;
+    auto put = [&](int place, unsigned long long u) {
+        mine_best[place] = BeamBest{u ? beam_order(own + (double(beam_logit(unsigned(u >> 32))) - lse)) : 0ull, int(~unsigned(u)), 0};
+    };
+    if (have <= BP_LIST) {
+        for (int c = tid; c < have; c += BP_THREADS) {
             const unsigned long long me = list[c];
             int place = 0;
+#pragma unroll 8
             for (int o = 0; o < have; ++o) place += list[o] > me;
-            if (place < k) cand[slot * k + place] = me;
+            if (place < k) put(place, me);
         }
-        for (int r = have + tid; r < k; r += BS_THREADS) cand[slot * k + r] = 0ull;
-        return;
-    }
-    // many logits at the bound (equal ones): every warp its k best one by one, then a merge of the warps' lists
-    __syncthreads();
-    for (int r = 0; r < k; ++r) {
-        unsigned long long most = 0ull;
-#pragma unroll
-        for (int j = 0; j < BS_PER; ++j) {
-            const unsigned long long u = (off >> j) & 1u ? 0ull : beam_pack(beam_key(v[j]), token(j));
-            most = u > most ? u : most;
-        }
-        most = warp_best(most);
-        if (lane == 0) list[warp * k + r] = most;
-#pragma unroll
-        for (int j = 0; j < BS_PER; ++j)
-            if (most && token(j) == int(~unsigned(most))) off |= 1u << j;
-    }
-    __syncthreads();
-    if (warp) return;
-    int at = 0;
-    for (int r = 0; r < k; ++r) {
-        const unsigned long long head = lane < BS_WARPS && at < k ? list[lane * k + at] : 0ull;
-        const unsigned long long best = warp_best(head);
-        if (best && head == best) ++at;
-        if (lane == 0) cand[slot * k + r] = best;
-    }
-}
-
-// One block per group, a warp per row in turn: the row's log-sum-exp and its k best in order; then one warp merges the rows.
-__global__ void __launch_bounds__(BS_THREADS) k_beam_join(const BeamChunk* __restrict__ parts, const unsigned long long* __restrict__ cand,
-                                                          int chunks, int beams, int k, const double* __restrict__ scores,
-                                                          int* __restrict__ parent, int* __restrict__ token, double* __restrict__ score) {
-    extern __shared__ unsigned long long best_of[];  // [beams][k], then [warp][BJ_STAGE]
-    unsigned long long* stage = best_of + beams * k;
-    pdl_wait();
-    __shared__ double lse[64];
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    for (int b = warp; b < beams; b += BS_WARPS) {
-        const int64_t row = int64_t(blockIdx.x) * beams + b;
-        // merge of the chunks' lists; a lane holds chunks lane, lane + 32, ... and looks again only when one of its own was taken
-        const unsigned long long* c = cand + row * chunks * k;
-        if (chunks <= 64 && chunks * k <= BJ_STAGE) {
-            unsigned long long* st = stage + warp * BJ_STAGE;
-            for (int i = lane; i < chunks * k; i += 32) st[i] = c[i];
-            c = st;
-        }
-        const BeamChunk* p = parts + row * chunks;
-        float M = -INFINITY;
-        for (int i = lane; i < chunks; i += 32) M = fmaxf(M, p[i].mx);
-        M = warp_max(M);
-        double t = 0.0;
-        for (int i = lane; i < chunks; i += 32) t += p[i].sum * exp(double(p[i].mx) - double(M));
-        t = warp_sum(t);
-        if (lane == 0) lse[b] = double(M) + log(t);
-        __syncwarp();
-        if (chunks <= 64) {
-            int h0 = 0, h1 = 0;
-            auto head = [&](int i, int h) { return i < chunks && h < k ? c[i * k + h] : 0ull; };
-            unsigned long long u0 = head(lane, 0), u1 = head(lane + 32, 0);
-            for (int r = 0; r < k; ++r) {
-                const unsigned long long best = warp_best(u0 > u1 ? u0 : u1);
-                if (lane == 0) best_of[b * k + r] = best;
-                if (best && u0 == best) u0 = head(lane, ++h0);
-                else if (best && u1 == best) u1 = head(lane + 32, ++h1);
-            }
-        } else {  // long rows: the next best is the largest below the last
-            unsigned long long below = ~0ull;
-            for (int r = 0; r < k; ++r) {
-                unsigned long long h = 0ull;
-                for (int64_t i = lane; i < int64_t(chunks) * k; i += 32) {
-                    const unsigned long long u = c[i];
+        for (int r = have + tid; r < k; r += BP_THREADS) put(r, 0ull);
+    } else {  // many logits at the bound (equal ones): one after the other
+        unsigned long long below = ~0ull;
+        for (int r = 0; r < k; ++r) {
+            unsigned long long h = 0ull;
+            for (int st = 0; st < steps; ++st)
+                for (int e = tid; e < taken * BS_SEG; e += BP_THREADS) {
+                    const unsigned long long u = key_at(e / BS_SEG, st, e % BS_SEG);
                     if (u < below && u > h) h = u;
                 }
-                below = warp_best(h);
-                if (lane == 0) best_of[b * k + r] = below;
-            }
+            h = warp_best(h);
+            if (lane == 0) red_k[warp] = h;
+            __syncthreads();
+            below = 0ull;
+            for (int w = 0; w < WARPS; ++w) below = red_k[w] > below ? red_k[w] : below;
+            if (tid == 0) put(r, below);
+            __syncthreads();
         }
-        __syncwarp();
     }
+    // the group's last block picks over its rows
+    __threadfence();
     __syncthreads();
-    if (warp) return;
-    // over the rows: lane holds rows lane and lane + 32, the score of each one's next candidate as an ordered number (0: none)
-    int at[2] = {0, 0};
-    unsigned long long next[2];
-    auto look = [&](int j) -> unsigned long long {
-        const int i = lane + 32 * j;
-        const unsigned long long u = i < beams && at[j] < k ? best_of[i * k + at[j]] : 0ull;
-        if (!u) return 0ull;
-        const double x = scores[int64_t(blockIdx.x) * beams + i] + (double(beam_logit(unsigned(u >> 32))) - lse[i]);
-        const unsigned long long bits = static_cast<unsigned long long>(__double_as_longlong(x));
-        return x > -INFINITY && x < INFINITY ? (bits >> 63 ? ~bits : bits | 0x8000000000000000ull) : 0ull;
-    };
-    next[0] = look(0);
-    next[1] = beams > 32 ? look(1) : 0ull;
-    for (int r = 0; r < k; ++r) {
-        const unsigned long long most = warp_best(next[0] > next[1] ? next[0] : next[1]);
-        // equal scores: the lowest row (ballots of rows 0-31, then 32-63; -0 and 0 are equal scores)
-        const unsigned a = __ballot_sync(0xffffffffu, most && next[0] == most), b = __ballot_sync(0xffffffffu, most && next[1] == most);
-        const int row = a ? __ffs(int(a)) - 1 : b ? 31 + __ffs(int(b)) : -1;
-        const int64_t w = int64_t(blockIdx.x) * k + r;
-        if (row < 0) {
-            if (lane == 0) { score[w] = -INFINITY; parent[w] = -1; token[w] = -1; }
-        } else if (lane == (row & 31)) {
-            const int j = row >> 5;
-            const unsigned long long bits = most >> 63 ? most & 0x7fffffffffffffffull : ~most;
-            score[w] = __longlong_as_double(static_cast<long long>(bits));
-            parent[w] = int(blockIdx.x) * beams + row;
-            token[w] = int(~unsigned(best_of[row * k + at[j]]));
-            ++at[j];
-            next[j] = look(j);
+    const int64_t group = row / beams;
+    if (tid == 0) last = atomicAdd(arrived + group, 1u) == unsigned(beams - 1);
+    __syncthreads();
+    if (!last) return;
+    __threadfence();
+    const BeamBest* best = rows_best + group * beams * k;
+    const int all = beams * k;
+    for (int i = tid; i < min(all, BP_LIST); i += BP_THREADS) list[i] = __ldcg(&best[i].score);
+    for (int r = tid; r < k; r += BP_THREADS) { score[group * k + r] = -INFINITY; parent[group * k + r] = -1; token[group * k + r] = -1; }
+    __syncthreads();
+    // (score, then row, then rank within the row: i = row * k + rank)
+    for (int i = tid; i < all; i += BP_THREADS) {
+        const unsigned long long me = i < BP_LIST ? list[i] : __ldcg(&best[i].score);
+        if (!me) continue;
+        int place = 0;
+#pragma unroll 4
+        for (int o = 0; o < min(all, BP_LIST); ++o) place += int(list[o] > me) + (int(list[o] == me) & int(o < i));
+        for (int o = BP_LIST; o < all && place < k; ++o) {
+            const unsigned long long u = __ldcg(&best[o].score);
+            place += int(u > me) + (int(u == me) & int(o < i));
         }
-        __syncwarp();
+        if (place >= k) continue;
+        const unsigned long long bits = me >> 63 ? me & 0x7fffffffffffffffull : ~me;
+        score[group * k + place] = __longlong_as_double(static_cast<long long>(bits));
+        parent[group * k + place] = int(group) * beams + i / k;
+        token[group * k + place] = __ldcg(&best[i].token);
     }
 }
 
-size_t chunks_of(int n) { return size_t(n + BS_CHUNK - 1) / BS_CHUNK; }
+// segments of a row and their length in steps of 512 logits
+struct BeamCut { int segs, steps; };
+BeamCut beam_cut(int n) {
+    const int64_t all = (int64_t(n) + BS_SEG - 1) / BS_SEG;
+    const int steps = int((all + BS_MAXSEG - 1) / BS_MAXSEG);
+    return BeamCut{int((all + steps - 1) / steps), steps};
+}
+size_t up256(size_t x) { return (x + 255) / 256 * 256; }
 
 }  // namespace
 
 size_t beam_select_work(int n_vocab, int n_group, int beams, int k) {
-    if (n_vocab <= 0 || n_group < 0 || beams <= 0 || beams > 64 || k <= 0 || k > BS_MAXK || int64_t(n_group) * beams > 65535) return 0;
-    return std::max<size_t>(256, size_t(n_group) * beams * chunks_of(n_vocab) * (sizeof(BeamChunk) + size_t(k) * 8));
+    if (n_vocab <= 0 || n_vocab > (1 << 30) || n_group < 0 || beams <= 0 || beams > 64 || k <= 0 || k > BS_MAXK || int64_t(n_group) * beams > 65535) return 0;
+    const size_t rows = size_t(n_group) * beams;
+    return std::max<size_t>(256, up256(rows * size_t(beam_cut(n_vocab).segs) * sizeof(BeamSeg)) + up256(rows * k * sizeof(BeamBest)) + up256(size_t(n_group) * 4));
 }
 
 int beam_select_launch(int device, const float* logits, int64_t ld, int n_vocab, int n_group, int beams, const double* scores,
@@ -292,19 +354,21 @@ int beam_select_launch(int device, const float* logits, int64_t ld, int n_vocab,
     if (reinterpret_cast<uintptr_t>(work) % 256) return fail(ELB_ERR_INVALID, "beam_select: the work buffer must start on a 256-byte boundary");
     DeviceScope on(device);
     if (on.rc != ELB_OK) return on.rc;
-    const int rows = n_group * beams, chunks = int(chunks_of(n_vocab));
-    auto* parts = static_cast<BeamChunk*>(work);
-    auto* cand = reinterpret_cast<unsigned long long*>(parts + size_t(rows) * chunks);
-    int groups_log = 3;  // groups of threads: a power of two, k at least, 8 (a warp each) to 64
-    while ((1 << groups_log) < k) ++groups_log;
+    const int rows = n_group * beams;
+    const BeamCut cut = beam_cut(n_vocab);
+    uint8_t* at = static_cast<uint8_t*>(work);
+    auto* parts = reinterpret_cast<BeamSeg*>(at);
+    at += up256(size_t(rows) * cut.segs * sizeof(BeamSeg));
+    auto* best = reinterpret_cast<BeamBest*>(at);
+    at += up256(size_t(rows) * k * sizeof(BeamBest));
+    auto* arrived = reinterpret_cast<unsigned*>(at);
     const bool vec = reinterpret_cast<uintptr_t>(logits) % 16 == 0 && ld % 4 == 0;
-    const dim3 grid{unsigned(chunks), unsigned(rows)};
-    if (vec) k_beam_chunks<true><<<grid, BS_THREADS, 0, s>>>(logits, ld, n_vocab, k, groups_log, allowed, allowed_ld, parts, cand);
-    else k_beam_chunks<false><<<grid, BS_THREADS, 0, s>>>(logits, ld, n_vocab, k, groups_log, allowed, allowed_ld, parts, cand);
+    const dim3 grid{unsigned((cut.segs + BS_WARPS - 1) / BS_WARPS), unsigned(rows)};
+    if (vec) k_beam_segments<true><<<grid, BS_THREADS, 0, s>>>(logits, ld, n_vocab, cut.segs, cut.steps, beams, allowed, allowed_ld, parts, arrived);
+    else k_beam_segments<false><<<grid, BS_THREADS, 0, s>>>(logits, ld, n_vocab, cut.segs, cut.steps, beams, allowed, allowed_ld, parts, arrived);
     ELB_CUDA(cudaGetLastError());
-    const size_t smem = (size_t(beams) * k + size_t(BS_WARPS) * BJ_STAGE) * 8;
-    ELB_TRY(ensure_dyn_smem(reinterpret_cast<const void*>(k_beam_join), (64 * BS_MAXK + BS_WARPS * BJ_STAGE) * 8));
-    ELB_TRY(launch_after(k_beam_join, dim3(unsigned(n_group)), dim3(BS_THREADS), smem, s, true, parts, cand, chunks, beams, k, scores, parent, token, score));
+    ELB_TRY(launch_after(k_beam_pick, dim3(unsigned(rows)), dim3(BP_THREADS), 0, s, true, logits, ld, n_vocab, cut.segs, cut.steps, beams, k, vec, allowed,
+                         allowed_ld, parts, scores, best, arrived, parent, token, score));
     return ELB_OK;
 }
 
