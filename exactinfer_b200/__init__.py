@@ -306,10 +306,11 @@ class Backend:
     """el::Backend (src/model.h:42-51) on the CUDA library: cfg(), n_ctx(), name(), eval(tokens, pos0) -> logits."""
 
     def __init__(self, spec: "synth.Spec", tensors, n_ctx: int, device: int = 0, max_batch: int = 0, tp=None,
-                 n_seq: int = 0):
+                 n_seq: int = 0, pages=None):
         """tp = (rank, size, id) makes this process rank `rank` of a tensor-parallel group of `size` GPUs; `id` is the
         128-byte value of tp_unique_id() made on one rank and given to all. `tensors` are the whole model's on every
-        rank; eval must then be called by all ranks with the same arguments."""
+        rank; eval must then be called by all ranks with the same arguments. pages = (page, n_pages, type): a paged cache
+        shared by all sequences (elb_model_set_pages)."""
         self.spec = spec
         self._cfg = spec_config(spec, max_batch, n_seq)
         self._n_ctx = n_ctx
@@ -322,6 +323,8 @@ class Backend:
             check(lib().elb_model_create_tp(C.byref(self._cfg), n_ctx, device, rank, size, buf, C.byref(h)))
         self._h = h
         try:
+            if pages is not None:
+                check(lib().elb_model_set_pages(h, *pages))
             keep = []
             for role, layer, t, rows, n, data in tensors:
                 data = np.ascontiguousarray(data, dtype=np.uint8)
@@ -422,6 +425,41 @@ class Backend:
                                              w.ctypes.data_as(C.c_void_p) if w is not None else None, k, ids.ctypes.data_as(i32),
                                              capi.fptr(vals), lse.ctypes.data_as(C.POINTER(C.c_double))))
         return ids, vals, lse
+
+    def eval_batch_beam(self, tokens, seq, pos, scores, beams: int, k: int, want=None):
+        """eval_batch with beam search's selection on the device: the wanted rows are groups of `beams` rows with scores[R] so far;
+        returns (parent[G][k], token[G][k], score[G][k]), parents counted over the wanted rows (elb_model_eval_batch_beam)."""
+        tokens = np.ascontiguousarray(tokens, dtype=np.int32)
+        seq = np.ascontiguousarray(seq, dtype=np.int32)
+        pos = np.ascontiguousarray(pos, dtype=np.int32)
+        scores = np.ascontiguousarray(scores, dtype=np.float64)
+        w = None if want is None else np.ascontiguousarray(want, dtype=np.uint8)
+        R = tokens.size if w is None else int(np.count_nonzero(w))
+        if scores.size != R or beams < 1 or R % beams:
+            raise ValueError("eval_batch_beam: one score per wanted row, and whole groups of beams")
+        G, i32, f64 = R // beams, C.POINTER(C.c_int32), C.POINTER(C.c_double)
+        parent, token, score = np.empty((G, max(k, 0)), np.int32), np.empty((G, max(k, 0)), np.int32), np.empty((G, max(k, 0)), np.float64)
+        check(lib().elb_model_eval_batch_beam(self._h, tokens.size, tokens.ctypes.data_as(i32), seq.ctypes.data_as(i32), pos.ctypes.data_as(i32),
+                                              w.ctypes.data_as(C.c_void_p) if w is not None else None, G, beams, scores.ctypes.data_as(f64), k,
+                                              parent.ctypes.data_as(i32), token.ctypes.data_as(i32), score.ctypes.data_as(f64)))
+        return parent, token, score
+
+    def reorder(self, seq, parent):
+        """Sequence seq[i] goes on from the state of parent[i], all at once (elb_model_reorder; paged models)."""
+        seq, parent = np.ascontiguousarray(seq, dtype=np.int32), np.ascontiguousarray(parent, dtype=np.int32)
+        if seq.size != parent.size:
+            raise ValueError("reorder: one parent per sequence")
+        i32 = C.POINTER(C.c_int32)
+        check(lib().elb_model_reorder(self._h, seq.size, seq.ctypes.data_as(i32), parent.ctypes.data_as(i32)))
+
+    def drop(self, seq: int):
+        """Gives a sequence's pages back (elb_model_drop; paged models)."""
+        check(lib().elb_model_drop(self._h, seq))
+
+    def free_pages(self) -> int:
+        n = C.c_int32()
+        check(lib().elb_model_free_pages(self._h, C.byref(n)))
+        return n.value
 
     def eval_steps(self, tokens, pos0: int) -> float:
         """Single-token steps back to back, logits left on the device; returns the device time in ms."""

@@ -113,6 +113,11 @@ SIGNATURES |= {
     "elb_kv_attention_work": (C.c_size_t, [_vp, _kvb, _i]),
     "elb_kv_attention_dev": (_i, [_vp, _i, _kvb, _vp, _l, _i, C.c_float, _vp, _l, _vp, C.c_size_t, _vp]),
     "elb_kv_reorder_dev": (_i, [_vp, _i, _vp, _vp, _vp, _l, _vp, _vp, _vp, _vp, _vp]),
+    "elb_model_eval_batch_beam": (_i, [_vp, _i, _i32p, _i32p, _i32p, _vp, _i, _i, _f64p, _i, _i32p, _i32p, _f64p]),
+    "elb_model_set_pages": (_i, [_vp, _i, _i, _i]),
+    "elb_model_reorder": (_i, [_vp, _i, _i32p, _i32p]),
+    "elb_model_drop": (_i, [_vp, _i]),
+    "elb_model_free_pages": (_i, [_vp, _i32p]),
     "elb_beam_select_work": (C.c_size_t, [_i] * 4),
     "elb_beam_select_dev": (_i, [_i, _vp, _l, _i, _i, _i, _vp, _vp, _l, _i, _vp, _vp, _vp, _vp, C.c_size_t, _vp]),
 }

@@ -509,6 +509,14 @@ int elb_model_eval_batch_top(elb_model* m, int n, const int32_t* tokens, const i
                              const uint8_t* want, int k, int32_t* ids, float* top_logits, double* lse) {
     return model_eval_batch_top(M(m), n, tokens, seq, pos, want, k, ids, top_logits, lse);
 }
+int elb_model_eval_batch_beam(elb_model* m, int n, const int32_t* tokens, const int32_t* seq, const int32_t* pos, const uint8_t* want,
+                              int n_group, int beams, const double* scores, int k, int32_t* parent, int32_t* token, double* score) {
+    return model_eval_batch_beam(M(m), n, tokens, seq, pos, want, n_group, beams, scores, k, parent, token, score);
+}
+int elb_model_set_pages(elb_model* m, int page, int n_pages, int type) { return model_set_pages(M(m), page, n_pages, type); }
+int elb_model_reorder(elb_model* m, int n, const int32_t* seq, const int32_t* parent) { return model_reorder(M(m), n, seq, parent); }
+int elb_model_drop(elb_model* m, int seq) { return model_drop(M(m), seq); }
+int elb_model_free_pages(const elb_model* m, int* n) { return model_free_pages(M(m), n); }
 int elb_model_eval_steps(elb_model* m, const int32_t* tokens, int n, int pos0, float* device_ms) {
     return model_eval_steps(M(m), tokens, n, pos0, device_ms);
 }

@@ -400,6 +400,12 @@ int model_eval_batch(Model* m, int n, const int32_t* tokens, const int32_t* seq,
                      float* logits);
 int model_eval_batch_top(Model* m, int n, const int32_t* tokens, const int32_t* seq, const int32_t* pos, const uint8_t* want, int k,
                          int32_t* ids, float* vals, double* lse);
+int model_eval_batch_beam(Model* m, int n, const int32_t* tokens, const int32_t* seq, const int32_t* pos, const uint8_t* want, int n_group,
+                          int beams, const double* scores, int k, int32_t* parent, int32_t* token, double* score);
+int model_set_pages(Model* m, int page, int n_pages, int type);
+int model_reorder(Model* m, int n, const int32_t* seq, const int32_t* parent);
+int model_drop(Model* m, int seq);
+int model_free_pages(const Model* m, int* n);
 int model_stats(const Model* m, float* ms, int64_t* launches);
 int model_hidden(Model* m, float* out);
 int model_fill_exchange(Model* m, int byte);

@@ -74,6 +74,5 @@ size_t kv_attn_few_work(const Kv* kv, const elb_kv_batch* b, int n_head);
 int kv_attn_join(const KvAttnArgs& a, int rows, int64_t tiles, cudaStream_t s);
 int kv_attn_tile_launch(const Kv* kv, int layer, KvAttnArgs a, const elb_kv_batch* b, cudaStream_t s);
 size_t kv_attn_tile_work(const Kv* kv, const elb_kv_batch* b, int n_head);
-int kv_attn_tile_check();
 
 }  // namespace elb

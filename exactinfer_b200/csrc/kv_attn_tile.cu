@@ -683,7 +683,7 @@ TilePlan tile_plan(const Kv* kv, const elb_kv_batch* b, int n_head) {
 
 }  // namespace
 
-int kv_attn_tile_check() {  // did a call's kernel give up on a wait?
+int kv_attention_check() {  // did a call's kernel give up on a wait?
     int* e = tile_error_word();
     if (e && *reinterpret_cast<volatile int*>(e)) {
         *e = 0;
@@ -701,7 +701,7 @@ size_t kv_attn_tile_work(const Kv* kv, const elb_kv_batch* b, int n_head) {
 int kv_attn_tile_launch(const Kv* kv, int layer, KvAttnArgs a, const elb_kv_batch* b, cudaStream_t s) {
     int* err = nullptr;
     if (!tile_error_word() || cudaHostGetDevicePointer(&err, tile_error_word(), 0) != cudaSuccess) return fail(ELB_ERR_CUDA, "kv_attention: no error word");
-    ELB_TRY(kv_attn_tile_check());
+    ELB_TRY(kv_attention_check());
     const TilePlan p = tile_plan(kv, b, a.H);
     a.splits = p.splits; a.chunk = p.chunk; a.tiles_max = p.tiles;
     const int64_t blocks = int64_t(b->n_seq) * p.tiles * kv->HKV;

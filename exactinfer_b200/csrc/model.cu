@@ -9,6 +9,8 @@
 #include "common.cuh"
 #include "split.cuh"
 #include "decode.cuh"
+#include "kv.cuh"
+#include "pages.cuh"
 
 namespace elb {
 
@@ -111,6 +113,20 @@ struct Model {
     unsigned* ap_counters = nullptr;
     float* xr = nullptr;            // [max_batch][E] this rank's partial sums before the all-reduce
     float* logits_local = nullptr;  // [vchunk] this rank's rows of the head
+    // paged cache (model_set_pages): takes the place of kcache / vcache; every evaluation runs as a batch of rows
+    int page = 0, n_pages = 0, page_type = 0;
+    Kv* kv = nullptr;
+    Rope* kv_rope = nullptr;
+    PageBook book;
+    int *table_dev = nullptr, *table_host = nullptr;   // [n_seq][book.width], pinned
+    int *rows_dev = nullptr, *rows_host = nullptr;     // [n_seq + 1] first rows, [n_seq] lengths, pinned
+    void* kv_work = nullptr;
+    size_t kv_work_bytes = 0;
+    int* fork_dev = nullptr;                           // reorder: parent, spare, new lengths, taken [n_seq] each, then a table
+    // beam selection over the rows of a batch, for up to n_seq rows
+    uint8_t *beam_dev = nullptr, *beam_host = nullptr;
+    void* beam_work = nullptr;
+    size_t beam_work_bytes = 0;
     std::vector<std::vector<uint8_t>> shard_store;  // column cuts of wo / down, valid until finalize
 };
 
@@ -219,7 +235,8 @@ int rows_all_reduce(Model* m, int B) {
 
 // Rows of one sequence at consecutive positions (seq0, pos0 + b), or (mixed) row b at posv_dev[b] of sequence seq_dev[b].
 // posv_host (mixed): the positions on the host.
-int body_prefill(Model* m, int B, int pos0, int seq0 = 0, const int* posv_host = nullptr) {
+// pages: rows of several sequences, sequence after sequence, over the paged cache.
+int body_prefill(Model* m, int B, int pos0, int seq0 = 0, const int* posv_host = nullptr, const elb_kv_batch* pages = nullptr) {
     const bool mixed = posv_host != nullptr;
     const elb_config& c = m->cfg;
     const int E = c.n_embd, F = int(m->F), H = m->H, HKV = m->HKV, QD = H * 128, KD = HKV * 128, QKV = QD + 2 * KD;
@@ -233,13 +250,17 @@ int body_prefill(Model* m, int B, int pos0, int seq0 = 0, const int* posv_host =
     for (int l = 0; l < c.n_layer; ++l) {
         Layer& L = m->layers[size_t(l)];
         const size_t seq_stride = size_t(m->n_ctx) * KD;
-        float* kc = m->kcache + (size_t(l) * m->n_seq + (mixed ? 0 : seq0)) * seq_stride;
-        float* vc = m->vcache + (size_t(l) * m->n_seq + (mixed ? 0 : seq0)) * seq_stride;
+        const size_t at = pages ? 0 : (size_t(l) * m->n_seq + (mixed ? 0 : seq0)) * seq_stride;
+        float *kc = m->kcache + at, *vc = m->vcache + at;
         bool q = false;
         for (auto& s : L.qkv) q |= !gemm_f16_tc_usable(s.w, B) && s.w->type != ELB_F16;
         ELB_TRY(split_tokens(m, m->x, E, E, m->nl_qkv, L.attn_norm, B, q));
         for (auto& s : L.qkv) ELB_TRY(linear_tokens(m, s.w, m->x, E, L.attn_norm, B, m->qkv + s.col, QKV, nullptr, EPI_STORE, m->nl_qkv));
-        if (mixed) {
+        if (pages) {
+            ELB_TRY(kv_append_launch(m->kv, l, pages, m->kv_rope, m->qkv + QD, QKV, m->qkv + QD + KD, QKV, L.k_norm, c.eps, m->qkv, QKV, H, L.q_norm,
+                                     m->qkv, QKV, m->stream));
+            ELB_TRY(kv_attention_launch(m->kv, l, pages, m->qkv, QKV, H, scale, m->att, QD, m->kv_work, m->kv_work_bytes, m->stream));
+        } else if (mixed) {
             ELB_TRY(qkv_post_launch(m->qkv, QKV, L.q_norm, L.k_norm, m->rope, 0, B, kc, vc, H, HKV, c.rope_dim, c.eps, m->stream,
                                     m->posv_dev, m->seq_dev, seq_stride, m->use_pdl));
             ELB_TRY(attn_rows_launch(m->qkv, QKV, kc, vc, seq_stride, m->posv_dev, m->seq_dev, posv_host, m->att, QD,
@@ -458,7 +479,7 @@ int chunk(Model* m, const int32_t* tokens, int B, int pos0, float* logits, const
 // false when the model's shape is not one of its shapes.
 static int setup_decode_one(Model* m) {
     const elb_config& c = m->cfg;
-    if (m->tp.size > 1 || env_on("ELB_NO_MEGA") || env_on("ELB_DK_OLD")) return ELB_OK;
+    if (m->kv || m->tp.size > 1 || env_on("ELB_NO_MEGA") || env_on("ELB_DK_OLD")) return ELB_OK;
     DeviceInfo di;
     ELB_TRY(device_info(m->device, &di));
     const int E = c.n_embd, F = int(m->F), QD = m->H * 128, KD = m->HKV * 128, L = c.n_layer, group = m->H / m->HKV;
@@ -580,7 +601,7 @@ static int setup_decode_one(Model* m) {
 // the collectives of this function (the other ranks are on their way into them) with "failed" as its answer.
 int setup_decode_kernel(Model* m, bool local_ok = true) {
     const elb_config& c = m->cfg;
-    if (env_on("ELB_NO_MEGA") || (m->tp.size > 1 && env_on("ELB_TP_NO_MEGA"))) return ELB_OK;
+    if (m->kv || env_on("ELB_NO_MEGA") || (m->tp.size > 1 && env_on("ELB_TP_NO_MEGA"))) return ELB_OK;
     DeviceInfo di;
     ELB_TRY(device_info(m->device, &di));
     auto kind_of = [](const Weight* w) {  // alone in its phase, whole tiles per CTA
@@ -862,6 +883,11 @@ void model_destroy(Model* m) {
     cudaFree(m->top_rows_dev); cudaFree(m->top_scratch);
     if (m->top_rows_host) cudaFreeHost(m->top_rows_host);
     cudaFree(m->seq_dev); cudaFree(m->posv_dev); cudaFree(m->logits_rows); cudaFree(m->rows_part); cudaFree(m->rows_counters);
+    kv_destroy(m->kv);
+    rope_destroy(m->kv_rope);
+    cudaFree(m->table_dev); cudaFree(m->rows_dev); cudaFree(m->kv_work); cudaFree(m->fork_dev); cudaFree(m->beam_dev); cudaFree(m->beam_work);
+    for (void* p : {(void*)m->table_host, (void*)m->rows_host, (void*)m->beam_host})
+        if (p) cudaFreeHost(p);
     tp_reduce_destroy(m->tpr);
     tp_rows_destroy(m->tprows);
     tp_comm_destroy(m->comm);
@@ -872,6 +898,34 @@ void model_destroy(Model* m) {
     if (m->ev1) cudaEventDestroy(m->ev1);
     if (m->stream) cudaStreamDestroy(m->stream);
     delete m;
+}
+
+// the paged cache, its positions and the buffers of its tables
+static int finalize_pages(Model* m) {
+    const elb_config& c = m->cfg;
+    ELB_TRY(kv_create(m->device, c.n_layer, m->HKV, 128, m->page, m->n_pages, m->page_type, nullptr, &m->kv));
+    elb_rope_config rc{};
+    rc.head_dim = 128; rc.dim = c.rope_dim; rc.layout = ELB_ROPE_HALF; rc.scaling = ELB_ROPE_PLAIN; rc.base = c.rope_base;
+    ELB_TRY(rope_create(m->device, &rc, &m->kv_rope));
+    m->book.init(m->page, m->n_pages, m->n_seq, m->n_ctx);
+    const size_t table = size_t(m->n_seq) * size_t(m->book.width) * sizeof(int), rows = size_t(2 * m->n_seq + 1) * sizeof(int);
+    ELB_CUDA(cudaMalloc(&m->table_dev, table));
+    ELB_CUDA(cudaMallocHost(&m->table_host, table));
+    ELB_CUDA(cudaMalloc(&m->rows_dev, rows));
+    ELB_CUDA(cudaMallocHost(&m->rows_host, rows));
+    ELB_CUDA(cudaMalloc(&m->fork_dev, size_t(4 * m->n_seq) * sizeof(int) + table));
+    return ELB_OK;
+}
+static int finalize_beams(Model* m) {
+    const size_t rows = size_t(m->n_seq);
+    m->beam_work_bytes = beam_select_work(m->cfg.n_vocab, m->n_seq, 1, 64);  // (groups of one beam need most)
+    if (!m->beam_work_bytes) return ELB_OK;  // (a vocabulary or batch beyond its limits: the call will say so)
+    // scores [n_seq], then per group k tokens, rows, scores: at most n_seq groups of 64
+    const size_t bytes = rows * sizeof(double) + rows * 64 * (2 * sizeof(int) + sizeof(double));
+    ELB_CUDA(cudaMalloc(&m->beam_work, m->beam_work_bytes));
+    ELB_CUDA(cudaMalloc(&m->beam_dev, bytes));
+    ELB_CUDA(cudaMallocHost(&m->beam_host, bytes));
+    return ELB_OK;
 }
 
 // everything of finalize that concerns this rank alone: uploads, re-layout, allocations; no collective in here
@@ -931,7 +985,8 @@ static int finalize_local(Model* m) {
     const int64_t F = m->F, QD = int64_t(m->H) * 128, KD = int64_t(m->HKV) * 128, QKV = QD + 2 * KD;
 
     // device memory budget before anything is allocated (pre-flight check of the reference, :1578-1591)
-    const size_t kv_bytes = size_t(c.n_layer) * size_t(m->n_seq) * size_t(m->n_ctx) * size_t(KD) * sizeof(float);
+    const size_t pool_bytes = m->page ? kv_bytes(c.n_layer, m->HKV, 128, m->page, m->n_pages, m->page_type) : 0;
+    const size_t kv_bytes = m->page ? pool_bytes / 2 : size_t(c.n_layer) * size_t(m->n_seq) * size_t(m->n_ctx) * size_t(KD) * sizeof(float);
     const int64_t maxn = std::max({E, QD, F});
     size_t need = 2 * kv_bytes + size_t(B) * size_t(E + QKV + QD + F) * 4 + size_t(V) * 4 + size_t(4) * B * maxn + size_t(B) * (maxn / 32 + 1) * 4;
     for (const HostTensor& t : m->pending)
@@ -1002,10 +1057,14 @@ static int finalize_local(Model* m) {
         ELB_CUDA(cudaMalloc(&m->rope, cs.size() * 4));
         ELB_CUDA(cudaMemcpy(m->rope, cs.data(), cs.size() * 4, cudaMemcpyHostToDevice));
     }
-    ELB_CUDA(cudaMalloc(&m->kcache, kv_bytes));
-    ELB_CUDA(cudaMalloc(&m->vcache, kv_bytes));
-    ELB_CUDA(cudaMemset(m->kcache, 0, kv_bytes));
-    ELB_CUDA(cudaMemset(m->vcache, 0, kv_bytes));
+    if (m->page) {
+        ELB_TRY(finalize_pages(m));
+    } else {
+        ELB_CUDA(cudaMalloc(&m->kcache, kv_bytes));
+        ELB_CUDA(cudaMalloc(&m->vcache, kv_bytes));
+        ELB_CUDA(cudaMemset(m->kcache, 0, kv_bytes));
+        ELB_CUDA(cudaMemset(m->vcache, 0, kv_bytes));
+    }
     ELB_CUDA(cudaMalloc(&m->x, size_t(B) * E * 4));
     ELB_CUDA(cudaMalloc(&m->qkv, size_t(B) * QKV * 4));
     ELB_CUDA(cudaMalloc(&m->att, size_t(B) * QD * 4));
@@ -1020,6 +1079,7 @@ static int finalize_local(Model* m) {
     ELB_CUDA(cudaMalloc(&m->xsum, size_t(B) * (maxn / 32 + 1) * 4));
     ELB_CUDA(cudaMalloc(&m->tokens_dev, size_t(B) * sizeof(int32_t)));
     ELB_CUDA(cudaMalloc(&m->pos_dev, sizeof(int)));
+    ELB_TRY(finalize_beams(m));
     if (m->n_seq > 1) {
         ELB_CUDA(cudaMalloc(&m->seq_dev, size_t(B) * sizeof(int)));
         ELB_CUDA(cudaMalloc(&m->posv_dev, size_t(B) * sizeof(int)));
@@ -1111,6 +1171,7 @@ int model_finalize(Model* m) {
 }
 
 namespace { struct TopOut; }
+static int paged_eval(Model* m, const int32_t* tokens, int n, int pos0, float* logits, const TopOut* top);
 int model_eval_impl(Model* m, const int32_t* tokens, int n, int pos0, float* logits, const TopOut* top);
 
 int model_eval_top(Model* m, const int32_t* tokens, int n, int pos0, int k, int32_t* ids, float* vals, double* lse,
@@ -1131,6 +1192,7 @@ int model_eval_impl(Model* m, const int32_t* tokens, int n, int pos0, float* log
     for (int i = 0; i < n; ++i)
         if (tokens[i] < 0 || tokens[i] >= m->cfg.n_vocab) return fail(ELB_ERR_RANGE, "eval: token id out of range");
     ELB_CUDA(cudaSetDevice(m->device));
+    if (m->kv) return paged_eval(m, tokens, n, pos0, logits, top);
     m->last_ms = 0.f;
     const int64_t before = m->launches;
     for (int done = 0; done < n;) {
@@ -1146,9 +1208,12 @@ int model_eval_impl(Model* m, const int32_t* tokens, int n, int pos0, float* log
 // Rows of several sequences in one pass: the prompt-chunk path with per-row sequence and position (body_prefill, mixed)
 // or, when all rows belong to one sequence at consecutive positions, exactly the prompt-chunk path on that sequence's
 // cache. The head runs over the wanted rows only.
-namespace { struct TopRows { int k; int32_t* ids; float* vals; double* lse; }; }
+namespace {
+struct TopRows { int k; int32_t* ids; float* vals; double* lse; const uint32_t* allowed = nullptr; };  // allowed: one row wanted
+struct BeamRows { int groups, beams, k; const double* scores; int32_t *parent, *token; double* score; };
+}
 static int eval_batch_impl(Model* m, int n, const int32_t* tokens, const int32_t* seq, const int32_t* pos, const uint8_t* want,
-                           float* logits, const TopRows* top);
+                           float* logits, const TopRows* top, const BeamRows* beam = nullptr);
 
 int model_eval_batch(Model* m, int n, const int32_t* tokens, const int32_t* seq, const int32_t* pos, const uint8_t* want,
                      float* logits) {
@@ -1164,8 +1229,83 @@ int model_eval_batch_top(Model* m, int n, const int32_t* tokens, const int32_t* 
     return eval_batch_impl(m, n, tokens, seq, pos, want, nullptr, &top);
 }
 
+// Rows of a batch over the paged cache: order[i] = place of the caller's row i when the rows of every sequence stand together;
+// pages for all positions that will be written (a last page that others use as well is copied first), lengths and tables to
+// the device. Nothing is changed when a page is missing.
+static int paged_batch(Model* m, int n, const int32_t* seq, const int32_t* pos, std::vector<int>* order, elb_kv_batch* b) {
+    const int S = m->n_seq;
+    std::vector<int> count(size_t(S), 0), first(size_t(S), -1);
+    for (int i = 0; i < n; ++i) {
+        if (first[size_t(seq[i])] < 0) first[size_t(seq[i])] = pos[i];
+        ++count[size_t(seq[i])];
+    }
+    PageBook& book = m->book;
+    int64_t need = 0;
+    for (int s = 0; s < S; ++s) {
+        if (!count[size_t(s)]) continue;
+        if (first[size_t(s)] > book.len[size_t(s)]) return fail(ELB_ERR_RANGE, "eval_batch: a sequence's rows must continue what it has cached");
+        need += book.need(s, first[size_t(s)], first[size_t(s)] + count[size_t(s)]);
+    }
+    if (need > int64_t(book.free.size())) return fail(ELB_ERR_MEMORY, "eval_batch: no free page left in the cache");
+    int at = 0, max_q = 1, max_len = 1;
+    for (int s = 0; s < S; ++s) {
+        m->rows_host[s] = at;
+        m->rows_host[S + 1 + s] = 0;
+        const int q = count[size_t(s)];
+        if (!q) continue;
+        const int p0 = first[size_t(s)], p1 = p0 + q;
+        auto& t = book.table[size_t(s)];
+        if (book.shared_tail(s, p0)) {  // two children of this sequence at length p0: the second has a last page of its own
+            const int mine = book.take();
+            std::vector<int> two = {0, 0, -1, mine, p0, p0};  // parents, spare pages, lengths
+            two.insert(two.end(), t.begin(), t.begin() + p0 / m->page + 1);
+            const int width = p0 / m->page + 1;
+            two.insert(two.end(), t.begin(), t.begin() + width);
+            int* d = nullptr;
+            ELB_CUDA(cudaMalloc(&d, (two.size() + 4 + size_t(2) * width) * sizeof(int)));
+            int* out = d + two.size();
+            cudaError_t e = cudaMemcpyAsync(d, two.data(), two.size() * sizeof(int), cudaMemcpyHostToDevice, m->stream);
+            const int rc = e == cudaSuccess ? kv_reorder_launch(m->kv, 2, d, d + 4, d + 6, width, d + 2, out, out + 4, out + 2, m->stream) : ELB_OK;
+            if (e == cudaSuccess) e = cudaStreamSynchronize(m->stream);
+            cudaFree(d);
+            if (rc != ELB_OK || e != cudaSuccess) {
+                book.drop(mine);
+                if (rc != ELB_OK) return rc;
+                ELB_CUDA(e);
+            }
+            ++m->launches;
+            book.drop(t[size_t(p0 / m->page)]);
+            t[size_t(p0 / m->page)] = mine;
+        }
+        book.shorten(s, p0);
+        while (int(t.size()) < book.pages_of(p1)) t.push_back(book.take());
+        book.len[size_t(s)] = p1;
+        m->rows_host[S + 1 + s] = p1;
+        at += q;
+        max_q = std::max(max_q, q);
+        max_len = std::max(max_len, p1);
+        for (int i = 0; i < book.width; ++i) m->table_host[size_t(s) * book.width + i] = i < int(t.size()) ? t[size_t(i)] : -1;
+    }
+    m->rows_host[S] = at;
+    order->resize(size_t(n));
+    std::vector<int> next(m->rows_host, m->rows_host + S);
+    for (int i = 0; i < n; ++i) (*order)[size_t(i)] = next[size_t(seq[i])]++;
+    ELB_CUDA(cudaMemcpyAsync(m->rows_dev, m->rows_host, size_t(2 * S + 1) * sizeof(int), cudaMemcpyHostToDevice, m->stream));
+    ELB_CUDA(cudaMemcpyAsync(m->table_dev, m->table_host, size_t(S) * book.width * sizeof(int), cudaMemcpyHostToDevice, m->stream));
+    *b = elb_kv_batch{S, n, max_q, max_len, m->rows_dev, m->rows_dev + S + 1, m->table_dev, book.width};
+    const size_t work = kv_attention_work(m->kv, b, m->H);
+    if (work > m->kv_work_bytes) {
+        cudaFree(m->kv_work);
+        m->kv_work = nullptr;
+        m->kv_work_bytes = 0;
+        if (device_malloc(&m->kv_work, work) != cudaSuccess) return fail(ELB_ERR_MEMORY, "eval_batch: out of device memory");
+        m->kv_work_bytes = work;
+    }
+    return ELB_OK;
+}
+
 static int eval_batch_impl(Model* m, int n, const int32_t* tokens, const int32_t* seq, const int32_t* pos, const uint8_t* want,
-                           float* logits, const TopRows* top) {
+                           float* logits, const TopRows* top, const BeamRows* beam) {
     if (!m || !tokens || !seq || !pos) return fail(ELB_ERR_INVALID, "eval_batch: null argument");
     if (!m->finalized) return fail(ELB_ERR_STATE, "eval_batch: model not finalized");
     if (n <= 0) return fail(ELB_ERR_INVALID, "eval_batch: empty batch");
@@ -1177,7 +1317,7 @@ static int eval_batch_impl(Model* m, int n, const int32_t* tokens, const int32_t
         if (seq[i] < 0 || seq[i] >= m->n_seq) return fail(ELB_ERR_RANGE, "eval_batch: sequence index out of range");
         if (pos[i] < 0 || pos[i] >= m->n_ctx) return fail(ELB_ERR_RANGE, "eval_batch: context window full");
         uniform = uniform && seq[i] == seq[0] && pos[i] == pos[0] + i;
-        if ((logits || top) && (!want || want[i])) rows.push_back(i);
+        if ((logits || top || beam) && (!want || want[i])) rows.push_back(i);
     }
     for (int i = 0; i < n; ++i)  // rows of one sequence: increasing, consecutive positions
         for (int j = i + 1; j < n; ++j)
@@ -1188,12 +1328,25 @@ static int eval_batch_impl(Model* m, int n, const int32_t* tokens, const int32_t
     if (!uniform && m->n_seq == 1) return fail(ELB_ERR_INVALID, "eval_batch: one sequence needs consecutive positions");
     if (int(rows.size()) > m->n_seq) return fail(ELB_ERR_UNSUPPORTED, "eval_batch: more wanted rows than sequences");
     if (m->tp.size > 1 && rows.size() > 1) return fail(ELB_ERR_UNSUPPORTED, "eval_batch: one wanted row under tensor parallelism");
+    if (beam && int64_t(beam->groups) * beam->beams != int64_t(rows.size()))
+        return fail(ELB_ERR_INVALID, "eval_batch_beam: the wanted rows must be the groups' beams");
     ELB_CUDA(cudaSetDevice(m->device));
+    // paged: the rows go sequence after sequence; order[i] is where the caller's row i went
+    elb_kv_batch pages{};
+    std::vector<int> order;
+    std::vector<int32_t> sorted;
+    if (m->kv) {
+        ELB_TRY(paged_batch(m, n, seq, pos, &order, &pages));
+        sorted.resize(size_t(n));
+        for (int i = 0; i < n; ++i) sorted[size_t(order[size_t(i)])] = tokens[i];
+        tokens = sorted.data();
+        for (int& r : rows) r = order[size_t(r)];
+    }
     const int E = m->cfg.n_embd;
     const int64_t V = m->cfg.n_vocab, before = m->launches;
     std::memcpy(m->tokens_host, tokens, size_t(n) * sizeof(int32_t));
     ELB_CUDA(cudaMemcpyAsync(m->tokens_dev, m->tokens_host, size_t(n) * sizeof(int32_t), cudaMemcpyHostToDevice, m->stream));
-    if (!uniform) {
+    if (!uniform && !m->kv) {
         // (pageable source: the copies are staged by the runtime before the call returns)
         ELB_CUDA(cudaMemcpyAsync(m->seq_dev, seq, size_t(n) * sizeof(int), cudaMemcpyHostToDevice, m->stream));
         ELB_CUDA(cudaMemcpyAsync(m->posv_dev, pos, size_t(n) * sizeof(int), cudaMemcpyHostToDevice, m->stream));
@@ -1201,15 +1354,17 @@ static int eval_batch_impl(Model* m, int n, const int32_t* tokens, const int32_t
     ELB_CUDA(cudaEventRecord(m->ev0, m->stream));
     ELB_TRY(launch_gather_rows(m->embd, m->tokens_dev, n, m->x, m->stream));
     ++m->launches;
-    ELB_TRY(body_prefill(m, n, pos[0], seq[0], uniform ? nullptr : pos));
-    m->last_rows = n;
+    ELB_TRY(body_prefill(m, n, pos[0], seq[0], uniform || m->kv ? nullptr : pos, m->kv ? &pages : nullptr));
+    m->last_rows = m->kv ? order.back() + 1 : n;  // (where the caller's last row is)
     float* out_dev = nullptr;
     if (rows.size() == 1) {
         ELB_TRY(head_logits(m, m->x + size_t(rows[0]) * E));
         out_dev = m->logits;
     } else if (rows.size() > 1) {
         float* xh = m->x;
-        if (int(rows.size()) != n) {  // compact the wanted rows (act is free after the last layer)
+        bool as_they_are = int(rows.size()) == n;
+        for (size_t r = 0; as_they_are && r < rows.size(); ++r) as_they_are = rows[r] == int(r);
+        if (!as_they_are) {  // compact the wanted rows (act is free after the last layer)
             xh = m->act;
             for (size_t r = 0; r < rows.size(); ++r)
                 ELB_CUDA(cudaMemcpyAsync(xh + r * E, m->x + size_t(rows[r]) * E, size_t(E) * sizeof(float), cudaMemcpyDeviceToDevice, m->stream));
@@ -1229,15 +1384,35 @@ static int eval_batch_impl(Model* m, int n, const int32_t* tokens, const int32_t
         out_dev = m->logits_rows;
     }
     if (out_dev && top) {  // k best tokens and the log-sum-exp of every wanted row, on the device
-        ELB_TRY(logits_top_launch(out_dev, int(V), V, int(rows.size()), top->k, m->top_rows_dev, m->top_scratch, m->n_seq, m->stream));
+        if (top->allowed) ELB_CUDA(cudaMemcpyAsync(m->mask_dev, top->allowed, size_t((V + 31) / 32) * 4, cudaMemcpyHostToDevice, m->stream));
+        ELB_TRY(logits_top_launch(out_dev, int(V), V, int(rows.size()), top->k, m->top_rows_dev, m->top_scratch, m->n_seq, m->stream,
+                                  top->allowed ? m->mask_dev : nullptr));
         ++m->launches;
+    }
+    const size_t picks = beam ? size_t(beam->groups) * beam->k : 0;
+    double* beam_scores = reinterpret_cast<double*>(m->beam_dev);  // [rows], then [picks] scores, rows, tokens
+    if (beam) {
+        std::memcpy(m->beam_host, beam->scores, rows.size() * sizeof(double));
+        ELB_CUDA(cudaMemcpyAsync(m->beam_dev, m->beam_host, rows.size() * sizeof(double), cudaMemcpyHostToDevice, m->stream));
+        double* score = beam_scores + rows.size();
+        int* parent = reinterpret_cast<int*>(score + picks);
+        ELB_TRY(beam_select_launch(m->device, out_dev, V, int(V), beam->groups, beam->beams, beam_scores, nullptr, 0, beam->k, parent, parent + picks,
+                                   score, m->beam_work, m->beam_work_bytes, m->stream));
+        m->launches += 2;
     }
     ELB_CUDA(cudaEventRecord(m->ev1, m->stream));
     if (out_dev && top) ELB_CUDA(cudaMemcpyAsync(m->top_rows_host, m->top_rows_dev, rows.size() * TOP_BYTES, cudaMemcpyDeviceToHost, m->stream));
+    else if (out_dev && beam) ELB_CUDA(cudaMemcpyAsync(m->beam_host, beam_scores + rows.size(), picks * 16, cudaMemcpyDeviceToHost, m->stream));
     else if (out_dev) ELB_CUDA(cudaMemcpyAsync(logits, out_dev, rows.size() * size_t(V) * sizeof(float), cudaMemcpyDeviceToHost, m->stream));
     ELB_CUDA(cudaStreamSynchronize(m->stream));
     ELB_TRY(gemm_tc_check());
     ELB_TRY(gemm_f16_tc_check());
+    if (m->kv) ELB_TRY(kv_attention_check());
+    if (out_dev && beam) {
+        std::memcpy(beam->score, m->beam_host, picks * sizeof(double));
+        std::memcpy(beam->parent, m->beam_host + picks * sizeof(double), picks * sizeof(int32_t));
+        std::memcpy(beam->token, m->beam_host + picks * (sizeof(double) + sizeof(int32_t)), picks * sizeof(int32_t));
+    }
     if (out_dev && top)
         for (size_t r = 0; r < rows.size(); ++r) {  // layout per row: lse (double), then k ids, then k logits
             const uint8_t* src = m->top_rows_host + r * TOP_BYTES;
@@ -1247,6 +1422,116 @@ static int eval_batch_impl(Model* m, int n, const int32_t* tokens, const int32_t
         }
     ELB_CUDA(cudaEventElapsedTime(&m->last_ms, m->ev0, m->ev1));
     m->last_launches = m->launches - before;
+    return ELB_OK;
+}
+
+// model_eval over the paged cache: chunks of rows of sequence 0
+static int paged_eval(Model* m, const int32_t* tokens, int n, int pos0, float* logits, const TopOut* top) {
+    float ms = 0.f;
+    int64_t launches = 0;
+    for (int done = 0; done < n;) {
+        const int b = std::min(m->max_batch, n - done);
+        const bool last = done + b == n;
+        std::vector<int32_t> seq(size_t(b), 0), pos(static_cast<size_t>(b));
+        std::vector<uint8_t> want(size_t(b), 0);
+        for (int i = 0; i < b; ++i) pos[size_t(i)] = pos0 + done + i;
+        want.back() = 1;
+        TopRows rows{};
+        if (top) { rows.k = top->k; rows.ids = top->ids; rows.vals = top->vals; rows.lse = top->lse; rows.allowed = top->allowed; }
+        ELB_TRY(eval_batch_impl(m, b, tokens + done, seq.data(), pos.data(), want.data(), last ? logits : nullptr, last && top ? &rows : nullptr));
+        ms += m->last_ms;
+        launches += m->last_launches;
+        done += b;
+    }
+    m->last_ms = ms;
+    m->last_launches = launches;
+    return ELB_OK;
+}
+
+int model_eval_batch_beam(Model* m, int n, const int32_t* tokens, const int32_t* seq, const int32_t* pos, const uint8_t* want, int n_group, int beams,
+                          const double* scores, int k, int32_t* parent, int32_t* token, double* score) {
+    if (!scores || !parent || !token || !score) return fail(ELB_ERR_INVALID, "eval_batch_beam: null argument");
+    if (n_group < 1 || beams < 1 || beams > 64 || k < 1 || k > 64 || (m && k > int64_t(beams) * m->cfg.n_vocab))
+        return fail(ELB_ERR_INVALID, "eval_batch_beam: groups of 1 to 64 beams and k between 1 and 64 are needed");
+    if (m && m->finalized && !m->beam_work) return fail(ELB_ERR_UNSUPPORTED, "eval_batch_beam: the vocabulary is too large");
+    const BeamRows b{n_group, beams, k, scores, parent, token, score};
+    return eval_batch_impl(m, n, tokens, seq, pos, want, nullptr, nullptr, &b);
+}
+
+int model_set_pages(Model* m, int page, int n_pages, int type) {
+    if (!m) return fail(ELB_ERR_INVALID, "set_pages: null model");
+    if (m->finalized) return fail(ELB_ERR_STATE, "set_pages: model already finalized");
+    if (m->tp.size > 1) return fail(ELB_ERR_UNSUPPORTED, "set_pages: not under tensor parallelism");
+    if (m->cfg.rope_dim % 8) return fail(ELB_ERR_UNSUPPORTED, "set_pages: the rotated part of a head must be a multiple of 8");
+    if (!kv_bytes(m->cfg.n_layer, m->HKV, 128, page, n_pages, type))
+        return fail(ELB_ERR_INVALID, "set_pages: a page holds 16, 32, 64, 128 or 256 positions of type F16 or PAIR, and a pool at most 2^31 rows");
+    if (m->n_seq > 4096) return fail(ELB_ERR_UNSUPPORTED, "set_pages: more than 4096 sequences");
+    m->page = page; m->n_pages = n_pages; m->page_type = type;
+    return ELB_OK;
+}
+
+int model_free_pages(const Model* m, int* n) {
+    if (!m || !n) return fail(ELB_ERR_INVALID, "free_pages: null argument");
+    if (!m->kv || !m->finalized) return fail(ELB_ERR_STATE, "free_pages: the model has no paged cache");
+    *n = int(m->book.free.size());
+    return ELB_OK;
+}
+
+int model_drop(Model* m, int seq) {
+    if (!m) return fail(ELB_ERR_INVALID, "drop: null model");
+    if (!m->kv || !m->finalized) return fail(ELB_ERR_STATE, "drop: the model has no paged cache");
+    if (seq < 0 || seq >= m->n_seq) return fail(ELB_ERR_RANGE, "drop: sequence index out of range");
+    m->book.shorten(seq, 0);
+    return ELB_OK;
+}
+
+// sequences seq[i] go on from parent[i]; the others stay. The device copies what last pages need it (elb_kv_reorder_dev over all
+// sequences), the host keeps the same tables.
+int model_reorder(Model* m, int n, const int32_t* seq, const int32_t* parent) {
+    if (!m || !seq || !parent) return fail(ELB_ERR_INVALID, "reorder: null argument");
+    if (!m->kv || !m->finalized) return fail(ELB_ERR_STATE, "reorder: the model has no paged cache");
+    if (n < 0) return fail(ELB_ERR_INVALID, "reorder: negative count");
+    const int S = m->n_seq;
+    PageBook& book = m->book;
+    std::vector<int> from(static_cast<size_t>(S));
+    std::vector<char> named(size_t(S), 0);
+    for (int s = 0; s < S; ++s) from[size_t(s)] = s;
+    for (int i = 0; i < n; ++i) {
+        if (seq[i] < 0 || seq[i] >= S || parent[i] < 0 || parent[i] >= S) return fail(ELB_ERR_RANGE, "reorder: sequence index out of range");
+        if (named[size_t(seq[i])]) return fail(ELB_ERR_INVALID, "reorder: a sequence is named twice");
+        named[size_t(seq[i])] = 1;
+        from[size_t(seq[i])] = parent[i];
+    }
+    const std::vector<char> copy = book.copies(from);
+    const int64_t need = std::count(copy.begin(), copy.end(), char(1));
+    if (need > int64_t(book.free.size())) return fail(ELB_ERR_MEMORY, "reorder: no free page left in the cache");
+    if (n == 0) return ELB_OK;
+    ELB_CUDA(cudaSetDevice(m->device));
+    std::vector<int> spare(size_t(S), -1);
+    for (int s = 0; s < S; ++s) {
+        if (copy[size_t(s)]) spare[size_t(s)] = book.take();
+        m->rows_host[s] = book.len[size_t(s)];
+        const auto& t = book.table[size_t(s)];
+        for (int i = 0; i < book.width; ++i) m->table_host[size_t(s) * book.width + i] = i < int(t.size()) ? t[size_t(i)] : -1;
+    }
+    auto run = [&]() -> int {
+        int *d_parent = m->fork_dev, *d_spare = d_parent + S, *d_len = d_spare + S, *d_taken = d_len + S, *d_table = d_taken + S;
+        ELB_CUDA(cudaMemcpyAsync(d_parent, from.data(), size_t(S) * sizeof(int), cudaMemcpyHostToDevice, m->stream));
+        ELB_CUDA(cudaMemcpyAsync(d_spare, spare.data(), size_t(S) * sizeof(int), cudaMemcpyHostToDevice, m->stream));
+        ELB_CUDA(cudaMemcpyAsync(m->rows_dev, m->rows_host, size_t(S) * sizeof(int), cudaMemcpyHostToDevice, m->stream));
+        ELB_CUDA(cudaMemcpyAsync(m->table_dev, m->table_host, size_t(S) * book.width * sizeof(int), cudaMemcpyHostToDevice, m->stream));
+        ELB_TRY(kv_reorder_launch(m->kv, S, d_parent, m->rows_dev, m->table_dev, book.width, d_spare, d_len, d_table, d_taken, m->stream));
+        ++m->launches;
+        ELB_CUDA(cudaStreamSynchronize(m->stream));
+        return ELB_OK;
+    };
+    const int rc = run();
+    if (rc != ELB_OK) {
+        for (int p : spare)
+            if (p >= 0) book.drop(p);
+        return rc;
+    }
+    book.reorder(from, spare);
     return ELB_OK;
 }
 
@@ -1260,6 +1545,18 @@ int model_eval_steps(Model* m, const int32_t* tokens, int n, int pos0, float* de
     for (int i = 0; i < n; ++i)
         if (tokens[i] < 0 || tokens[i] >= m->cfg.n_vocab) return fail(ELB_ERR_RANGE, "eval_steps: token id out of range");
     ELB_CUDA(cudaSetDevice(m->device));
+    if (m->kv) {  // row by row
+        float ms = 0.f;
+        int64_t launches = 0;
+        for (int i = 0; i < n; ++i) {
+            ELB_TRY(paged_eval(m, tokens + i, 1, pos0 + i, nullptr, nullptr));
+            ms += m->last_ms;
+            launches += m->last_launches;
+        }
+        *device_ms = m->last_ms = ms;
+        m->last_launches = launches;
+        return ELB_OK;
+    }
     int32_t* pin = nullptr;  // [n] tokens, [n] positions, then the control words; pinned so that the copies stay asynchronous
     ELB_CUDA(cudaMallocHost(&pin, (size_t(2) * n + 4) * sizeof(int32_t)));
     for (int i = 0; i < n; ++i) { pin[i] = tokens[i]; pin[n + i] = pos0 + i; }
@@ -1378,7 +1675,9 @@ int model_config(const Model* m, elb_config* out) {
     return ELB_OK;
 }
 size_t model_weight_bytes(const Model* m) { return m->weight_bytes; }
-size_t model_kv_bytes_per_token(const Model* m) { return size_t(2) * m->cfg.n_layer * m->HKV * 128 * sizeof(float); }
+size_t model_kv_bytes_per_token(const Model* m) {
+    return size_t(2) * m->cfg.n_layer * m->HKV * 128 * (m->page ? size_t(2 * m->page_type) : sizeof(float));
+}
 int model_device(const Model* m) { return m->device; }
 
 }  // namespace elb

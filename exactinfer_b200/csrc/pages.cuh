@@ -1,0 +1,78 @@
+// Which page of the pool belongs to which sequence of a model: tables, reference counts, free pages (host memory only).
+#pragma once
+
+#include <algorithm>
+#include <vector>
+
+namespace elb {
+
+struct PageBook {
+    int page = 0, width = 0;                // positions of a page, pages of a sequence
+    std::vector<int> free, refs;            // pages nobody has; users of each page
+    std::vector<std::vector<int>> table;    // per sequence
+    std::vector<int> len;                   // positions of each sequence
+
+    void init(int page_, int n_pages, int n_seq, int n_ctx) {
+        page = page_;
+        width = (n_ctx + page - 1) / page;
+        refs.assign(size_t(n_pages), 0);
+        free.clear();
+        for (int p = n_pages - 1; p >= 0; --p) free.push_back(p);
+        table.assign(size_t(n_seq), {});
+        len.assign(size_t(n_seq), 0);
+    }
+    int pages_of(int positions) const { return (positions + page - 1) / page; }
+    int take() {
+        const int p = free.back();
+        free.pop_back();
+        refs[size_t(p)] = 1;
+        return p;
+    }
+    void drop(int p) {
+        if (--refs[size_t(p)] == 0) free.push_back(p);
+    }
+    // the sequence keeps its first `positions` positions
+    void shorten(int s, int positions) {
+        auto& t = table[size_t(s)];
+        while (int(t.size()) > pages_of(positions)) {
+            drop(t.back());
+            t.pop_back();
+        }
+        len[size_t(s)] = std::min(len[size_t(s)], positions);
+    }
+    // free pages that sequence s needs to be written from position p0 (<= len) to p1 (exclusive): new ones, and one for a last page
+    // that it keeps in part and shares
+    int need(int s, int p0, int p1) const {
+        const int kept = std::min(pages_of(p0), int(table[size_t(s)].size()));
+        return std::max(0, pages_of(p1) - kept) + (shared_tail(s, p0) ? 1 : 0);
+    }
+    bool shared_tail(int s, int p0) const { return p0 % page && refs[size_t(table[size_t(s)][size_t(p0 / page)])] > 1; }
+    // sequences 0.. go on from parent[s]: who needs a copy of the parent's last page (the rule of elb_kv_reorder_dev)
+    std::vector<char> copies(const std::vector<int>& parent) const {
+        std::vector<char> seen(parent.size(), 0), copy(parent.size(), 0);
+        for (size_t s = 0; s < parent.size(); ++s) {
+            const size_t p = size_t(parent[s]);
+            copy[s] = seen[p] && len[p] % page;
+            seen[p] = 1;
+        }
+        return copy;
+    }
+    void reorder(const std::vector<int>& parent, const std::vector<int>& spare) {  // spare[s]: a page taken for s, or -1
+        std::vector<std::vector<int>> next(table.size());
+        std::vector<int> next_len(len.size());
+        for (size_t s = 0; s < parent.size(); ++s) {
+            const size_t p = size_t(parent[s]);
+            next_len[s] = len[p];
+            next[s].assign(table[p].begin(), table[p].begin() + pages_of(len[p]));
+            if (spare[s] >= 0) next[s].back() = spare[s];
+            for (int pg : next[s])
+                if (pg != spare[s]) ++refs[size_t(pg)];
+        }
+        for (auto& t : table)
+            for (int pg : t) drop(pg);
+        table.swap(next);
+        len.swap(next_len);
+    }
+};
+
+}  // namespace elb

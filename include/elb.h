@@ -210,6 +210,25 @@ int elb_model_eval_batch(elb_model* m, int n, const int32_t* tokens, const int32
 int elb_model_eval_batch_top(elb_model* m, int n, const int32_t* tokens, const int32_t* seq, const int32_t* pos,
                              const uint8_t* want, int k, int32_t* ids, float* top_logits, double* lse);
 
+/* elb_model_eval_batch with beam search's selection on the device: the wanted rows are n_group groups of `beams` rows (in row
+ * order), scores[b] the score so far of wanted row b; of every group the k best continuations come back as
+ * elb_beam_select_dev gives them (parent counts the wanted rows). scores, parent, token and score are host memory. */
+int elb_model_eval_batch_beam(elb_model* m, int n, const int32_t* tokens, const int32_t* seq, const int32_t* pos, const uint8_t* want,
+                              int n_group, int beams, const double* scores, int k, int32_t* parent, int32_t* token, double* score);
+
+/* A paged cache instead of n_ctx contiguous fp32 rows per sequence: between create and finalize, n_pages pages of `page`
+ * positions for all n_seq sequences together, values as in elb_kv_create (ELB_KV_F16, ELB_KV_PAIR). Pages are given out as
+ * sequences grow; when none is left, an evaluation returns ELB_ERR_MEMORY and changes nothing. A sequence's rows must start at
+ * most at its length, and cut it there. Every evaluation runs as a batch of rows through elb_kv_append_dev and
+ * elb_kv_attention_dev; the single-kernel decode step needs the contiguous cache. Not under tensor parallelism. */
+int elb_model_set_pages(elb_model* m, int page, int n_pages, int type);
+/* Sequence seq[i] goes on from the state of sequence parent[i], for all i at once (a beam search's step, or a shared prefix);
+ * the other sequences stay as they are. Full pages are shared, last pages copied (elb_kv_reorder_dev). Paged models only. */
+int elb_model_reorder(elb_model* m, int n, const int32_t* seq, const int32_t* parent);
+/* Gives a sequence's pages back: its length is 0. */
+int elb_model_drop(elb_model* m, int seq);
+int elb_model_free_pages(const elb_model* m, int* n);
+
 /* n single-token steps at positions pos0.., enqueued back to back without reading logits back (the tg loop of the
  * reference's bench command, src/main.cpp:639, without its per-token host round trip). device_ms receives the device
  * time of the whole run (CUDA events on the model's stream). Same argument checks as elb_model_eval. */
