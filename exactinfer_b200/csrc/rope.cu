@@ -113,7 +113,7 @@ __device__ __forceinline__ void fill_angles(const RopeArgs& a, int tokens, const
 // Thread: unit u of every slots-th (token, head) pair of the block, RP_BATCH pairs at a time, whose loads go out together - the first
 // ones before the block knows its tokens.
 template <bool NORM>
-__global__ void __launch_bounds__(RP_THREADS) k_rope(const RopeArgs a, int tokens, int heads_per_block, int upt_log) {
+__global__ void __launch_bounds__(RP_THREADS, 4) k_rope(const RopeArgs a, int tokens, int heads_per_block, int upt_log) {
     __shared__ float2 cs[RP_TOKENS][RP_MAXHALF];
     __shared__ Tok tok[RP_TOKENS];
     __shared__ int seq[RP_TOKENS];
@@ -153,24 +153,38 @@ __global__ void __launch_bounds__(RP_THREADS) k_rope(const RopeArgs a, int token
             if (a.turns) fill_angles(a, tokens, tok, cs);
             __syncthreads();
         }
+        // Mean squares of the batch's four heads at once: the first two steps of the reduction across a head's lanes halve what a
+        // lane holds, so that it ends with one head's sum, and every lane forms one factor
+        float inv = 1.f;
+        if (NORM) {
+            static_assert(RP_BATCH == 4, "two halving steps");
+            double ss[4];
+#pragma unroll
+            for (int b = 0; b < 4; ++b) {
+                ss[b] = 0.0;
+#pragma unroll
+                for (int i = 0; i < 8; ++i) ss[b] = fma(double(v[b][i]), double(v[b][i]), ss[b]);
+            }
+            const bool odd = u & 1, third = u & 2;
+            const double k0 = odd ? ss[2] : ss[0], k1 = odd ? ss[3] : ss[1], g0 = odd ? ss[0] : ss[2], g1 = odd ? ss[1] : ss[3];
+            const double a0 = k0 + __shfl_xor_sync(0xffffffffu, g0, 1), a1 = k1 + __shfl_xor_sync(0xffffffffu, g1, 1);
+            double sum = (third ? a1 : a0) + __shfl_xor_sync(0xffffffffu, third ? a0 : a1, 2);
+            for (int o = 4; o < upt; o <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+            inv = inv_rms(sum * part + double(a.eps));  // of head 2 (u & 1) + (u / 2 & 1)
+        }
 #pragma unroll
         for (int b = 0; b < RP_BATCH; ++b) {
             const int h = ht[b], t = min(tk[b], tokens - 1);
             const bool is_v = h >= a.n_head + a.HKV, is_k = !is_v && h >= a.n_head, turn = turned && !is_v, ap = apart && !is_v;
             const int e0 = ap ? 4 * u : 8 * u, e1 = ap ? half + 4 * u : 8 * u + 4;
-            if (NORM && __any_sync(0xffffffffu, h >= 0 && !is_v)) {
-                double ss = 0.0;
-#pragma unroll
-                for (int i = 0; i < 8; ++i) ss += double(v[b][i]) * double(v[b][i]);
-                for (int o = upt / 2; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
+            if (NORM) {
+                const float mine = __shfl_sync(0xffffffffu, inv, (int(threadIdx.x) & 31 & ~3) | (b >> 1) | (b & 1) << 1);
                 const float* w = is_v ? nullptr : is_k ? a.k_norm : a.q_norm;
                 if (w && h >= 0) {
-                    const float inv = inv_rms(ss * part + double(a.eps));
+                    const float4 w0 = *reinterpret_cast<const float4*>(w + e0), w1 = *reinterpret_cast<const float4*>(w + e1);
+                    const float ww[8] = {w0.x, w0.y, w0.z, w0.w, w1.x, w1.y, w1.z, w1.w};
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        v[b][i] = __fmul_rn(__fmul_rn(v[b][i], inv), w[e0 + i]);
-                        v[b][i + 4] = __fmul_rn(__fmul_rn(v[b][i + 4], inv), w[e1 + i]);
-                    }
+                    for (int i = 0; i < 8; ++i) v[b][i] = __fmul_rn(__fmul_rn(v[b][i], mine), ww[i]);
                 }
             }
             if (turn) {
@@ -344,7 +358,7 @@ int rope_launch(const Rope* r, const float* x, int64_t ldx, float* y, int64_t ld
     a.turns = r->d_turns; a.dim = r->dim; a.layout = r->layout; a.head_dim = r->head_dim; a.mscale = r->mscale; a.eps = eps;
     a.q = x; a.q_out = y; a.q_norm = norm; a.ldq = ldx; a.ldqo = ldy; a.n_head = heads; a.n = n; a.pos = pos;
     const int d = r->head_dim;
-    if ((d == 32 || d == 64 || d == 128 || d == 256) && r->dim % 8 == 0 && aligned16(x, ldx) && aligned16(y, ldy)) return rope_run(a, s);
+    if ((d == 32 || d == 64 || d == 128 || d == 256) && r->dim % 8 == 0 && aligned16(x, ldx) && aligned16(y, ldy) && aligned16(norm, 0)) return rope_run(a, s);
     k_rope_any<<<dim3(unsigned(n), unsigned(std::min((heads + 7) / 8, n < 512 ? 8 : 1))), RP_THREADS, 0, s>>>(a);
     ELB_CUDA(cudaGetLastError());
     return ELB_OK;
@@ -365,6 +379,7 @@ int kv_append_launch(Kv* kv, int layer, const elb_kv_batch* b, const Rope* rope,
         if (!aligned16(q, ldq) || !aligned16(q_out, ldqo)) return fail(ELB_ERR_UNSUPPORTED, "kv_append: rows must start on 16-byte boundaries");
     }
     if ((k_norm || (q && q_norm)) && !(eps >= 0.f)) return fail(ELB_ERR_INVALID, "kv_append: eps must not be negative");
+    if (!aligned16(k_norm, 0) || (q && !aligned16(q_norm, 0))) return fail(ELB_ERR_UNSUPPORTED, "kv_append: norm weights must start on a 16-byte boundary");
     if (rope && (rope->head_dim != KV_D || rope->device != kv->device)) return fail(ELB_ERR_INVALID, "kv_append: the positions are for another head_dim or device");
     if (rope && rope->dim % 8) return fail(ELB_ERR_UNSUPPORTED, "kv_append: the rotated part of a head must be a multiple of 8");
     if (b->n_tok == 0 || b->n_seq == 0) return ELB_OK;

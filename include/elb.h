@@ -339,7 +339,8 @@ typedef struct {
 
 /* Keys and values of the new tokens into their pages of one layer: k = rotation(norm(k)), v as it is; with d_q also
  * q_out = rotation(norm(q)) for n_head query heads (q_out may be q with the same stride). rope NULL: no rotation. d_k_norm,
- * d_q_norm: [128] weights of the per-head RMSNorm or NULL. Row strides in floats; every row starts on a 16-byte boundary.
+ * d_q_norm: [128] weights of the per-head RMSNorm or NULL. Row strides in floats; every row, and the weights, start on a
+ * 16-byte boundary.
  * Rows that belong to nothing are left as they are, and so is their q_out. Two rows must not share a position. */
 int elb_kv_append_dev(elb_kv* kv, int layer, const elb_kv_batch* b, const elb_rope* rope, const float* d_k, int64_t ldk, const float* d_v,
                       int64_t ldv, const float* d_k_norm, float eps, const float* d_q, int64_t ldq, int n_head, const float* d_q_norm,

@@ -116,6 +116,15 @@ def test_rope_norm_beyond_fp32_squares(size):
     assert ((y - want).abs() <= 4 * U * want.abs()).all()
 
 
+def test_rope_norm_weights_anywhere():
+    g = gen(40)
+    r, x, w = e.Rope(128), randn(g, 5, 256), randn(g, 129) * 0.1 + 1
+    y, pos = torch.empty_like(x), torch.arange(5, device="cuda", dtype=torch.int32)
+    r.apply(x, pos, y, 5, 2, norm=w[1:], eps=1e-6, stream=stream())
+    want, tol = turned(normed(x.to(F64).view(5, 2, 128), w[1:], 1e-6), pos, r.config)
+    assert ((y.to(F64).view_as(want) - want).abs() <= tol + 4 * U * (want.abs() + tol / (4 * U))).all()
+
+
 def test_rope_refusals():
     r, x, p = e.Rope(128), torch.zeros(4, 256, device="cuda"), torch.zeros(4, device="cuda", dtype=torch.int32)
     for kw in (dict(n=-1), dict(heads=0), dict(ldx=255), dict(ldy=100), dict(y=None), dict(x=None), dict(pos=None), dict(eps=-1.0, norm=x)):
@@ -492,7 +501,7 @@ def test_attention_and_append_refusals():
                dict(rope=e.Rope(64))):
         with pytest.raises(ValueError):
             app(**kw)
-    for kw in (dict(k=x.data_ptr() + 4), dict(ldv=8 * D + 2), dict(rope=e.Rope(D, dim=6))):
+    for kw in (dict(k=x.data_ptr() + 4), dict(ldv=8 * D + 2), dict(rope=e.Rope(D, dim=6)), dict(k_norm=x.data_ptr() + 4)):
         with pytest.raises(e.ElbError):
             app(**kw)
     with pytest.raises(IndexError):
