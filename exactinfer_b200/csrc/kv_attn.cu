@@ -9,14 +9,24 @@
 
 namespace elb {
 
-// Up to 16 query rows per key head go to the narrow kernel, more to the 128-row tiles
-static bool few_rows(const Kv* kv, const elb_kv_batch* b, int n_head) {
-    return int64_t(std::min(b->max_q, b->n_tok)) * (n_head / kv->HKV) <= 16;
+// Up to 16 query rows per key head go to the narrow kernel, more to the 128-row tiles. A batch that may hold many sequences of
+// either kind (a server's step with a chunk of somebody's prompt in it) takes both, each for its sequences: 63 single tokens and a
+// chunk of 512 rows behind 100-4000 keys 296 -> 160 us. few_max: 0 for one kernel, else the rows up to which a sequence is
+// the narrow one's.
+constexpr int FEW_ROWS = 16;
+struct AttnWay { bool few, tile; int few_max; };
+static AttnWay attn_way(const elb_kv_batch* b, int group) {
+    const int64_t most = std::min(b->max_q, b->n_tok);
+    if (most * group <= FEW_ROWS) return {true, false, 0};
+    const bool both = b->n_seq >= 4 && 2 * int64_t(b->n_tok) < b->n_seq * most;
+    return {both, true, both ? FEW_ROWS : 0};
 }
+static size_t up256(size_t x) { return (x + 255) / 256 * 256; }
 
 size_t kv_attention_work(const Kv* kv, const elb_kv_batch* b, int n_head) {
     if (!kv || !b || n_head <= 0 || n_head % kv->HKV) return 0;
-    return std::max<size_t>(256, few_rows(kv, b, n_head) ? kv_attn_few_work(kv, b, n_head) : kv_attn_tile_work(kv, b, n_head));
+    const AttnWay w = attn_way(b, n_head / kv->HKV);
+    return std::max<size_t>(256, (w.few ? up256(kv_attn_few_work(kv, b, n_head, w.few_max)) : 0) + (w.tile ? kv_attn_tile_work(kv, b, n_head, w.few_max) : 0));
 }
 
 int kv_attention_launch(const Kv* kv, int layer, const elb_kv_batch* b, const float* q, int64_t ldq, int n_head, float scale, float* out,
@@ -40,8 +50,18 @@ int kv_attention_launch(const Kv* kv, int layer, const elb_kv_batch* b, const fl
     a.q = q; a.out = out; a.ldq = ldq; a.ldo = ldo;
     a.H = n_head; a.HKV = kv->HKV; a.group = n_head / kv->HKV; a.planes = kv->planes;
     a.scale2 = scale * 1.44269504088896340736f;
-    a.part = static_cast<float*>(work);
-    return few_rows(kv, b, n_head) ? kv_attn_few_launch(kv, a, b, s) : kv_attn_tile_launch(kv, layer, a, b, s);
+    const AttnWay w = attn_way(b, a.group);
+    a.few_max = w.few_max;
+    uint8_t* at = static_cast<uint8_t*>(work);
+    ELB_TRY(kv_attention_check());
+    if (w.few) {
+        a.part = reinterpret_cast<float*>(at);
+        at += up256(kv_attn_few_work(kv, b, n_head, w.few_max));
+        ELB_TRY(kv_attn_few_launch(kv, a, b, s));
+    }
+    if (!w.tile) return ELB_OK;
+    a.part = reinterpret_cast<float*>(at);
+    return kv_attn_tile_launch(kv, layer, a, b, s);
 }
 
 }  // namespace elb

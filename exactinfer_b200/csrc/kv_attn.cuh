@@ -14,9 +14,11 @@ struct KvAttnArgs {
     int H, HKV, group, planes;
     float scale2;        // scale * log2(e): weights are powers of two
     // the cut: tiles of R query rows (row r of a sequence and key head: token r / group, head r % group), their keys in `splits`
-    // ranges of `chunk` (the last takes what is left). Tiles from tiles_max on are not cut.
+    // ranges of `chunk` (the last takes what is left). Narrow kernel: tiles_max of every sequence, tiles from tiles_max on are not
+    // cut. 128-row tiles: tiles_max of all sequences together, counted through (kv_tile_of).
     int splits, chunk, tiles_max;
-    float* part;         // [sequence][tile][key head][split]: R rows of 128 sums, then R maxima, then R denominators
+    float* part;         // [tile][key head][split]: R rows of 128 sums, then R maxima, then R denominators
+    int few_max;         // both kernels run: sequences of up to so many query rows belong to the narrow one (0: one kernel has all)
 };
 
 constexpr float KA_P = 14.f;  // weights are formed as 2^(x - m + 14): small ones keep their bits in fp16
@@ -25,6 +27,40 @@ constexpr float KA_P = 14.f;  // weights are formed as 2^(x - m + 14): small one
 __device__ __forceinline__ int kv_visible(const KvRows& b, const KvSeq& s, int t) {
     const int64_t cap = b.table_ld << b.page_log;
     return int(min(int64_t(max(s.len - s.nq + t + 1, 0)), cap));
+}
+
+// The u-th 128-row tile of a batch: its sequence and its number there; false when there are fewer. A whole warp calls it with the same u.
+__device__ __forceinline__ bool kv_tile_of(const KvAttnArgs& a, int u, int* s, int* i) {
+    if (a.rows.n_seq == 1) {
+        *s = 0;
+        *i = u;
+        const KvSeq q = kv_seq(a.rows, 0);
+        return int64_t(u) * 128 < int64_t(q.nq) * a.group;
+    }
+    const int lane = threadIdx.x & 31;
+    for (int s0 = 0; s0 < a.rows.n_seq; s0 += 32) {
+        int tiles = 0;
+        if (s0 + lane < a.rows.n_seq) {
+            const int lo = min(max(a.rows.q_start[s0 + lane], 0), a.rows.n_tok);
+            const int rows = (min(max(a.rows.q_start[s0 + lane + 1], lo), a.rows.n_tok) - lo) * a.group;
+            tiles = rows > a.few_max ? (rows + 127) / 128 : 0;
+        }
+        int upto = tiles;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const int x = __shfl_up_sync(0xffffffffu, upto, o);
+            if (lane >= o) upto += x;
+        }
+        const unsigned here = __ballot_sync(0xffffffffu, upto > u);
+        if (here) {
+            const int l = __ffs(int(here)) - 1;
+            *s = s0 + l;
+            *i = u - __shfl_sync(0xffffffffu, upto - tiles, l);
+            return true;
+        }
+        u -= __shfl_sync(0xffffffffu, upto, 31);
+    }
+    return false;
 }
 
 __device__ __forceinline__ float ex2(float x) {
@@ -69,10 +105,10 @@ __device__ __forceinline__ RowScale row_scale(float m, float scale2) {
 }
 
 int kv_attn_few_launch(const Kv* kv, KvAttnArgs a, const elb_kv_batch* b, cudaStream_t s);
-size_t kv_attn_few_work(const Kv* kv, const elb_kv_batch* b, int n_head);
+size_t kv_attn_few_work(const Kv* kv, const elb_kv_batch* b, int n_head, int few_max);
 // rows whose keys were cut: `tiles` tiles of `rows` (8, 16 or 128) query rows
 int kv_attn_join(const KvAttnArgs& a, int rows, int64_t tiles, cudaStream_t s);
 int kv_attn_tile_launch(const Kv* kv, int layer, KvAttnArgs a, const elb_kv_batch* b, cudaStream_t s);
-size_t kv_attn_tile_work(const Kv* kv, const elb_kv_batch* b, int n_head);
+size_t kv_attn_tile_work(const Kv* kv, const elb_kv_batch* b, int n_head, int few_max);
 
 }  // namespace elb

@@ -63,6 +63,7 @@ __global__ void __launch_bounds__(KF_THREADS) k_kv_attn_few(const KvAttnArgs a) 
     const int i0 = int(x % a.tiles_max), s = int(x / a.tiles_max);
     const KvSeq sq = kv_seq(a.rows, s);
     const int nrows = sq.nq * a.group;
+    if (a.few_max && nrows > a.few_max) return;
     const int64_t plane = int64_t(a.rows.page) * KV_D, head = PL * plane;
     const uint32_t ring = uint32_t(__cvta_generic_to_shared(few_smem)) + uint32_t(warp) * (S::STAGES * S::STAGE);
 
@@ -310,9 +311,16 @@ __global__ void __launch_bounds__(256) k_kv_attn_join(const KvAttnArgs a) {
     const int64_t slot = x * a.splits;
     const int j = int(x % a.HKV);
     x /= a.HKV;
-    const int i = int(x % a.tiles_max), s = int(x / a.tiles_max);
-    if (s >= a.rows.n_seq) return;
+    int i = 0, s = 0;
+    if (ROWS == 128) {
+        if (x >= a.tiles_max || !kv_tile_of(a, int(x), &s, &i)) return;
+    } else {
+        i = int(x % a.tiles_max);
+        s = int(x / a.tiles_max);
+        if (s >= a.rows.n_seq) return;
+    }
     const KvSeq sq = kv_seq(a.rows, s);
+    if (ROWS != 128 && a.few_max && sq.nq * a.group > a.few_max) return;
     const int row = i * ROWS + r;
     if (row >= sq.nq * a.group) return;
     const int vis = kv_visible(a.rows, sq, min(((i + 1) * ROWS - 1) / a.group, sq.nq - 1));
@@ -339,11 +347,13 @@ __global__ void __launch_bounds__(256) k_kv_attn_join(const KvAttnArgs a) {
 
 struct FewPlan { int nt, tiles, splits, chunk; };
 
-FewPlan few_plan(const Kv* kv, const elb_kv_batch* b, int n_head) {
+FewPlan few_plan(const Kv* kv, const elb_kv_batch* b, int n_head, int few_max) {
     FewPlan p{};
     const int group = n_head / kv->HKV;
-    const int64_t rows = int64_t(std::max(1, std::min(b->max_q, b->n_tok))) * group;
-    p.nt = rows > 8 ? 2 : 1;
+    int64_t rows = int64_t(std::max(1, std::min(b->max_q, b->n_tok))) * group;
+    if (few_max) rows = few_max;
+    // (beside the other kernel: mostly single tokens, whose rows fill one group of 8 when the heads do)
+    p.nt = rows > 8 && !(few_max && group <= 8) ? 2 : 1;
     p.tiles = int((rows + 8 * p.nt - 1) / (8 * p.nt));
     const int resident = kv->sm_count * (kv->planes == 1 ? 2 : 1);
     const int64_t base = int64_t(b->n_seq) * kv->HKV * p.tiles;
@@ -376,14 +386,14 @@ int kv_attn_join(const KvAttnArgs& a, int rows, int64_t tiles, cudaStream_t s) {
     return ELB_OK;
 }
 
-size_t kv_attn_few_work(const Kv* kv, const elb_kv_batch* b, int n_head) {
-    const FewPlan p = few_plan(kv, b, n_head);
+size_t kv_attn_few_work(const Kv* kv, const elb_kv_batch* b, int n_head, int few_max) {
+    const FewPlan p = few_plan(kv, b, n_head, few_max);
     if (p.splits == 1) return 0;
     return size_t(b->n_seq) * p.tiles * kv->HKV * p.splits * 8 * p.nt * (KV_D + 2) * 4;
 }
 
 int kv_attn_few_launch(const Kv* kv, KvAttnArgs a, const elb_kv_batch* b, cudaStream_t s) {
-    const FewPlan p = few_plan(kv, b, a.H);
+    const FewPlan p = few_plan(kv, b, a.H, a.few_max);
     a.splits = p.splits; a.chunk = p.chunk; a.tiles_max = p.tiles;
     const int64_t blocks = int64_t(b->n_seq) * p.tiles * kv->HKV;
     if (blocks * p.splits > 0x7fffffff || blocks * 2 * p.nt > 0x7fffffff) return fail(ELB_ERR_UNSUPPORTED, "kv_attention: too many rows");

@@ -53,7 +53,6 @@ struct TileBars {
 
 __device__ __forceinline__ uint32_t su32(const void* p) { return uint32_t(__cvta_generic_to_shared(p)); }
 __device__ __forceinline__ void bar_init(uint64_t* b, int count) { asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(su32(b)), "r"(count) : "memory"); }
-__device__ __forceinline__ void bar_inval(uint64_t* b) { asm volatile("mbarrier.inval.shared::cta.b64 [%0];" ::"r"(su32(b)) : "memory"); }
 __device__ __forceinline__ void bar_expect(uint64_t* b, uint32_t bytes) {
     asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(su32(b)), "r"(bytes) : "memory");
 }
@@ -273,40 +272,33 @@ __global__ void __launch_bounds__(KT_THREADS, 1) k_kv_attn_tile(const __grid_con
     float* ex = reinterpret_cast<float*>(smem + S::RING + 1024);  // [2][128] x 2 words between the teams
     const int tid = threadIdx.x, warp = uniform(tid >> 5), lane = tid & 31;
     TileJob b;
-    {   // block -> (tile, sequence, key head, split): the last tiles, which see most, first; splits fastest
-        int64_t x = blockIdx.x;
-        b.c = int(x % a.splits);
-        x /= a.splits;
-        b.j = int(x % a.HKV);
-        x /= a.HKV;
-        b.s = int(x % a.rows.n_seq);
-        b.i = a.tiles_max - 1 - int(x / a.rows.n_seq);
-    }
     if (warp == 9) {
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(su32(&bars->tmem)) : "memory");
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
     }
-    b.sq = kv_seq(a.rows, b.s);
-    const int nrows = uniform(b.sq.nq * a.group);
+    // block -> (tile, key head, split): the last tiles, which see most of a sequence, first; splits fastest
+    int64_t bx = blockIdx.x;
+    b.c = int(bx % a.splits);
+    bx /= a.splits;
+    b.j = int(bx % a.HKV);
+    const int u = a.tiles_max - 1 - int(bx / a.HKV);
+    bool work = kv_tile_of(a, u, &b.s, &b.i);
+    int nrows = 0;
+    if (work) {
+        b.sq = kv_seq(a.rows, b.s);
+        nrows = uniform(b.sq.nq * a.group);
+        b.vis = uniform(kv_visible(a.rows, b.sq, min(((b.i + 1) * KT_ROWS - 1) / a.group, b.sq.nq - 1)));
+        b.vis_min = uniform(kv_visible(a.rows, b.sq, b.i * KT_ROWS / a.group));
+        b.cut = a.splits > 1;
+        b.kb = b.c * a.chunk;
+        b.ke = b.c < a.splits - 1 ? min(b.vis, b.kb + a.chunk) : b.vis;
+        work = !b.c || b.kb < b.ke;  // (an empty range: the join does not look at it)
+        b.tiles = uniform(max(0, (b.ke - b.kb + KT_KEYS - 1) / KT_KEYS));
+        // edge tiles: those with keys that not every row sees, and a last one that ends inside (at most 3)
+        b.edge0 = uniform(max(0, min(b.vis_min, b.vis / KT_KEYS * KT_KEYS) - b.kb) / KT_KEYS);
+    }
     if (tid == 0) bars->fail = 0;
     bool ok = true;
-    // the next tile of query rows of this CTA (more than one only when there are more rows than announced)
-    auto take = [&]() {
-        for (;; b.i += a.tiles_max) {
-            if (b.i * KT_ROWS >= nrows) return false;
-            b.cut = a.splits > 1 && b.i < a.tiles_max;
-            if (!b.cut && b.c) return false;
-            b.vis = uniform(kv_visible(a.rows, b.sq, min(((b.i + 1) * KT_ROWS - 1) / a.group, b.sq.nq - 1)));
-            b.vis_min = uniform(kv_visible(a.rows, b.sq, b.i * KT_ROWS / a.group));
-            b.kb = b.cut ? b.c * a.chunk : 0;
-            b.ke = b.cut && b.c < a.splits - 1 ? min(b.vis, b.kb + a.chunk) : b.vis;
-            if (b.c && b.kb >= b.ke) continue;  // nothing here; the join does not look at it
-            b.tiles = uniform(max(0, (b.ke - b.kb + KT_KEYS - 1) / KT_KEYS));
-            // edge tiles: those with keys that not every row sees, and a last one that ends inside (at most 3)
-            b.edge0 = uniform(max(0, min(b.vis_min, b.vis / KT_KEYS * KT_KEYS) - b.kb) / KT_KEYS);
-            return true;
-        }
-    };
     auto all_here = [] { asm volatile("bar.sync 0, %0;" ::"n"(KT_THREADS) : "memory"); };
     // Ring elements in the order of use: K0, K1, V0, K2, V1, K3, V2, ...: K of tile n is element 2n - 1 (K0: 0), V is 2n + 2
     // (the last tile's one earlier: no K comes before it)
@@ -316,7 +308,7 @@ __global__ void __launch_bounds__(KT_THREADS, 1) k_kv_attn_tile(const __grid_con
     if (warp >= 8) {
         // 384 threads start with 168 registers; 128 of them give what the 256 rows take: 128 * 56 + 256 * 224 = 384 * 168
         asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
-        for (; take(); b.i += a.tiles_max) {
+        if (work) {
         const int N = b.tiles, edge0 = b.edge0;
         before_sync();
         all_here();
@@ -466,11 +458,10 @@ __global__ void __launch_bounds__(KT_THREADS, 1) k_kv_attn_tile(const __grid_con
         before_sync();
         all_here();
         after_sync();
-        if (bars->fail) break;
         }
     } else {
         asm volatile("setmaxnreg.inc.sync.aligned.u32 224;");
-        for (; take(); b.i += a.tiles_max) {
+        if (work) {
         const int N = b.tiles, edge0 = b.edge0;
             // queries: a warp copies 16 whole rows into the end of the ring, then every thread takes half of its row to tensor
             // memory as hi | lo (a thread per row straight from global memory: 10000 clocks)
@@ -621,7 +612,7 @@ __global__ void __launch_bounds__(KT_THREADS, 1) k_kv_attn_tile(const __grid_con
                 const float2 x = parts(O[d / 2]), y = parts(O[d / 2 + 1]);
                 own_row[d / 4] = make_float4(x.x * ki, x.y * ki, y.x * ki, y.y * ki);
             }
-            const int64_t slot = ((int64_t(b.s) * a.tiles_max + b.i) * a.HKV + b.j) * a.splits + b.c;
+            const int64_t slot = (int64_t(u) * a.HKV + b.j) * a.splits + b.c;
             float* part = a.part + slot * KT_ROWS * (KV_D + 2);
             if (!final_here && team == 0) { part[KT_ROWS * KV_D + r] = M; part[KT_ROWS * (KV_D + 1) + r] = den; }
             asm volatile("bar.sync 1, 256;" ::: "memory");
@@ -636,17 +627,9 @@ __global__ void __launch_bounds__(KT_THREADS, 1) k_kv_attn_tile(const __grid_con
                 }
             }
         }
-        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");  // the ring is written by TMA again
         before_sync();
         all_here();
         after_sync();
-        if (bars->fail) break;
-        if (tid == 0) {
-            for (int s = 0; s < S::SLOTS; ++s) { bar_inval(bars->full + s); bar_inval(bars->empty + s); }
-            for (int w = 0; w < 2; ++w) { bar_inval(bars->s_full + w); bar_inval(bars->pv_ready + w); bar_inval(bars->o_full + w); }
-            bar_inval(&bars->q_full);
-            for (int k = 0; k < KT_MAXEDGE; ++k) { bar_inval(bars->go + k); bar_inval(bars->edge + k); }
-        }
         }
     }
     all_here();
@@ -664,13 +647,15 @@ int* tile_error_word() {  // pinned, mapped: raised by a kernel whose bounded wa
     return host;
 }
 
-struct TilePlan { int tiles, splits, chunk; };
+struct TilePlan { int64_t tiles; int splits, chunk; };
 
-TilePlan tile_plan(const Kv* kv, const elb_kv_batch* b, int n_head) {
+// few_max: sequences of up to so many query rows belong to the narrow kernel
+TilePlan tile_plan(const Kv* kv, const elb_kv_batch* b, int n_head, int few_max) {
     TilePlan p{};
-    const int64_t rows = int64_t(std::max(1, std::min(b->max_q, b->n_tok))) * (n_head / kv->HKV);
-    p.tiles = int((rows + KT_ROWS - 1) / KT_ROWS);
-    const int64_t base = int64_t(b->n_seq) * kv->HKV * p.tiles;
+    const int64_t rows = int64_t(b->n_tok) * (n_head / kv->HKV);
+    // tiles of 128 rows: whatever the sequences' lengths are, each adds at most one that is not full
+    p.tiles = b->n_seq == 1 ? (rows + KT_ROWS - 1) / KT_ROWS : rows / KT_ROWS + std::min<int64_t>(b->n_seq, rows / (few_max + 1));
+    const int64_t base = kv->HKV * std::max<int64_t>(p.tiles, 1);
     const int len = std::max(b->max_len, 1);
     // A CTA's start and end cost as much as 5 tiles of keys: one wave of long ranges when all sequences are alike, two when they may
     // not be, and at least 4 tiles each (nine turns behind 203-4100 keys: four waves 90 us, two 60)
@@ -692,20 +677,20 @@ int kv_attention_check() {  // did a call's kernel give up on a wait?
     return ELB_OK;
 }
 
-size_t kv_attn_tile_work(const Kv* kv, const elb_kv_batch* b, int n_head) {
-    const TilePlan p = tile_plan(kv, b, n_head);
+size_t kv_attn_tile_work(const Kv* kv, const elb_kv_batch* b, int n_head, int few_max) {
+    const TilePlan p = tile_plan(kv, b, n_head, few_max);
     if (p.splits == 1) return 0;
-    return size_t(b->n_seq) * p.tiles * kv->HKV * p.splits * KT_ROWS * (KV_D + 2) * 4;
+    return size_t(p.tiles) * kv->HKV * p.splits * KT_ROWS * (KV_D + 2) * 4;
 }
 
 int kv_attn_tile_launch(const Kv* kv, int layer, KvAttnArgs a, const elb_kv_batch* b, cudaStream_t s) {
     int* err = nullptr;
     if (!tile_error_word() || cudaHostGetDevicePointer(&err, tile_error_word(), 0) != cudaSuccess) return fail(ELB_ERR_CUDA, "kv_attention: no error word");
-    ELB_TRY(kv_attention_check());
-    const TilePlan p = tile_plan(kv, b, a.H);
-    a.splits = p.splits; a.chunk = p.chunk; a.tiles_max = p.tiles;
-    const int64_t blocks = int64_t(b->n_seq) * p.tiles * kv->HKV;
+    const TilePlan p = tile_plan(kv, b, a.H, a.few_max);
+    const int64_t blocks = p.tiles * kv->HKV;
     if (blocks * p.splits > 0x7fffffff || blocks * KT_ROWS / 8 > 0x7fffffff) return fail(ELB_ERR_UNSUPPORTED, "kv_attention: too many rows");
+    if (blocks == 0) return ELB_OK;
+    a.splits = p.splits; a.chunk = p.chunk; a.tiles_max = int(p.tiles);
     const int64_t layer_rows = kv->layer_halves() / KV_D;
     auto run = [&](auto kernel, int smem) -> int {
         ELB_TRY(ensure_dyn_smem(reinterpret_cast<const void*>(kernel), size_t(smem)));

@@ -408,6 +408,26 @@ def test_expectations_do_not_change_results(nq, max_q, max_len):
     check(p, 8)
 
 
+@pytest.mark.parametrize("kind", (e.KV_F16, e.KV_PAIR))
+@pytest.mark.parametrize("h,hkv", [(8, 2), (24, 2), (4, 4)])
+@pytest.mark.parametrize("order", (0, 1))
+def test_single_tokens_and_chunks_in_one_batch(order, h, hkv, kind):
+    """A server's step: one token of most sequences, chunks of some, nothing of others, rows in front of and behind them all."""
+    nq = [1, 1, 1, 40, 1, 0, 1, 9, 1, 4, 1, 1, 70, 1, 2, 1] + [1] * 40
+    lens = [300, 5, 1, 700, 16, 33, 1200, 9, 64, 400, 17, 1, 70, 250, 1, 90] + list(range(1, 400, 10))
+    if order:
+        nq, lens = nq[::-1], lens[::-1]
+    p = Paged(33, hkv, 16, kind, nq, lens, extra_rows=3, gap=2).fill()
+    q = randn(p.g, p.n_tok, h * D)
+    want, tol = p.expected(h, q)
+    r = p.rows()
+    for max_q, max_len in ((70, 1200), (1, 1200), (200, 1), (30, 5000)):
+        p.batch = e.KvBatch(len(nq), p.n_tok, max_q, max_len, p.d_start, p.d_len, p.d_table, p.width)
+        got = p.attention(h, q, out=torch.full_like(q, 7.0))
+        assert ((got[r].to(F64) - want[r]).abs() <= tol[r]).all()
+        assert (got[:2] == 7).all() and (got[-3:] == 7).all()
+
+
 def test_lengths_beyond_the_table():
     """More positions than the table has pages for: nothing outside is read; the keys that there are count, with zeros behind."""
     p = Paged(20, 2, 16, 1, (1, 40), (48, 64), width=4).fill()
