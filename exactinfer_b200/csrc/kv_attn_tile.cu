@@ -306,8 +306,8 @@ __global__ void __launch_bounds__(KT_THREADS, 1) k_kv_attn_tile(const __grid_con
     auto v_elem = [&](int n) { return n == b.tiles - 1 ? 2 * n + 1 : 2 * n + 2; };
 
     if (warp >= 8) {
-        // 384 threads start with 168 registers; 128 of them give what the 256 rows take: 128 * 56 + 256 * 224 = 384 * 168
-        asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
+        // 384 threads start with 168 registers; 128 of them give what the 256 of the rows take: 128 * 80 + 256 * 208 <= 384 * 168
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 80;");
         if (work) {
         const int N = b.tiles, edge0 = b.edge0;
         before_sync();
@@ -460,7 +460,7 @@ __global__ void __launch_bounds__(KT_THREADS, 1) k_kv_attn_tile(const __grid_con
         after_sync();
         }
     } else {
-        asm volatile("setmaxnreg.inc.sync.aligned.u32 224;");
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 208;");
         if (work) {
         const int N = b.tiles, edge0 = b.edge0;
             // queries: a warp copies 16 whole rows into the end of the ring, then every thread takes half of its row to tensor
@@ -658,7 +658,9 @@ TilePlan tile_plan(const Kv* kv, const elb_kv_batch* b, int n_head, int few_max)
     const int64_t base = kv->HKV * std::max<int64_t>(p.tiles, 1);
     const int len = std::max(b->max_len, 1);
     // A CTA's start and end cost as much as 5 tiles of keys: one wave of long ranges when all sequences are alike, two when they may
-    // not be, and at least 4 tiles each (nine turns behind 203-4100 keys: four waves 90 us, two 60)
+    // not be, and at least 4 tiles each. Cut for two, three or four waves (us): 9 turns of 3-77 tokens behind 203-4100 keys, pairs, 95, 80,
+    // 88; 9 of 64 tokens at 4096 keys 57, 77, 69; 3 of 300 tokens at 2000 keys 95, 95, 129. (All key tiles of a batch dealt
+    // out evenly over one CTA per SM, which walks from tile to tile: a launch before and a join behind it, 93, 73, 123 us.)
     int64_t want = base >= 2 * kv->sm_count ? 1 : std::max<int64_t>(1, int64_t(kv->sm_count) * (b->n_seq > 1 ? 2 : 1) / base);
     want = std::min<int64_t>(want, (len + 4 * KT_KEYS - 1) / (4 * KT_KEYS));
     p.chunk = int((len + want - 1) / want + KT_KEYS - 1) / KT_KEYS * KT_KEYS;
