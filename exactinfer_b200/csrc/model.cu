@@ -1240,13 +1240,12 @@ static int paged_batch(Model* m, int n, const int32_t* seq, const int32_t* pos, 
         ++count[size_t(seq[i])];
     }
     PageBook& book = m->book;
-    int64_t need = 0;
-    for (int s = 0; s < S; ++s) {
-        if (!count[size_t(s)]) continue;
-        if (first[size_t(s)] > book.len[size_t(s)]) return fail(ELB_ERR_RANGE, "eval_batch: a sequence's rows must continue what it has cached");
-        need += book.need(s, first[size_t(s)], first[size_t(s)] + count[size_t(s)]);
-    }
-    if (need > int64_t(book.free.size())) return fail(ELB_ERR_MEMORY, "eval_batch: no free page left in the cache");
+    for (int s = 0; s < S; ++s)
+        if (count[size_t(s)] && first[size_t(s)] > book.len[size_t(s)])
+            return fail(ELB_ERR_RANGE, "eval_batch: a sequence's rows must continue what it has cached");
+    if (!book.fits(first, count)) return fail(ELB_ERR_MEMORY, "eval_batch: no free page left in the cache");
+    for (int s = 0; s < S; ++s)
+        if (count[size_t(s)]) book.shorten(s, first[size_t(s)]);
     int at = 0, max_q = 1, max_len = 1;
     for (int s = 0; s < S; ++s) {
         m->rows_host[s] = at;
@@ -1262,7 +1261,10 @@ static int paged_batch(Model* m, int n, const int32_t* seq, const int32_t* pos, 
             const int width = p0 / m->page + 1;
             two.insert(two.end(), t.begin(), t.begin() + width);
             int* d = nullptr;
-            ELB_CUDA(cudaMalloc(&d, (two.size() + 4 + size_t(2) * width) * sizeof(int)));
+            if (cudaMalloc(&d, (two.size() + 4 + size_t(2) * width) * sizeof(int)) != cudaSuccess) {
+                book.drop(mine);
+                return fail(ELB_ERR_MEMORY, "eval_batch: out of device memory");
+            }
             int* out = d + two.size();
             cudaError_t e = cudaMemcpyAsync(d, two.data(), two.size() * sizeof(int), cudaMemcpyHostToDevice, m->stream);
             const int rc = e == cudaSuccess ? kv_reorder_launch(m->kv, 2, d, d + 4, d + 6, width, d + 2, out, out + 4, out + 2, m->stream) : ELB_OK;
@@ -1277,7 +1279,6 @@ static int paged_batch(Model* m, int n, const int32_t* seq, const int32_t* pos, 
             book.drop(t[size_t(p0 / m->page)]);
             t[size_t(p0 / m->page)] = mine;
         }
-        book.shorten(s, p0);
         while (int(t.size()) < book.pages_of(p1)) t.push_back(book.take());
         book.len[size_t(s)] = p1;
         m->rows_host[S + 1 + s] = p1;

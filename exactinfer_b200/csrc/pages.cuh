@@ -2,6 +2,7 @@
 #pragma once
 
 #include <algorithm>
+#include <cstdint>
 #include <vector>
 
 namespace elb {
@@ -40,11 +41,36 @@ struct PageBook {
         }
         len[size_t(s)] = std::min(len[size_t(s)], positions);
     }
-    // free pages that sequence s needs to be written from position p0 (<= len) to p1 (exclusive): new ones, and one for a last page
+    // the most free pages that sequence s needs to be written from position p0 (<= len) to p1 (exclusive): new ones, and one for a last page
     // that it keeps in part and shares
     int need(int s, int p0, int p1) const {
         const int kept = std::min(pages_of(p0), int(table[size_t(s)].size()));
         return std::max(0, pages_of(p1) - kept) + (shared_tail(s, p0) ? 1 : 0);
+    }
+    // Are there pages for count[s] rows of every sequence s from first[s] on? Exactly: with what the sequences themselves give back
+    bool fits(const std::vector<int>& first, const std::vector<int>& count) const {
+        int64_t most = 0;
+        for (size_t s = 0; s < count.size(); ++s)
+            if (count[s]) most += need(int(s), first[s], first[s] + count[s]);
+        if (most <= int64_t(free.size())) return true;
+        PageBook b = *this;
+        for (size_t s = 0; s < count.size(); ++s)
+            if (count[s]) b.shorten(int(s), first[s]);
+        for (size_t s = 0; s < count.size(); ++s) {
+            if (!count[s]) continue;
+            auto& t = b.table[s];
+            if (b.shared_tail(int(s), first[s])) {
+                if (b.free.empty()) return false;
+                const int mine = b.take();
+                b.drop(t.back());
+                t.back() = mine;
+            }
+            while (int(t.size()) < b.pages_of(first[s] + count[s])) {
+                if (b.free.empty()) return false;
+                t.push_back(b.take());
+            }
+        }
+        return true;
     }
     bool shared_tail(int s, int p0) const { return p0 % page && refs[size_t(table[size_t(s)][size_t(p0 / page)])] > 1; }
     // sequences 0.. go on from parent[s]: who needs a copy of the parent's last page (the rule of elb_kv_reorder_dev)

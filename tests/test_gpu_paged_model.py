@@ -297,3 +297,37 @@ def test_refusals(models):
         with pytest.raises(ValueError):
             beam(**kw)
     beam()
+
+
+def test_pages_that_the_rows_themselves_give_back(models):
+    """A full pool: a sequence that starts over, and one that shares the last page of another, need only what they do not free."""
+    spec, make, flat = models
+    rng = np.random.default_rng(21)
+    paged = make(pages=(16, 4, e.KV_PAIR))
+    a, b = rng.integers(0, spec.n_vocab, 32), rng.integers(0, spec.n_vocab, 32)
+    for s in (0, 1):  # two pages each: none is left
+        assert rel(prompt(paged, s, a), prompt(flat, s, a)) <= REL_TOL
+    assert paged.free_pages() == 0
+    assert rel(prompt(paged, 0, b), prompt(flat, 0, b)) <= REL_TOL  # from position 0 on, over its own pages
+    # both at once: one gives back a page that the other takes
+    toks, seq = np.concatenate([b[:8], a[:16]]), [0] * 8 + [1] * 16
+    pos, want = list(range(8)) + list(range(32, 48)), np.array([0] * 7 + [1] + [0] * 15 + [1], np.uint8)
+    assert rel(paged.eval_batch(toks, seq, pos, want), flat.eval_batch(toks, seq, pos, want)) <= REL_TOL
+    assert paged.free_pages() == 0
+    # the sixth sequence goes on from the first, whose 8 rows fill half a page: no page for the copy; a full page is shared
+    with pytest.raises(MemoryError):
+        paged.reorder([5], [0])
+    paged.drop(1)
+    prompt(paged, 0, b[:16])
+    paged.reorder([5], [0])
+    assert paged.free_pages() == 3
+    for s in (2, 3):
+        prompt(paged, s, a[:16])
+    assert paged.free_pages() == 1
+    # both write from position 8 of the page they share: one copy, the other keeps the page
+    prompt(flat, 0, b[:16])
+    prompt(flat, 5, b[:16])
+    toks, seq, pos = np.concatenate([a[:4], b[20:24]]), [0] * 4 + [5] * 4, list(range(8, 12)) * 2
+    want = np.array([0, 0, 0, 1] * 2, np.uint8)
+    assert rel(paged.eval_batch(toks, seq, pos, want), flat.eval_batch(toks, seq, pos, want)) <= REL_TOL
+    assert paged.free_pages() == 0
