@@ -125,7 +125,14 @@ __global__ void __launch_bounds__(BS_THREADS, 5) k_beam_segments(const float* __
             mx = here;
         }
         // Terms below e^-700 of the largest, and places behind the row's end, count as e^-700: nothing beside the largest's 1
-        if (mx > -INFINITY) {
+        if (fabsf(mx) >= 16777216.f && mx > -INFINITY) {  // mx - 700 is no fp32 number
+            const double from = mx;
+#pragma unroll
+            for (int j = 0; j < BS_PER; ++j) {
+                const double y = double(v[j]) - from;
+                sum = add_exp(sum, y < -700.0 ? -700.0 : y, tab);
+            }
+        } else if (mx > -INFINITY) {
             const float low = mx - 700.f;
             const double from = mx;
 #pragma unroll
@@ -354,6 +361,13 @@ int beam_select_launch(int device, const float* logits, int64_t ld, int n_vocab,
     if (reinterpret_cast<uintptr_t>(work) % 256) return fail(ELB_ERR_INVALID, "beam_select: the work buffer must start on a 256-byte boundary");
     DeviceScope on(device);
     if (on.rc != ELB_OK) return on.rc;
+    // A row's block reads its score at its start, and a group's results come behind all of its rows: in place they may only stand
+    // where the group's own scores do.
+    const uintptr_t s0 = reinterpret_cast<uintptr_t>(scores), r0 = reinterpret_cast<uintptr_t>(score);
+    const size_t rows_bytes = size_t(n_group) * beams * sizeof(double), picks = size_t(n_group) * k;
+    auto touches = [&](const void* p, size_t n) { const uintptr_t x = reinterpret_cast<uintptr_t>(p); return x < s0 + rows_bytes && s0 < x + n; };
+    if (touches(parent, picks * 4) || touches(token, picks * 4) || (touches(score, picks * 8) && !(s0 == r0 && k == beams)))
+        return fail(ELB_ERR_INVALID, "beam_select: outputs must not overlap the scores (d_score may be d_scores when k = beams)");
     const int rows = n_group * beams;
     const BeamCut cut = beam_cut(n_vocab);
     uint8_t* at = static_cast<uint8_t*>(work);

@@ -76,7 +76,7 @@ __global__ void __launch_bounds__(KR_THREADS) k_kv_reorder(uint8_t* __restrict__
             int v = -1;
             if (i < used) {
                 v = table[p * table_ld + i];
-                if (second && i == used - 1 && unsigned(v) < unsigned(n_pages) && unsigned(spare[r]) < unsigned(n_pages)) v = spare[r];
+                if (second && i == used - 1 && unsigned(v) < unsigned(n_pages)) v = spare[r];  // (one outside the pool: not the first child's page either)
             }
             table_out[r * table_ld + i] = v;
         }
@@ -133,6 +133,8 @@ int kv_create(int device, int n_layer, int n_head_kv, int head_dim, int page, in
     cudaDriverEntryPointQueryResult q;
     if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &fp, cudaEnableDefault, &q) != cudaSuccess || q != cudaDriverEntryPointSuccess)
         return fail(ELB_ERR_CUDA, "kv_create: cuTensorMapEncodeTiled is not available");
+    ELB_TRY(kv_attention_prepare());
+    ELB_TRY(ensure_dyn_smem(reinterpret_cast<const void*>(k_kv_reorder), KR_MAXROWS * 12));
     auto* kv = new (std::nothrow) Kv;
     if (!kv) return fail(ELB_ERR_MEMORY, "kv_create: out of memory");
     kv->device = device; kv->n_layer = n_layer; kv->HKV = n_head_kv; kv->page = page; kv->n_pages = n_pages; kv->planes = type;
@@ -179,7 +181,7 @@ int kv_check_batch(const Kv* kv, int layer, const elb_kv_batch* b, const char* w
     if (b->n_seq > 65536) return fail(ELB_ERR_UNSUPPORTED, w + "more than 65536 sequences");
     if (b->n_seq > 0 && b->n_tok > 0 && (!b->d_q_start || !b->d_len || !b->d_table)) return fail(ELB_ERR_INVALID, w + "null argument");
     if (b->table_ld < 0 || (b->n_seq > 0 && b->table_ld == 0)) return fail(ELB_ERR_INVALID, w + "a page table needs a positive row stride");
-    if (b->table_ld > (int64_t(1) << 31) / kv->page) return fail(ELB_ERR_UNSUPPORTED, w + "tables for more than 2^31 positions");
+    if (b->table_ld > (int64_t(1) << 30) / kv->page) return fail(ELB_ERR_UNSUPPORTED, w + "tables for more than 2^30 positions");  // (a pool has fewer)
     return ELB_OK;
 }
 
@@ -203,7 +205,6 @@ int kv_reorder_launch(Kv* kv, int n, const int* parent, const int* len, const in
     DeviceScope on(kv->device);
     if (on.rc != ELB_OK) return on.rc;
     const size_t smem = size_t((n + 1) / 2 * 2) * 4 + size_t(n) * 8;
-    ELB_TRY(ensure_dyn_smem(reinterpret_cast<const void*>(k_kv_reorder), KR_MAXROWS * 12));
     const int64_t page_bytes = kv->page_halves() * 2, most = (int64_t(n) * kv->n_layer * page_bytes + KR_CHUNK - 1) / KR_CHUNK;
     const int grid = int(std::min<int64_t>(std::max<int64_t>(most, 1), int64_t(kv->sm_count) * 4));
     k_kv_reorder<<<grid, KR_THREADS, smem, s>>>(reinterpret_cast<uint8_t*>(kv->mem), kv->layer_halves() * 2, page_bytes, kv->n_layer, kv->n_pages,

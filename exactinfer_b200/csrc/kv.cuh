@@ -95,7 +95,8 @@ int kv_reorder_launch(Kv* kv, int n, const int* parent, const int* len, const in
 size_t kv_attention_work(const Kv* kv, const elb_kv_batch* b, int n_head);
 int kv_attention_launch(const Kv* kv, int layer, const elb_kv_batch* b, const float* q, int64_t ldq, int n_head, float scale, float* out,
                         int64_t ldo, void* work, size_t work_bytes, cudaStream_t s);
-int kv_attention_check();  // after a synchronize: did a kernel give up on a bounded wait?
+int kv_attention_prepare();  // on the current device: what a captured call must find in place
+int kv_attention_check();    // did a kernel of an earlier call give up on a bounded wait?
 // beam.cu
 size_t beam_select_work(int n_vocab, int n_group, int beams, int k);
 int beam_select_launch(int device, const float* logits, int64_t ld, int n_vocab, int n_group, int beams, const double* scores,

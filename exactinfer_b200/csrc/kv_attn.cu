@@ -23,6 +23,11 @@ static AttnWay attn_way(const elb_kv_batch* b, int group) {
 }
 static size_t up256(size_t x) { return (x + 255) / 256 * 256; }
 
+int kv_attention_prepare() {
+    ELB_TRY(kv_attn_few_prepare());
+    return kv_attn_tile_prepare();
+}
+
 size_t kv_attention_work(const Kv* kv, const elb_kv_batch* b, int n_head) {
     if (!kv || !b || n_head <= 0 || n_head % kv->HKV) return 0;
     const AttnWay w = attn_way(b, n_head / kv->HKV);

@@ -1,6 +1,8 @@
 // Attention over a paged cache: what its two kernels and the joining of their partial results share.
 #pragma once
 
+#include <algorithm>
+
 #include "kv.cuh"
 
 namespace elb {
@@ -104,6 +106,11 @@ __device__ __forceinline__ RowScale row_scale(float m, float scale2) {
     return r;
 }
 
+// Most positions of a sequence that the plans count with: what the caller expects, as far as the table goes (2^30 at most)
+inline int kv_most(const Kv* kv, const elb_kv_batch* b) { return int(std::max<int64_t>(1, std::min(int64_t(b->max_len), b->table_ld * kv->page))); }
+
+int kv_attn_few_prepare();
+int kv_attn_tile_prepare();
 int kv_attn_few_launch(const Kv* kv, KvAttnArgs a, const elb_kv_batch* b, cudaStream_t s);
 size_t kv_attn_few_work(const Kv* kv, const elb_kv_batch* b, int n_head, int few_max);
 // rows whose keys were cut: `tiles` tiles of `rows` (8, 16 or 128) query rows

@@ -357,7 +357,7 @@ FewPlan few_plan(const Kv* kv, const elb_kv_batch* b, int n_head, int few_max) {
     p.tiles = int((rows + 8 * p.nt - 1) / (8 * p.nt));
     const int resident = kv->sm_count * (kv->planes == 1 ? 2 : 1);
     const int64_t base = int64_t(b->n_seq) * kv->HKV * p.tiles;
-    const int len = std::max(b->max_len, 1);
+    const int len = kv_most(kv, b);
     // one sequence: one wave of equal ranges. Several: lengths differ, ranges short enough that the last ones even out
     int64_t want = b->n_seq == 1 ? std::max<int64_t>(1, resident / base) : std::max<int64_t>(1, (int64_t(resident) * 12 + base - 1) / base);
     want = std::min<int64_t>(want, (len + 255) / 256);
@@ -369,13 +369,19 @@ FewPlan few_plan(const Kv* kv, const elb_kv_batch* b, int n_head, int few_max) {
 template <int PL, int NT> int few_run(const KvAttnArgs& a, int64_t blocks, cudaStream_t s) {
     using S = FewShape<PL, NT>;
     auto kernel = k_kv_attn_few<PL, NT>;
-    ELB_TRY(ensure_dyn_smem(reinterpret_cast<const void*>(kernel), S::SMEM));
     kernel<<<unsigned(blocks * a.splits), KF_THREADS, S::SMEM, s>>>(a);
     ELB_CUDA(cudaGetLastError());
     return a.splits > 1 ? kv_attn_join(a, S::ROWS, blocks, s) : ELB_OK;
 }
 
 }  // namespace
+
+int kv_attn_few_prepare() {
+    ELB_TRY(ensure_dyn_smem(reinterpret_cast<const void*>(k_kv_attn_few<1, 1>), FewShape<1, 1>::SMEM));
+    ELB_TRY(ensure_dyn_smem(reinterpret_cast<const void*>(k_kv_attn_few<1, 2>), FewShape<1, 2>::SMEM));
+    ELB_TRY(ensure_dyn_smem(reinterpret_cast<const void*>(k_kv_attn_few<2, 1>), FewShape<2, 1>::SMEM));
+    return ensure_dyn_smem(reinterpret_cast<const void*>(k_kv_attn_few<2, 2>), FewShape<2, 2>::SMEM);
+}
 
 int kv_attn_join(const KvAttnArgs& a, int rows, int64_t tiles, cudaStream_t s) {
     const unsigned blocks = unsigned((tiles * rows + 7) / 8);

@@ -11,12 +11,15 @@
 //
 // Two teams of four warps work on alternate key tiles, a thread per query row (= TMEM lane), each with its own running
 // maximum, denominator and 128 sums, joined once at the end: while one team forms its weights, the tensor core
-// multiplies for the other. One warp brings keys and values by TMA, page by page, into a ring of 128-key tiles in the
-// order of their use; two warps issue the MMAs, one searches the values. TMEM: Q hi | lo (128 columns, the A operand of S: read from there, the
-// shared memory has only K to deliver), per team S (128 columns, overwritten by the weights hi | lo, the A operand of O) and one
-// O (128): a team takes it into its registers while the tensor core forms the next S. V lies [key][dimension] as in the page and is a B operand with N along the rows.
+// multiplies for the other. Warp 8 brings keys and values by TMA, page by page, into a ring of 128-key tiles in the order of their
+// use; warps 9 and 10 issue the MMAs, one per team; warp 11 searches the values of edge tiles. TMEM: Q hi | lo (128 columns, the A
+// operand of S: read from there, the shared memory has only K to deliver), per team S (128 columns, overwritten by the weights
+// hi | lo, the A operand of O) and one O (128): a team takes it into its registers while the tensor core forms the next S. V lies
+// [key][dimension] as in the page and is a B operand with N along the rows.
 // A tile's 128 keys take 2048 (F16) or 3 * 1024 (pairs) clocks of the tensor pipe. (64-key tiles: an MMA with N = 64 took 51
-// clocks instead of 32, and the whole 1860 a tile.)
+// clocks instead of 32, and the whole 1860 a tile.) What bounds it is the chain S, weights, O, sums of a tile with one O: the
+// tensor pipe is 54 % busy. 4096 causal rows, 32 query heads on 8: F16 260 us (528 TFLOP/s of useful products, 1056 of both
+// halves), pairs 330 us. (Four teams' warps with half a row a thread: 277 us.)
 //
 // Behind the last visible key the weights are 0, but 0 * NaN is not: the PV product stops at the last 16 keys, and the rows of
 // V behind the last key are emptied in shared memory. In the few tiles that only some rows see, V is searched for infinities and
@@ -656,7 +659,7 @@ TilePlan tile_plan(const Kv* kv, const elb_kv_batch* b, int n_head, int few_max)
     // tiles of 128 rows: whatever the sequences' lengths are, each adds at most one that is not full
     p.tiles = b->n_seq == 1 ? (rows + KT_ROWS - 1) / KT_ROWS : rows / KT_ROWS + std::min<int64_t>(b->n_seq, rows / (few_max + 1));
     const int64_t base = kv->HKV * std::max<int64_t>(p.tiles, 1);
-    const int len = std::max(b->max_len, 1);
+    const int len = kv_most(kv, b);
     // A CTA's start and end cost as much as 5 tiles of keys: one wave of long ranges when all sequences are alike, two when they may
     // not be, and at least 4 tiles each. Cut for two, three or four waves (us): 9 turns of 3-77 tokens behind 203-4100 keys, pairs, 95, 80,
     // 88; 9 of 64 tokens at 4096 keys 57, 77, 69; 3 of 300 tokens at 2000 keys 95, 95, 129. (All key tiles of a batch dealt
@@ -670,7 +673,13 @@ TilePlan tile_plan(const Kv* kv, const elb_kv_batch* b, int n_head, int few_max)
 
 }  // namespace
 
-int kv_attention_check() {  // did a call's kernel give up on a wait?
+int kv_attn_tile_prepare() {
+    if (!tile_error_word()) return fail(ELB_ERR_CUDA, "kv_create: no error word");
+    ELB_TRY(ensure_dyn_smem(reinterpret_cast<const void*>(k_kv_attn_tile<1>), TileShape<1>::SMEM));
+    return ensure_dyn_smem(reinterpret_cast<const void*>(k_kv_attn_tile<2>), TileShape<2>::SMEM);
+}
+
+int kv_attention_check() {
     int* e = tile_error_word();
     if (e && *reinterpret_cast<volatile int*>(e)) {
         *e = 0;
@@ -687,7 +696,7 @@ size_t kv_attn_tile_work(const Kv* kv, const elb_kv_batch* b, int n_head, int fe
 
 int kv_attn_tile_launch(const Kv* kv, int layer, KvAttnArgs a, const elb_kv_batch* b, cudaStream_t s) {
     int* err = nullptr;
-    if (!tile_error_word() || cudaHostGetDevicePointer(&err, tile_error_word(), 0) != cudaSuccess) return fail(ELB_ERR_CUDA, "kv_attention: no error word");
+    if (cudaHostGetDevicePointer(&err, tile_error_word(), 0) != cudaSuccess) return fail(ELB_ERR_CUDA, "kv_attention: no error word");
     const TilePlan p = tile_plan(kv, b, a.H, a.few_max);
     const int64_t blocks = p.tiles * kv->HKV;
     if (blocks * p.splits > 0x7fffffff || blocks * KT_ROWS / 8 > 0x7fffffff) return fail(ELB_ERR_UNSUPPORTED, "kv_attention: too many rows");
@@ -695,7 +704,6 @@ int kv_attn_tile_launch(const Kv* kv, int layer, KvAttnArgs a, const elb_kv_batc
     a.splits = p.splits; a.chunk = p.chunk; a.tiles_max = int(p.tiles);
     const int64_t layer_rows = kv->layer_halves() / KV_D;
     auto run = [&](auto kernel, int smem) -> int {
-        ELB_TRY(ensure_dyn_smem(reinterpret_cast<const void*>(kernel), size_t(smem)));
         kernel<<<unsigned(blocks * p.splits), KT_THREADS, smem, s>>>(kv->map, a, int(layer * layer_rows), int(kv->n_layer * layer_rows), err);
         ELB_CUDA(cudaGetLastError());
         return ELB_OK;

@@ -281,7 +281,8 @@ int elb_model_load_gguf_tp(const char* path, int n_ctx, int device, int max_batc
  * captured into a CUDA graph; lengths and tables are read from device memory when the kernels run. All d_* pointers are
  * memory of the handle's device, and the caller's current device stays as it is. Calls that may overlap need work buffers
  * of their own. Errors that only the device can see (a page number outside the pool, lengths longer than a table) touch no
- * memory outside the given buffers: such a page is not written, and reads as zeros. */
+ * memory outside the given buffers: such a page is not written, and reads as zeros. A wait inside a kernel that runs out of time
+ * (all are bounded) makes the next elb_kv_attention_dev call of the process return ELB_ERR_CUDA. */
 
 /* Rotary positions (rope of the reference, src/model.cpp:23-32, with what other checkpoints and longer contexts need). The
  * first `dim` values of a head are rotated in pairs, pair i by the angle pos * f_i in double precision, and multiplied
@@ -350,7 +351,7 @@ int elb_kv_append_dev(elb_kv* kv, int layer, const elb_kv_batch* b, const elb_ro
  * key head h / (n_head / n_head_kv): out = sum_j softmax_j(scale q.k_j) v_j. Every row's queries are used as given (append's
  * q_out). A row at a negative position has no keys: its output is 0. Rows outside every range are left as they are.
  * What lies in a page behind a sequence's length has no influence, infinities and NaN included; nor has a key or value that
- * a row does not attend to. n_head: a multiple of n_head_kv, at most 64 times it. Row strides in floats, rows on 16-byte
+ * a row does not attend to. A row that attends to an infinite or NaN key is NaN or 0. d_out must not overlap d_q. n_head: a multiple of n_head_kv, at most 64 times it. Row strides in floats, rows on 16-byte
  * boundaries. d_work: elb_kv_attention_work bytes, 256-byte aligned; what it holds before and after does not matter. */
 size_t elb_kv_attention_work(const elb_kv* kv, const elb_kv_batch* b, int n_head); /* 0: bad argument */
 int elb_kv_attention_dev(const elb_kv* kv, int layer, const elb_kv_batch* b, const float* d_q, int64_t ldq, int n_head, float scale,
@@ -360,7 +361,8 @@ int elb_kv_attention_dev(const elb_kv* kv, int layer, const elb_kv_batch* b, con
  * d_len[d_parent[r]] positions. d_table_out[r] receives the parent's pages that hold them and -1 behind, d_len_out[r] the
  * length. Full pages are shared. A last page that is not full belongs to the parent's first child (the lowest r); for
  * every other child its content is copied, in every layer, into the page d_spare[r], which takes its place, and d_taken[r]
- * is 1 (0 otherwise). A parent outside [0, n): an empty row, length 0. The spare pages must be in no table. The output
+ * is 1 (0 otherwise; a spare page outside the pool stands in the table all the same). A parent outside [0, n): an empty
+ * row, length 0. The spare pages must be in no table and differ. The output
  * arrays must not overlap the inputs. n <= 4096. */
 int elb_kv_reorder_dev(elb_kv* kv, int n, const int32_t* d_parent, const int32_t* d_len, const int32_t* d_table, int64_t table_ld,
                        const int32_t* d_spare, int32_t* d_len_out, int32_t* d_table_out, int32_t* d_taken, void* stream);
@@ -371,7 +373,8 @@ int elb_kv_reorder_dev(elb_kv* kv, int n, const int32_t* d_parent, const int32_t
  * the score. Equal scores: the lower row first; within a row the larger logit, then the lower token. d_allowed, when not NULL: bit t
  * of row b's words d_allowed[b * allowed_ld + t / 32] says whether t may be picked (allowed_ld 0: one mask for all rows). Not
  * candidates: logits of -infinity or NaN, rows whose score or log-sum-exp is not finite (a beam that does not exist has score
- * -infinity). Where candidates run out, row and token are -1 and the score is -infinity. beams <= 64. d_work:
+ * -infinity). Where candidates run out, row and token are -1 and the score is -infinity. beams <= 64. The outputs must not overlap
+ * d_scores, but d_score may be d_scores when k = beams. d_work:
  * elb_beam_select_work bytes, 256-byte aligned. */
 size_t elb_beam_select_work(int n_vocab, int n_group, int beams, int k); /* 0: bad argument */
 int elb_beam_select_dev(int device, const float* d_logits, int64_t ld, int n_vocab, int n_group, int beams, const double* d_scores,
