@@ -17,7 +17,7 @@ namespace elb {
 
 namespace {
 
-constexpr int RP_THREADS = 256, RP_TOKENS = 4, RP_MAXHALF = 128, RP_BATCH = 4;
+constexpr int RP_THREADS = 256, RP_TOKENS = 4, RP_MAXHALF = 128, RP_BATCH = 4, RP_PAIRS = 256;
 
 struct RopeArgs {
     const double* turns;  // [half] or null: no rotation
@@ -46,18 +46,21 @@ __device__ __forceinline__ float inv_rms(double ms) {
     return float(y * (1.5 - 0.5 * ms * y * y));
 }
 
-__device__ __forceinline__ void split_pair(float x, __half& hi, __half& lo) {
-    hi = __float2half_rn(x);
-    lo = __hisinf(hi) ? __float2half_rn(0.f) : __float2half_rn(x - __half2float(hi));
-}
-
-// four values -> the fp16 planes of a pool row (lo plane: `plane` halves behind)
+// four values -> the fp16 planes of a pool row (lo plane: `plane` halves behind); the remainder of an infinity is 0
 __device__ __forceinline__ void store4(__half* dst, int planes, int64_t plane, const float* v) {
-    __half hi[4], lo[4];
+    uint32_t hi[2], lo[2];
 #pragma unroll
-    for (int i = 0; i < 4; ++i) split_pair(v[i], hi[i], lo[i]);
-    *reinterpret_cast<uint2*>(dst) = *reinterpret_cast<const uint2*>(hi);
-    if (planes == 2) *reinterpret_cast<uint2*>(dst + plane) = *reinterpret_cast<const uint2*>(lo);
+    for (int i = 0; i < 2; ++i) {
+        const __half2 h = __floats2half2_rn(v[2 * i], v[2 * i + 1]);
+        hi[i] = *reinterpret_cast<const uint32_t*>(&h);
+        if (planes == 2) {
+            const float2 f = __half22float2(h);
+            const __half2 l = __floats2half2_rn(isinf(f.x) ? 0.f : v[2 * i] - f.x, isinf(f.y) ? 0.f : v[2 * i + 1] - f.y);
+            lo[i] = *reinterpret_cast<const uint32_t*>(&l);
+        }
+    }
+    *reinterpret_cast<uint2*>(dst) = make_uint2(hi[0], hi[1]);
+    if (planes == 2) *reinterpret_cast<uint2*>(dst + plane) = make_uint2(lo[0], lo[1]);
 }
 
 // What a block knows of one of its tokens
@@ -109,48 +112,68 @@ __device__ __forceinline__ void fill_angles(const RopeArgs& a, int tokens, const
     }
 }
 
+// A (token, head) pair of a block: where it comes from (null: nowhere) and goes to (0: nowhere), its kind (0: queries, 1: keys, 2:
+// values) in the address's lowest two bits and the token's number in the next two (rows start on 16-byte boundaries)
+struct Pair { const float* src; unsigned long long dst; };
+
 // head_dim 32, 64, 128 or 256 (2^upt_log units), dim a multiple of 8, rows on 16-byte boundaries; grid (token groups, head groups).
-// Thread: unit u of every slots-th (token, head) pair of the block, RP_BATCH pairs at a time, whose loads go out together - the first
-// ones before the block knows its tokens.
-template <bool NORM>
+// Thread: unit u of every slots-th pair of the block, RP_BATCH pairs at a time, whose loads go out together - the first ones before
+// the block knows its tokens. Addresses are worked out once per pair, into shared memory (by every thread for itself they were 40
+// % of the instructions: 2048 tokens of 32 + 8 + 8 heads 38 us), and a thread's place in a head is the same for all pairs:
+// values, which are not turned, are read and written in the pairs' order too.
+template <bool NORM, bool HALF>
 __global__ void __launch_bounds__(RP_THREADS, 4) k_rope(const RopeArgs a, int tokens, int heads_per_block, int upt_log) {
-    __shared__ float2 cs[RP_TOKENS][RP_MAXHALF];
+    __shared__ __align__(16) float2 cs[RP_TOKENS][RP_MAXHALF];
+    __shared__ __align__(16) float weights[NORM ? 2 : 1][NORM ? 2 * RP_MAXHALF : 4];  // of queries, keys
+    __shared__ __align__(16) Pair pair[RP_PAIRS];
     __shared__ Tok tok[RP_TOKENS];
     __shared__ int seq[RP_TOKENS];
     const int64_t t0 = int64_t(blockIdx.x) * tokens;
     const int heads = a.n_head + 2 * a.HKV, h0 = blockIdx.y * heads_per_block, nh = min(heads_per_block, heads - h0);
     const int upt = 1 << upt_log, u = threadIdx.x & (upt - 1), slot = threadIdx.x >> upt_log, slots = RP_THREADS >> upt_log;
-    const int pairs = tokens * nh, half = a.dim / 2;
+    const int pairs = tokens * nh;
     const double part = 1.0 / double(1 << (upt_log + 3));  // 1 / head_dim, exact
-    const bool turned = a.turns && 8 * u < a.dim, apart = turned && a.layout == ELB_ROPE_HALF;
-    int th = slot, tt = 0;  // pair of the next load
-    while (th >= nh) { th -= nh; ++tt; }
-    for (int p0 = 0; p0 < pairs; p0 += RP_BATCH * slots) {  // (whole warps stay together for the reductions)
+    const bool turned = a.turns && 8 * u < a.dim;
+    const int e0 = HALF && turned ? 4 * u : 8 * u, e1 = HALF && turned ? a.dim / 2 + 4 * u : 8 * u + 4;
+    for (int p = threadIdx.x; p < pairs; p += RP_THREADS) {
+        const int tt = p / nh, h = h0 + p - tt * nh, hk = h - a.n_head, hv = hk - a.HKV;
+        const int64_t t = t0 + tt;
+        pair[p].src = t >= a.n ? nullptr : hv >= 0 ? a.v + t * a.ldv + hv * KV_D : hk >= 0 ? a.k + t * a.ldk + hk * KV_D
+                                                                                           : a.q + t * a.ldq + int64_t(h) * a.head_dim;
+    }
+    if (NORM)
+        for (int i = threadIdx.x; i < a.head_dim; i += RP_THREADS) {
+            if (a.q_norm) weights[0][i] = a.q_norm[i];
+            if (a.k_norm) weights[NORM][i] = a.k_norm[i];
+        }
+    __syncthreads();
+    for (int p0 = slot; p0 - slot < pairs; p0 += RP_BATCH * slots) {  // (whole warps stay together for the reductions)
         float v[RP_BATCH][8];
-        int ht[RP_BATCH], tk[RP_BATCH];
 #pragma unroll
         for (int b = 0; b < RP_BATCH; ++b) {
-            const int h = h0 + th;
-            ht[b] = tt < tokens ? h : -1;
-            tk[b] = tt;
-            if (tt < tokens && t0 + tt < a.n) {
-                const bool is_v = h >= a.n_head + a.HKV, is_k = h >= a.n_head;
-                const int64_t t = t0 + tt;
-                const float* src = is_v ? a.v + t * a.ldv + (h - a.n_head - a.HKV) * KV_D : is_k ? a.k + t * a.ldk + (h - a.n_head) * KV_D
-                                                                                                  : a.q + t * a.ldq + int64_t(h) * a.head_dim;
-                const bool ap = apart && !is_v;
-                *reinterpret_cast<float4*>(v[b]) = __ldcg(reinterpret_cast<const float4*>(src + (ap ? 4 * u : 8 * u)));
-                *reinterpret_cast<float4*>(v[b] + 4) = __ldcg(reinterpret_cast<const float4*>(src + (ap ? half + 4 * u : 8 * u + 4)));
+            const int p = p0 + b * slots;
+            const float* src = p < pairs ? pair[p].src : nullptr;
+            if (src) {
+                *reinterpret_cast<float4*>(v[b]) = __ldcg(reinterpret_cast<const float4*>(src + e0));
+                *reinterpret_cast<float4*>(v[b] + 4) = __ldcg(reinterpret_cast<const float4*>(src + e1));
             } else {
 #pragma unroll
                 for (int i = 0; i < 8; ++i) v[b][i] = 0.f;
             }
-            th += slots;
-            while (th >= nh) { th -= nh; ++tt; }
         }
-        if (p0 == 0) {
+        if (p0 == slot) {
             find_tokens(a, t0, tokens, tok, seq);
             if (a.turns) fill_angles(a, tokens, tok, cs);
+            for (int p = threadIdx.x; p < pairs; p += RP_THREADS) {
+                const int tt = p / nh, h = h0 + p - tt * nh, hk = h - a.n_head, is_v = hk >= a.HKV;
+                unsigned long long to = 0;
+                if (hk < 0) {
+                    if (tok[tt].on) to = reinterpret_cast<unsigned long long>(a.q_out + (t0 + tt) * a.ldqo + int64_t(h) * a.head_dim);
+                } else if (tok[tt].on && tok[tt].row >= 0) {
+                    to = reinterpret_cast<unsigned long long>(a.pool + tok[tt].row + int64_t(hk) * a.planes * a.rows.page * KV_D) | (1 + is_v);
+                }
+                pair[p].dst = to ? to | unsigned(tt << 2) : 0ull;
+            }
             __syncthreads();
         }
         // Mean squares of the batch's four heads at once: the first two steps of the reduction across a head's lanes halve what a
@@ -174,40 +197,37 @@ __global__ void __launch_bounds__(RP_THREADS, 4) k_rope(const RopeArgs a, int to
         }
 #pragma unroll
         for (int b = 0; b < RP_BATCH; ++b) {
-            const int h = ht[b], t = min(tk[b], tokens - 1);
-            const bool is_v = h >= a.n_head + a.HKV, is_k = !is_v && h >= a.n_head, turn = turned && !is_v, ap = apart && !is_v;
-            const int e0 = ap ? 4 * u : 8 * u, e1 = ap ? half + 4 * u : 8 * u + 4;
-            if (NORM) {
-                const float mine = __shfl_sync(0xffffffffu, inv, (int(threadIdx.x) & 31 & ~3) | (b >> 1) | (b & 1) << 1);
-                const float* w = is_v ? nullptr : is_k ? a.k_norm : a.q_norm;
-                if (w && h >= 0) {
-                    const float4 w0 = *reinterpret_cast<const float4*>(w + e0), w1 = *reinterpret_cast<const float4*>(w + e1);
-                    const float ww[8] = {w0.x, w0.y, w0.z, w0.w, w1.x, w1.y, w1.z, w1.w};
+            const int p = p0 + b * slots;
+            const float mine = NORM ? __shfl_sync(0xffffffffu, inv, (int(threadIdx.x) & 31 & ~3) | (b >> 1) | (b & 1) << 1) : 1.f;
+            const unsigned long long to = p < pairs ? pair[p].dst : 0ull;
+            if (!to) continue;
+            const unsigned kind = unsigned(to) & 3u, t = unsigned(to) >> 2 & 3u;
+            if (NORM && kind < 2 && (kind ? a.k_norm : a.q_norm)) {
+                const float4 w0 = *reinterpret_cast<const float4*>(weights[kind] + e0), w1 = *reinterpret_cast<const float4*>(weights[kind] + e1);
+                const float ww[8] = {w0.x, w0.y, w0.z, w0.w, w1.x, w1.y, w1.z, w1.w};
 #pragma unroll
-                    for (int i = 0; i < 8; ++i) v[b][i] = __fmul_rn(__fmul_rn(v[b][i], mine), ww[i]);
-                }
+                for (int i = 0; i < 8; ++i) v[b][i] = __fmul_rn(__fmul_rn(v[b][i], mine), ww[i]);
             }
-            if (turn) {
+            if (turned && kind < 2) {
+                const float4 c0 = *reinterpret_cast<const float4*>(cs[t] + 4 * u), c1 = *reinterpret_cast<const float4*>(cs[t] + 4 * u + 2);
+                const float c[4] = {c0.x, c0.z, c1.x, c1.z}, sn[4] = {c0.y, c0.w, c1.y, c1.w};
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
-                    const float2 c = cs[t][4 * u + i];
-                    const float x0 = ap ? v[b][i] : v[b][2 * i], y0 = ap ? v[b][i + 4] : v[b][2 * i + 1];
-                    const float x = x0 * c.x - y0 * c.y, y = x0 * c.y + y0 * c.x;
-                    if (ap) { v[b][i] = x; v[b][i + 4] = y; }
-                    else { v[b][2 * i] = x; v[b][2 * i + 1] = y; }
+                    float &x = v[b][HALF ? i : 2 * i], &y = v[b][HALF ? i + 4 : 2 * i + 1];
+                    const float x0 = x, y0 = y;
+                    x = x0 * c[i] - y0 * sn[i];
+                    y = x0 * sn[i] + y0 * c[i];
                 }
             }
-            if (h < 0 || !tok[t].on) continue;
-            if (is_k || is_v) {
-                if (tok[t].row < 0) continue;
-                const int64_t plane = int64_t(a.rows.page) * KV_D;
-                __half* dst = a.pool + tok[t].row + (int64_t(is_v) * a.HKV + h - a.n_head - (is_v ? a.HKV : 0)) * a.planes * plane;
-                store4(dst + e0, a.planes, plane, v[b]);
-                store4(dst + e1, a.planes, plane, v[b] + 4);
-            } else {
-                float* dst = a.q_out + (t0 + t) * a.ldqo + int64_t(h) * a.head_dim;
+            const unsigned long long at = to & ~15ull;
+            if (kind == 0) {
+                float* dst = reinterpret_cast<float*>(at);
                 *reinterpret_cast<float4*>(dst + e0) = *reinterpret_cast<const float4*>(v[b]);
                 *reinterpret_cast<float4*>(dst + e1) = *reinterpret_cast<const float4*>(v[b] + 4);
+            } else {
+                __half* dst = reinterpret_cast<__half*>(at);
+                store4(dst + e0, a.planes, int64_t(a.rows.page) * KV_D, v[b]);
+                store4(dst + e1, a.planes, int64_t(a.rows.page) * KV_D, v[b] + 4);
             }
         }
     }
@@ -251,13 +271,14 @@ int rope_run(RopeArgs& a, cudaStream_t s) {
     // Heads are cut over blocks while the grid is small
     const int heads = a.n_head + 2 * a.HKV, tokens = a.n >= 1024 ? 4 : a.n >= 512 ? 2 : 1;
     const int64_t groups = (a.n + tokens - 1) / tokens;
-    int per = heads;
+    int cuts = (heads * tokens + RP_PAIRS - 1) / RP_PAIRS, per = (heads + cuts - 1) / cuts;
     while (per > 16 && groups * ((heads + per - 1) / per) < 296) per = (per + 1) / 2;
     int upt_log = 2;
     while ((8 << upt_log) < a.head_dim) ++upt_log;
     const dim3 grid{unsigned(groups), unsigned((heads + per - 1) / per)};
-    if (a.q_norm || a.k_norm) k_rope<true><<<grid, RP_THREADS, 0, s>>>(a, tokens, per, upt_log);
-    else k_rope<false><<<grid, RP_THREADS, 0, s>>>(a, tokens, per, upt_log);
+    const bool norm = a.q_norm || a.k_norm, half = a.layout == ELB_ROPE_HALF;
+    const auto kernel = norm ? (half ? k_rope<true, true> : k_rope<true, false>) : (half ? k_rope<false, true> : k_rope<false, false>);
+    kernel<<<grid, RP_THREADS, 0, s>>>(a, tokens, per, upt_log);
     ELB_CUDA(cudaGetLastError());
     return ELB_OK;
 }
