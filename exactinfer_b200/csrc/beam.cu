@@ -12,6 +12,7 @@
 // ln 2 / 128 and the Taylor sum of e^r to r^4 / 24 (4e-14 off at most), nine double operations a logit.
 #include <algorithm>
 #include <cmath>
+#include <cstring>
 
 #include "kv.cuh"
 
@@ -44,7 +45,9 @@ __device__ __forceinline__ unsigned long long warp_best(unsigned long long v) {
     return (static_cast<unsigned long long>(hi) << 32) | lo;
 }
 
-// sum + e^y for -701 <= y <= 0; tab[i] = 2^(i/64). NaN stays NaN
+// 2^(i/64), i << 14 less in the upper word: adding n << 14 to that of entry n & 63 multiplies by the whole powers of two in n / 64
+struct BeamTab { unsigned long long e[64]; };
+// sum + e^y for -701 <= y <= 0. NaN stays NaN
 __device__ __forceinline__ double add_exp(double sum, double y, const double* tab) {
     const double t = fma(y, 92.332482616893656769, 6755399441055744.0);  // 64 / ln 2; 1.5 * 2^52: the low word is the rounded integer
     const double r = fma(t - 6755399441055744.0, -0.010830424696249145, y);  // ln 2 / 64
@@ -54,7 +57,12 @@ __device__ __forceinline__ double add_exp(double sum, double y, const double* ta
     p = fma(p, r, 1.0);
     p = fma(p, r, 1.0);
     const double s = tab[n & 63];
-    return fma(__hiloint2double(__double2hiint(s) + ((n & ~63) << 14), __double2loint(s)), p, sum);
+    return fma(__hiloint2double(__double2hiint(s) + n * 16384, __double2loint(s)), p, sum);
+}
+__device__ __forceinline__ float max3(float a, float b, float c) {
+    float r;
+    asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+    return r;
 }
 __device__ __forceinline__ float max_nan(float a, float b) {
     float r;
@@ -72,7 +80,8 @@ __device__ __forceinline__ unsigned long long beam_order(double x) {
 template <bool VEC>
 __global__ void __launch_bounds__(BS_THREADS, 5) k_beam_segments(const float* __restrict__ logits, int64_t ld, int n, int segs, int steps, int beams,
                                                                  const uint32_t* __restrict__ allowed, int64_t allowed_ld,
-                                                                 BeamSeg* __restrict__ parts, unsigned* __restrict__ arrived) {
+                                                                 BeamSeg* __restrict__ parts, unsigned* __restrict__ arrived,
+                                                                 const __grid_constant__ BeamTab powers) {
     __shared__ double tab[64];
     pdl_launch_dependents();
     const int tid = threadIdx.x, lane = tid & 31, seg = int(blockIdx.x) * BS_WARPS + (tid >> 5);
@@ -105,17 +114,17 @@ __global__ void __launch_bounds__(BS_THREADS, 5) k_beam_segments(const float* __
             }
         }
         if (st == 0) {
-            if (tid < 64) tab[tid] = exp2(tid / 64.0);
+            if (tid < 64) tab[tid] = __longlong_as_double(static_cast<long long>(powers.e[tid]));
             __syncthreads();
         }
-        float here = v[0];  // (NaN is passed over here and spoils the sum below)
+        float here = -INFINITY;  // (NaN is passed over here and spoils the sum below)
 #pragma unroll
-        for (int j = 1; j < BS_PER; ++j) here = fmaxf(here, v[j]);
+        for (int j = 0; j < BS_PER; j += 2) here = max3(here, v[j], v[j + 1]);
         float best = here;
         if (mask) {
             best = -INFINITY;
 #pragma unroll
-            for (int j = 0; j < BS_PER; ++j) best = (off >> j) & 1u ? best : fmaxf(best, v[j]);
+            for (int j = 0; j < BS_PER; j += 2) best = max3(best, (off >> j) & 1u ? -INFINITY : v[j], (off >> j) & 2u ? -INFINITY : v[j + 1]);
         }
         top = max(top, __reduce_max_sync(0xffffffffu, beam_key(best)));
         const unsigned most = __reduce_max_sync(0xffffffffu, beam_key(here));
@@ -378,8 +387,14 @@ int beam_select_launch(int device, const float* logits, int64_t ld, int n_vocab,
     auto* arrived = reinterpret_cast<unsigned*>(at);
     const bool vec = reinterpret_cast<uintptr_t>(logits) % 16 == 0 && ld % 4 == 0;
     const dim3 grid{unsigned((cut.segs + BS_WARPS - 1) / BS_WARPS), unsigned(rows)};
-    if (vec) k_beam_segments<true><<<grid, BS_THREADS, 0, s>>>(logits, ld, n_vocab, cut.segs, cut.steps, beams, allowed, allowed_ld, parts, arrived);
-    else k_beam_segments<false><<<grid, BS_THREADS, 0, s>>>(logits, ld, n_vocab, cut.segs, cut.steps, beams, allowed, allowed_ld, parts, arrived);
+    BeamTab powers;
+    for (int i = 0; i < 64; ++i) {
+        const double e = std::exp2(i / 64.0);
+        std::memcpy(powers.e + i, &e, sizeof e);
+        powers.e[i] -= static_cast<unsigned long long>(i << 14) << 32;
+    }
+    if (vec) k_beam_segments<true><<<grid, BS_THREADS, 0, s>>>(logits, ld, n_vocab, cut.segs, cut.steps, beams, allowed, allowed_ld, parts, arrived, powers);
+    else k_beam_segments<false><<<grid, BS_THREADS, 0, s>>>(logits, ld, n_vocab, cut.segs, cut.steps, beams, allowed, allowed_ld, parts, arrived, powers);
     ELB_CUDA(cudaGetLastError());
     ELB_TRY(launch_after(k_beam_pick, dim3(unsigned(rows)), dim3(BP_THREADS), 0, s, true, logits, ld, n_vocab, cut.segs, cut.steps, beams, k, vec, allowed,
                          allowed_ld, parts, scores, best, arrived, parent, token, score));
