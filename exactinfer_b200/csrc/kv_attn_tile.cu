@@ -658,13 +658,20 @@ TilePlan tile_plan(const Kv* kv, const elb_kv_batch* b, int n_head, int few_max)
     const int64_t rows = int64_t(b->n_tok) * (n_head / kv->HKV);
     // tiles of 128 rows: whatever the sequences' lengths are, each adds at most one that is not full
     p.tiles = b->n_seq == 1 ? (rows + KT_ROWS - 1) / KT_ROWS : rows / KT_ROWS + std::min<int64_t>(b->n_seq, rows / (few_max + 1));
-    const int64_t base = kv->HKV * std::max<int64_t>(p.tiles, 1);
+    // The cut of the keys. A CTA's start and end cost as much as 5 to 8 tiles of keys, so its range should be long, at least 4 tiles;
+    // but a second wave of CTAs costs as much as the first. When the sequences have about as many rows each, their tiles are
+    // known and the ranges are made for one wave; when not (lengths will differ as well, and short ones leave early), half of the
+    // sequences' last tiles are counted and the ranges are made for one and a half. Cut in 1, 2, 3, 4, 6 ranges, us, F16: 9 sequences
+    // of 64 tokens at 4096 keys, 16 heads on 8 (72 CTAs) 76, 56, 76, 70, 83; 2 of 64 at 8000, 32 on 8 (32) 154, 93, 69, 59, 80; 3 of
+    // 300 at 2000 (240) 93, 126, 133, 148, 169; 9 of 3-77 at 203-4100, 16 on 8 65, 53, 49, 52, 59; 4 of 20-300 at 300-3000 66, 85,
+    // 91, 85, 105. (All key tiles dealt out evenly over one CTA per SM, which walks from tile to tile, with a launch before
+    // and a join behind: 73, -, 123, -, -.)
+    const int64_t most_q = std::max(1, std::min(b->max_q, b->n_tok));
+    const bool alike = 4 * int64_t(b->n_tok) >= 3 * b->n_seq * most_q;
+    const int64_t likely = std::min(b->n_seq * ((most_q * (n_head / kv->HKV) + KT_ROWS - 1) / KT_ROWS), rows / KT_ROWS + (b->n_seq + 1) / 2);
+    const int64_t base = kv->HKV * std::max<int64_t>(1, b->n_seq == 1 ? p.tiles : std::min(p.tiles, likely));
     const int len = kv_most(kv, b);
-    // A CTA's start and end cost as much as 5 tiles of keys: one wave of long ranges when all sequences are alike, two when they may
-    // not be, and at least 4 tiles each. Cut for two, three or four waves (us): 9 turns of 3-77 tokens behind 203-4100 keys, pairs, 95, 80,
-    // 88; 9 of 64 tokens at 4096 keys 57, 77, 69; 3 of 300 tokens at 2000 keys 95, 95, 129. (All key tiles of a batch dealt
-    // out evenly over one CTA per SM, which walks from tile to tile: a launch before and a join behind it, 93, 73, 123 us.)
-    int64_t want = base >= 2 * kv->sm_count ? 1 : std::max<int64_t>(1, int64_t(kv->sm_count) * (b->n_seq > 1 ? 2 : 1) / base);
+    int64_t want = std::max<int64_t>(1, alike ? kv->sm_count / base : (3 * kv->sm_count + base) / (2 * base));
     want = std::min<int64_t>(want, (len + 4 * KT_KEYS - 1) / (4 * KT_KEYS));
     p.chunk = int((len + want - 1) / want + KT_KEYS - 1) / KT_KEYS * KT_KEYS;
     p.splits = (len + p.chunk - 1) / p.chunk;
