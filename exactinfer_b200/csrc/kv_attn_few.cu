@@ -358,8 +358,10 @@ FewPlan few_plan(const Kv* kv, const elb_kv_batch* b, int n_head, int few_max) {
     const int resident = kv->sm_count * (kv->planes == 1 ? 2 : 1);
     const int64_t base = int64_t(b->n_seq) * kv->HKV * p.tiles;
     const int len = kv_most(kv, b);
-    // one sequence: one wave of equal ranges. Several: lengths differ, ranges short enough that the last ones even out
-    int64_t want = b->n_seq == 1 ? std::max<int64_t>(1, resident / base) : std::max<int64_t>(1, (int64_t(resident) * 12 + base - 1) / base);
+    // One sequence: one wave of equal ranges. Several: lengths differ, ranges short enough for four waves, so that the last ones even
+    // out. For 12, 8, 4, 2 waves, us, F16: 64 single tokens at 100-8000 keys 198, 199, 201, 206; 64 at 100-4000 98, 96, 93, 95; 16 at
+    // 100-20000 52, 47, 44, 45; 256 at 700 131, 131, 116, 116; 64 of 4 tokens 128, 118, 114, 112.
+    int64_t want = b->n_seq == 1 ? std::max<int64_t>(1, resident / base) : std::max<int64_t>(1, (int64_t(resident) * 4 + base - 1) / base);
     want = std::min<int64_t>(want, (len + 255) / 256);
     p.chunk = int((len + want - 1) / want + 63) / 64 * 64;
     p.splits = (len + p.chunk - 1) / p.chunk;
