@@ -9,7 +9,9 @@
 // Places are found by counting the larger ones.
 //
 // Exponentials are the work beside the loads: double precision, e^y = 2^(i/64) 2^n e^r with y = (64 n + i) ln 2 / 64 + r, |r| <=
-// ln 2 / 128 and the Taylor sum of e^r to r^4 / 24 (4e-14 off at most), nine double operations a logit.
+// ln 2 / 128 and the Taylor sum of e^r to r^4 / 24 (4e-14 off at most), nine double operations a logit. 64 rows of 151936 logits
+// in 16 groups under masks: 26.5 us, 17 of them k_beam_segments (65 % of the issue slots; bytes alone 6); one group of 4 rows 12 us,
+// the length of the two kernels' chains.
 #include <algorithm>
 #include <cmath>
 #include <cstring>

@@ -4,8 +4,11 @@
 //
 // Bound by memory: every value is read and written once. A block takes a few tokens, computes the cosines and sines that
 // all their heads share once, in double, into shared memory, and streams the heads through registers: a thread takes 8
-// values (a "unit": 4 pairs, or 8 values that are kept), 16-byte loads. Angles are formed in turns, t = pos * (f / 2 pi) and
+// values (a "unit": 4 pairs, or 8 values that are kept) as two 16-byte quads. Angles are formed in turns, t = pos * (f / 2 pi) and
 // the fraction of t, so that no position needs more than one double-precision product and a sine of at most one turn.
+// 4096 rows of 32 heads of 128, interleaved: 23.5 us, 5.7 TB/s (26.7 with a thread's eight values side by side: every load and
+// store touched half of its sectors). Append of 2048 tokens, 32 + 8 + 8 heads, pairs: 37.5 us, 4.3 TB/s: one wave of blocks, whose first
+// loads wait beside the search for their tokens and the angles.
 #include <algorithm>
 #include <cmath>
 #include <new>
@@ -101,14 +104,15 @@ __device__ __forceinline__ void find_tokens(const RopeArgs& a, int64_t t0, int t
     __syncthreads();
 }
 
-__device__ __forceinline__ void fill_angles(const RopeArgs& a, int tokens, const Tok* tok, float2 (*cs)[RP_MAXHALF]) {
+// PERM: pairs 4 u, 4 u + 1 of all u first, then 4 u + 2, 4 u + 3: lanes that each read four pairs in two 16-byte loads meet no conflicts
+template <bool PERM> __device__ __forceinline__ void fill_angles(const RopeArgs& a, int tokens, const Tok* tok, float2 (*cs)[RP_MAXHALF]) {
     const int half = a.dim / 2;
     for (int i = threadIdx.x; i < tokens * half; i += RP_THREADS) {
         const int t = i / half, f = i - t * half;
         const double turn = double(tok[t].pos) * a.turns[f];
         double sn, c;
         sincospi(2.0 * (turn - rint(turn)), &sn, &c);
-        cs[t][f] = make_float2(float(c * a.mscale), float(sn * a.mscale));
+        cs[t][PERM ? (f >> 2) * 2 + (f & 2) * (RP_MAXHALF / 4) + (f & 1) : f] = make_float2(float(c * a.mscale), float(sn * a.mscale));
     }
 }
 
@@ -116,11 +120,17 @@ __device__ __forceinline__ void fill_angles(const RopeArgs& a, int tokens, const
 // values) in the address's lowest two bits and the token's number in the next two (rows start on 16-byte boundaries)
 struct Pair { const float* src; unsigned long long dst; };
 
+__device__ __forceinline__ void turn(float& x, float& y, float c, float s) {
+    const float x0 = x, y0 = y;
+    x = x0 * c - y0 * s;
+    y = x0 * s + y0 * c;
+}
+
 // head_dim 32, 64, 128 or 256 (2^upt_log units), dim a multiple of 8, rows on 16-byte boundaries; grid (token groups, head groups).
 // Thread: unit u of every slots-th pair of the block, RP_BATCH pairs at a time, whose loads go out together - the first ones before
 // the block knows its tokens. Addresses are worked out once per pair, into shared memory (by every thread for itself they were 40
-// % of the instructions: 2048 tokens of 32 + 8 + 8 heads 38 us), and a thread's place in a head is the same for all pairs:
-// values, which are not turned, are read and written in the pairs' order too.
+// % of the instructions), and a thread's place in a head is the same for all pairs: values, which are not turned, are read and
+// written in the pairs' order too.
 template <bool NORM, bool HALF>
 __global__ void __launch_bounds__(RP_THREADS, 4) k_rope(const RopeArgs a, int tokens, int heads_per_block, int upt_log) {
     __shared__ __align__(16) float2 cs[RP_TOKENS][RP_MAXHALF];
@@ -133,8 +143,10 @@ __global__ void __launch_bounds__(RP_THREADS, 4) k_rope(const RopeArgs a, int to
     const int upt = 1 << upt_log, u = threadIdx.x & (upt - 1), slot = threadIdx.x >> upt_log, slots = RP_THREADS >> upt_log;
     const int pairs = tokens * nh;
     const double part = 1.0 / double(1 << (upt_log + 3));  // 1 / head_dim, exact
-    const bool turned = a.turns && 8 * u < a.dim;
-    const int e0 = HALF && turned ? 4 * u : 8 * u, e1 = HALF && turned ? a.dim / 2 + 4 * u : 8 * u + 4;
+    // a thread's two quads of a head: pairs' halves, or two pairs each
+    const bool both = a.turns && 8 * u < a.dim;
+    const int e0 = HALF ? (both ? 4 * u : 8 * u) : 4 * u, e1 = HALF ? (both ? a.dim / 2 + 4 * u : 8 * u + 4) : 4 * u + a.head_dim / 2;
+    const bool turn0 = HALF ? both : a.turns && e0 < a.dim, turn1 = HALF ? both : a.turns && e1 < a.dim;
     for (int p = threadIdx.x; p < pairs; p += RP_THREADS) {
         const int tt = p / nh, h = h0 + p - tt * nh, hk = h - a.n_head, hv = hk - a.HKV;
         const int64_t t = t0 + tt;
@@ -163,7 +175,7 @@ __global__ void __launch_bounds__(RP_THREADS, 4) k_rope(const RopeArgs a, int to
         }
         if (p0 == slot) {
             find_tokens(a, t0, tokens, tok, seq);
-            if (a.turns) fill_angles(a, tokens, tok, cs);
+            if (a.turns) fill_angles<HALF>(a, tokens, tok, cs);
             for (int p = threadIdx.x; p < pairs; p += RP_THREADS) {
                 const int tt = p / nh, h = h0 + p - tt * nh, hk = h - a.n_head, is_v = hk >= a.HKV;
                 unsigned long long to = 0;
@@ -208,15 +220,23 @@ __global__ void __launch_bounds__(RP_THREADS, 4) k_rope(const RopeArgs a, int to
 #pragma unroll
                 for (int i = 0; i < 8; ++i) v[b][i] = __fmul_rn(__fmul_rn(v[b][i], mine), ww[i]);
             }
-            if (turned && kind < 2) {
-                const float4 c0 = *reinterpret_cast<const float4*>(cs[t] + 4 * u), c1 = *reinterpret_cast<const float4*>(cs[t] + 4 * u + 2);
-                const float c[4] = {c0.x, c0.z, c1.x, c1.z}, sn[4] = {c0.y, c0.w, c1.y, c1.w};
-#pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    float &x = v[b][HALF ? i : 2 * i], &y = v[b][HALF ? i + 4 : 2 * i + 1];
-                    const float x0 = x, y0 = y;
-                    x = x0 * c[i] - y0 * sn[i];
-                    y = x0 * sn[i] + y0 * c[i];
+            if (turn0 && kind < 2) {
+                const float4* c = reinterpret_cast<const float4*>(cs[t]) + u;
+                if (HALF) {
+                    const float4 c0 = c[0], c1 = c[RP_MAXHALF / 4];
+                    turn(v[b][0], v[b][4], c0.x, c0.y);
+                    turn(v[b][1], v[b][5], c0.z, c0.w);
+                    turn(v[b][2], v[b][6], c1.x, c1.y);
+                    turn(v[b][3], v[b][7], c1.z, c1.w);
+                } else {
+                    const float4 c0 = c[0];
+                    turn(v[b][0], v[b][1], c0.x, c0.y);
+                    turn(v[b][2], v[b][3], c0.z, c0.w);
+                    if (turn1) {
+                        const float4 c1 = c[upt];
+                        turn(v[b][4], v[b][5], c1.x, c1.y);
+                        turn(v[b][6], v[b][7], c1.z, c1.w);
+                    }
                 }
             }
             const unsigned long long at = to & ~15ull;
@@ -240,7 +260,7 @@ __global__ void __launch_bounds__(RP_THREADS) k_rope_any(const RopeArgs a) {
     __shared__ int seq[RP_TOKENS];
     const int64_t t0 = blockIdx.x;
     find_tokens(a, t0, 1, tok, seq);
-    fill_angles(a, 1, tok, cs);
+    fill_angles<false>(a, 1, tok, cs);
     __syncthreads();
     const int lane = threadIdx.x & 31, half = a.dim / 2;
     for (int h = int(threadIdx.x) / 32 + 8 * int(blockIdx.y); h < a.n_head; h += 8 * int(gridDim.y)) {
