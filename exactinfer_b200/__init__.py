@@ -149,9 +149,12 @@ def split_limbs(x: np.ndarray, nl: int, device: int = 0):
 
 def _ptr(x):
     """Device address of x: a number, a DeviceBuffer, anything with data_ptr() (a torch tensor, say) or None."""
-    if x is None or isinstance(x, int):
+    if x is None or type(x) is int:
         return x
-    return x.ptr if isinstance(x, DeviceBuffer) else x.data_ptr()
+    try:  # (a decoding step makes a few of these calls per layer: every microsecond of them counts)
+        return x.data_ptr()
+    except AttributeError:
+        return x.ptr if isinstance(x, DeviceBuffer) else int(x)
 
 
 ROPE_HALF, ROPE_INTERLEAVED = 0, 1
@@ -180,13 +183,14 @@ class Rope:
         self.config = rope_config(head_dim, **config)
         self.head_dim, h = head_dim, C.c_void_p()
         check(lib().elb_rope_create(device, C.byref(self.config), C.byref(h)))
-        self._h, self._destroy = h, lib().elb_rope_destroy
+        self._h, self._destroy, self._apply = h, lib().elb_rope_destroy, lib().elb_rope_dev
 
     def apply(self, x, pos, y, n: int, heads: int, ldx: int | None = None, ldy: int | None = None, norm=None, eps: float = 0.0, stream: int = 0):
         """y[n][heads] = x rotated at the positions pos[n] (elb_rope_dev); strides in floats, default the row's width."""
         w = heads * self.head_dim
-        check(lib().elb_rope_dev(self._h, _ptr(x), w if ldx is None else ldx, _ptr(y), w if ldy is None else ldy, n, heads, _ptr(pos), _ptr(norm), eps,
-                                 stream))
+        rc = self._apply(self._h, _ptr(x), w if ldx is None else ldx, _ptr(y), w if ldy is None else ldy, n, heads, _ptr(pos), _ptr(norm), eps, stream)
+        if rc:
+            check(rc)
 
     def close(self):
         if getattr(self, "_h", None):
@@ -215,6 +219,7 @@ class KvCache:
         self._mem, self.head_dim, self.n_head_kv = mem, head_dim, n_head_kv
         check(lib().elb_kv_create(device, n_layer, n_head_kv, head_dim, page, n_pages, type, _ptr(mem), C.byref(h)))
         self._h, self._destroy = h, lib().elb_kv_destroy
+        self._append, self._attention = lib().elb_kv_append_dev, lib().elb_kv_attention_dev
 
     @staticmethod
     def bytes(n_layer: int, n_head_kv: int, page: int, n_pages: int, type: int = KV_F16, head_dim: int = 128) -> int:
@@ -228,8 +233,10 @@ class KvCache:
     def append(self, layer: int, batch: KvBatch, k, v, ldk: int, ldv: int, rope: Rope | None = None, k_norm=None, eps: float = 0.0, q=None,
                ldq: int = 0, n_head: int = 0, q_norm=None, q_out=None, ldqo: int = 0, stream: int = 0):
         """Keys and values of the batch's rows into their pages, its queries rotated into q_out (elb_kv_append_dev)."""
-        check(lib().elb_kv_append_dev(self._h, layer, batch._as_parameter_, rope._h if rope else None, _ptr(k), ldk, _ptr(v), ldv, _ptr(k_norm), eps,
-                                      _ptr(q), ldq, n_head, _ptr(q_norm), _ptr(q_out), ldqo, stream))
+        rc = self._append(self._h, layer, batch._as_parameter_, rope._h if rope else None, _ptr(k), ldk, _ptr(v), ldv, _ptr(k_norm), eps, _ptr(q), ldq,
+                          n_head, _ptr(q_norm), _ptr(q_out), ldqo, stream)
+        if rc:
+            check(rc)
 
     def attention_work(self, batch: KvBatch, n_head: int) -> int:
         """Bytes of working memory that attention() needs for a batch."""
@@ -239,8 +246,10 @@ class KvCache:
                   ldo: int | None = None, stream: int = 0):
         """Attention of the batch's rows over their sequences' pages (elb_kv_attention_dev)."""
         w = n_head * self.head_dim
-        check(lib().elb_kv_attention_dev(self._h, layer, batch._as_parameter_, _ptr(q), w if ldq is None else ldq, n_head, scale, _ptr(out),
-                                         w if ldo is None else ldo, _ptr(work), work_bytes, stream))
+        rc = self._attention(self._h, layer, batch._as_parameter_, _ptr(q), w if ldq is None else ldq, n_head, scale, _ptr(out), w if ldo is None else ldo,
+                             _ptr(work), work_bytes, stream)
+        if rc:
+            check(rc)
 
     def reorder(self, n: int, parent, length, table, table_ld: int, spare, length_out, table_out, taken, stream: int = 0):
         """Row r goes on from row parent[r]: tables and lengths, last pages copied where they are shared (elb_kv_reorder_dev)."""
@@ -263,8 +272,10 @@ def beam_select_work(n_vocab: int, n_group: int, beams: int, k: int) -> int:
 def beam_select(logits, n_vocab: int, n_group: int, beams: int, scores, k: int, parent, token, score, work, work_bytes: int, ld: int | None = None,
                 allowed=None, allowed_ld: int = 0, device: int = 0, stream: int = 0):
     """The k best continuations of every group of beams (elb_beam_select_dev): parent[n_group][k], token, score (double)."""
-    check(lib().elb_beam_select_dev(device, _ptr(logits), n_vocab if ld is None else ld, n_vocab, n_group, beams, _ptr(scores), _ptr(allowed),
-                                    allowed_ld, k, _ptr(parent), _ptr(token), _ptr(score), _ptr(work), work_bytes, stream))
+    rc = lib().elb_beam_select_dev(device, _ptr(logits), n_vocab if ld is None else ld, n_vocab, n_group, beams, _ptr(scores), _ptr(allowed),
+                                   allowed_ld, k, _ptr(parent), _ptr(token), _ptr(score), _ptr(work), work_bytes, stream)
+    if rc:
+        check(rc)
 
 
 def spec_config(spec: "synth.Spec", max_batch: int = 0, n_seq: int = 0) -> Config:

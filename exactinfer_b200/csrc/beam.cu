@@ -389,12 +389,15 @@ int beam_select_launch(int device, const float* logits, int64_t ld, int n_vocab,
     auto* arrived = reinterpret_cast<unsigned*>(at);
     const bool vec = reinterpret_cast<uintptr_t>(logits) % 16 == 0 && ld % 4 == 0;
     const dim3 grid{unsigned((cut.segs + BS_WARPS - 1) / BS_WARPS), unsigned(rows)};
-    BeamTab powers;
-    for (int i = 0; i < 64; ++i) {
-        const double e = std::exp2(i / 64.0);
-        std::memcpy(powers.e + i, &e, sizeof e);
-        powers.e[i] -= static_cast<unsigned long long>(i << 14) << 32;
-    }
+    static const BeamTab powers = [] {
+        BeamTab t;
+        for (int i = 0; i < 64; ++i) {
+            const double e = std::exp2(i / 64.0);
+            std::memcpy(t.e + i, &e, sizeof e);
+            t.e[i] -= static_cast<unsigned long long>(i << 14) << 32;
+        }
+        return t;
+    }();
     if (vec) k_beam_segments<true><<<grid, BS_THREADS, 0, s>>>(logits, ld, n_vocab, cut.segs, cut.steps, beams, allowed, allowed_ld, parts, arrived, powers);
     else k_beam_segments<false><<<grid, BS_THREADS, 0, s>>>(logits, ld, n_vocab, cut.segs, cut.steps, beams, allowed, allowed_ld, parts, arrived, powers);
     ELB_CUDA(cudaGetLastError());

@@ -174,14 +174,13 @@ void kv_destroy(Kv* kv) {
 }
 
 int kv_check_batch(const Kv* kv, int layer, const elb_kv_batch* b, const char* what) {
-    const std::string w = std::string(what) + ": ";
-    if (!kv || !b) return fail(ELB_ERR_INVALID, w + "null argument");
-    if (layer < 0 || layer >= kv->n_layer) return fail(ELB_ERR_RANGE, w + "layer out of range");
-    if (b->n_seq < 0 || b->n_tok < 0 || b->max_q < 0 || b->max_len < 0) return fail(ELB_ERR_INVALID, w + "negative count");
-    if (b->n_seq > 65536) return fail(ELB_ERR_UNSUPPORTED, w + "more than 65536 sequences");
-    if (b->n_seq > 0 && b->n_tok > 0 && (!b->d_q_start || !b->d_len || !b->d_table)) return fail(ELB_ERR_INVALID, w + "null argument");
-    if (b->table_ld < 0 || (b->n_seq > 0 && b->table_ld == 0)) return fail(ELB_ERR_INVALID, w + "a page table needs a positive row stride");
-    if (b->table_ld > (int64_t(1) << 30) / kv->page) return fail(ELB_ERR_UNSUPPORTED, w + "tables for more than 2^30 positions");  // (a pool has fewer)
+    if (!kv || !b) return fail(ELB_ERR_INVALID, std::string(what) + ": null argument");
+    if (layer < 0 || layer >= kv->n_layer) return fail(ELB_ERR_RANGE, std::string(what) + ": layer out of range");
+    if (b->n_seq < 0 || b->n_tok < 0 || b->max_q < 0 || b->max_len < 0) return fail(ELB_ERR_INVALID, std::string(what) + ": negative count");
+    if (b->n_seq > 65536) return fail(ELB_ERR_UNSUPPORTED, std::string(what) + ": more than 65536 sequences");
+    if (b->n_seq > 0 && b->n_tok > 0 && (!b->d_q_start || !b->d_len || !b->d_table)) return fail(ELB_ERR_INVALID, std::string(what) + ": null argument");
+    if (b->table_ld < 0 || (b->n_seq > 0 && b->table_ld == 0)) return fail(ELB_ERR_INVALID, std::string(what) + ": a page table needs a positive row stride");
+    if (b->table_ld > (int64_t(1) << 30) / kv->page) return fail(ELB_ERR_UNSUPPORTED, std::string(what) + ": tables for more than 2^30 positions");  // (a pool has fewer)
     return ELB_OK;
 }
 
