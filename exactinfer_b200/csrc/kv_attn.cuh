@@ -19,11 +19,15 @@ struct KvAttnArgs {
     // ranges of `chunk` (the last takes what is left). Narrow kernel: tiles_max of every sequence, tiles from tiles_max on are not
     // cut. 128-row tiles: tiles_max of all sequences together, counted through (kv_tile_of).
     int splits, chunk, tiles_max;
-    float* part;         // [tile][key head][split]: R rows of 128 sums, then R maxima, then R denominators
+    float* part;         // [tile][key head][split]: R rows of 128 sums, then R maxima (of S), R denominators, R factors f (KA_ROW words a row)
     int few_max;         // both kernels run: sequences of up to so many query rows belong to the narrow one (0: one kernel has all)
 };
 
-constexpr float KA_P = 14.f;  // weights are formed as 2^(x - m + 14): small ones keep their bits in fp16
+// Weights are formed as 2^((S - m) f + 14), m the largest S of the row so far: small ones keep their bits in fp16. The difference comes first:
+// it is never above 0 and exact where weights count, so that no weight passes 2^14 and the largest is 2^14 however large the
+// scores S f are. (As 2^(S f - (m f - 14)), rounded at m f, weights overflowed or all vanished from scores of 2^25 on.)
+constexpr float KA_P = 14.f;
+constexpr int KA_ROW = KV_D + 3;  // words of a row's partial result
 
 // what is visible: positions 0 .. kv_visible - 1 to token t of a sequence (as far as the table goes)
 __device__ __forceinline__ int kv_visible(const KvRows& b, const KvSeq& s, int t) {
@@ -92,17 +96,20 @@ __device__ __forceinline__ void half_pair_finite(float x, float y, uint32_t& hi,
     lo = *reinterpret_cast<const uint32_t*>(&l);
 }
 
-// Power of two that brings a row of queries with largest magnitude m into [2^14, 2^15), and what undoes it in the scale
+// Power of two 2^k that brings a row of queries with largest magnitude m into [2^14, 2^15), with the sign of the scale, and what undoes it in
+// the scale. f is kept from 0 and infinity, which would make NaN of the -infinity of masked scores and of S - m = 0: S is below
+// 2^39, so that below 1e-37 all scores are 0, and at the largest fp32 number all but the largest weigh nothing.
 struct RowScale {
     Pow2 up;
-    float f;  // scale2 * 2^-k
+    float f;  // |scale2| * 2^-k
 };
 __device__ __forceinline__ RowScale row_scale(float m, float scale2) {
     const int e = int((__float_as_uint(m) >> 23) & 255u);
     const int k = m > 0.f && e < 255 ? 14 - (max(e, 1) - 127) : 0;
     RowScale r{make_pow2(k), 0.f};
     const Pow2 down = make_pow2(-k);
-    r.f = scale2 * down.s1 * down.s2;
+    r.f = fminf(fmaxf(fabsf(scale2) * down.s1 * down.s2, 1e-37f), 3.4028235e38f);
+    if (scale2 < 0.f) r.up.s1 = -r.up.s1;
     return r;
 }
 

@@ -30,7 +30,7 @@ template <int PL, int NT> struct FewShape {
     static constexpr int TILE = KF_KEYS * KV_D * 2;  // bytes of 16 keys, one plane
     static constexpr int STAGE = 2 * PL * TILE;
     static constexpr int SMEM = KF_WARPS * STAGES * STAGE;
-    static_assert(SMEM >= KF_WARPS * ROWS * (KF_LD + 2) * 4, "the warps' results take the place of the rings");
+    static_assert(SMEM >= KF_WARPS * ROWS * (KF_LD + 4) * 4, "the warps' results take the place of the rings");
 };
 
 __device__ __forceinline__ void ldsm4(uint32_t (&r)[4], uint32_t a) {
@@ -106,7 +106,7 @@ __global__ void __launch_bounds__(KF_THREADS) k_kv_attn_few(const KvAttnArgs a) 
 
         // queries: lane (g, t) holds, of row g of each group of 8, the values 16 ks + 2 t, + 1, + 8, + 9 as hi and lo
         uint32_t qh[NT][8][2], ql[NT][8][2];
-        float f[NT][2];     // scale of rows 2 t, 2 t + 1
+        float f[NT][2];     // factors of rows 2 t, 2 t + 1
         int see[NT][2];     // their visible keys
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) {
@@ -172,8 +172,8 @@ __global__ void __launch_bounds__(KF_THREADS) k_kv_attn_few(const KvAttnArgs a) 
             for (int nt = 0; nt < NT; ++nt) {
 #pragma unroll
                 for (int b = 0; b < 2; ++b) {  // row 2 t + b: keys g and g + 8
-                    float x0 = (sh[nt][0][b] + sh[nt][1][b] + sx[nt][b]) * f[nt][b];
-                    float x1 = (sh[nt][0][b + 2] + sh[nt][1][b + 2] + sx[nt][b + 2]) * f[nt][b];
+                    float x0 = sh[nt][0][b] + sh[nt][1][b] + sx[nt][b];
+                    float x1 = sh[nt][0][b + 2] + sh[nt][1][b + 2] + sx[nt][b + 2];
                     if (edge) {
                         if (key0 + g >= see[nt][b]) x0 = -INFINITY;
                         if (key0 + g + 8 >= see[nt][b]) x1 = -INFINITY;
@@ -183,11 +183,11 @@ __global__ void __launch_bounds__(KF_THREADS) k_kv_attn_few(const KvAttnArgs a) 
                     mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 8));
                     mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 16));
                     mx = fmaxf(mx, m[nt][b]);
-                    corr[nt][b] = mx == -INFINITY ? 1.f : ex2(m[nt][b] - mx);
+                    corr[nt][b] = mx == -INFINITY ? 1.f : ex2((m[nt][b] - mx) * f[nt][b]);
                     m[nt][b] = mx;
-                    const float base = mx == -INFINITY ? 0.f : mx - KA_P;
-                    p[nt][b] = ex2(x0 - base);
-                    p[nt][b + 2] = ex2(x1 - base);
+                    const float base = mx == -INFINITY ? 0.f : mx;
+                    p[nt][b] = ex2(fmaf(x0 - base, f[nt][b], KA_P));
+                    p[nt][b + 2] = ex2(fmaf(x1 - base, f[nt][b], KA_P));
                     l[nt][b] = l[nt][b] * corr[nt][b] + (p[nt][b] + p[nt][b + 2]);
                 }
                 half_pair_finite(p[nt][0], p[nt][1], ph[nt][0], pl[nt][0]);
@@ -255,8 +255,8 @@ __global__ void __launch_bounds__(KF_THREADS) k_kv_attn_few(const KvAttnArgs a) 
         }
         asm volatile("cp.async.wait_group 0;" ::: "memory");
         __syncthreads();  // the rings are free on every warp
-        float* sO = reinterpret_cast<float*>(few_smem);  // [warp][row][KF_LD], then [warp][row] (m, l)
-        float2* sml = reinterpret_cast<float2*>(sO + KF_WARPS * S::ROWS * KF_LD);
+        float* sO = reinterpret_cast<float*>(few_smem);  // [warp][row][KF_LD], then [warp][row] (m, l, f)
+        float4* sml = reinterpret_cast<float4*>(sO + KF_WARPS * S::ROWS * KF_LD);
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) {
 #pragma unroll
@@ -265,7 +265,7 @@ __global__ void __launch_bounds__(KF_THREADS) k_kv_attn_few(const KvAttnArgs a) 
                 v += __shfl_xor_sync(0xffffffffu, v, 4);
                 v += __shfl_xor_sync(0xffffffffu, v, 8);
                 v += __shfl_xor_sync(0xffffffffu, v, 16);
-                if (g == 0) sml[warp * S::ROWS + nt * 8 + 2 * t + b] = make_float2(m[nt][b], v);
+                if (g == 0) sml[warp * S::ROWS + nt * 8 + 2 * t + b] = make_float4(m[nt][b], v, f[nt][b], 0.f);
             }
             float* dst = sO + (warp * S::ROWS + nt * 8 + 2 * t) * KF_LD + g;
 #pragma unroll
@@ -276,7 +276,7 @@ __global__ void __launch_bounds__(KF_THREADS) k_kv_attn_few(const KvAttnArgs a) 
         __syncthreads();
         const bool final_here = !cut || vis <= a.chunk;
         const int64_t slot = ((int64_t(s) * a.tiles_max + i) * a.HKV + j) * a.splits + c;
-        float* part = a.part + slot * S::ROWS * (KV_D + 2);
+        float* part = a.part + slot * S::ROWS * KA_ROW;
         for (int r = 0; r < S::ROWS; ++r) {
             const int row = i * S::ROWS + r;
             if (row >= nrows) break;
@@ -285,8 +285,8 @@ __global__ void __launch_bounds__(KF_THREADS) k_kv_attn_few(const KvAttnArgs a) 
             for (int w = 0; w < KF_WARPS; ++w) M = fmaxf(M, sml[w * S::ROWS + r].x);
 #pragma unroll
             for (int w = 0; w < KF_WARPS; ++w) {
-                const float2 ml = sml[w * S::ROWS + r];
-                const float k = M == -INFINITY ? 1.f : ex2(ml.x - M);
+                const float4 ml = sml[w * S::ROWS + r];
+                const float k = M == -INFINITY ? 1.f : ex2((ml.x - M) * ml.z);
                 den += k * ml.y;
                 num += k * sO[(w * S::ROWS + r) * KF_LD + tid];
             }
@@ -294,7 +294,7 @@ __global__ void __launch_bounds__(KF_THREADS) k_kv_attn_few(const KvAttnArgs a) 
                 a.out[(sq.row0 + row / a.group) * a.ldo + (j * a.group + row % a.group) * KV_D + tid] = den == 0.f ? 0.f : num / den;
             } else {
                 part[r * KV_D + tid] = num;
-                if (tid == 0) { part[S::ROWS * KV_D + r] = M; part[S::ROWS * (KV_D + 1) + r] = den; }
+                if (tid == 0) { part[S::ROWS * KV_D + r] = M; part[S::ROWS * (KV_D + 1) + r] = den; part[S::ROWS * (KV_D + 2) + r] = sml[r].z; }
             }
         }
         __syncthreads();  // before the rings fill again
@@ -327,16 +327,17 @@ __global__ void __launch_bounds__(256) k_kv_attn_join(const KvAttnArgs a) {
     const int vis = kv_visible(a.rows, sq, min(((i + 1) * ROWS - 1) / a.group, sq.nq - 1));
     if (vis <= a.chunk) return;
     const int n = min(a.splits, (vis + a.chunk - 1) / a.chunk);
-    const float* part = a.part + slot * ROWS * (KV_D + 2);
+    const float* part = a.part + slot * ROWS * KA_ROW;
+    const float f = part[ROWS * (KV_D + 2) + r];
     float M = -INFINITY;
-    for (int c = lane; c < n; c += 32) M = fmaxf(M, part[c * ROWS * (KV_D + 2) + ROWS * KV_D + r]);
+    for (int c = lane; c < n; c += 32) M = fmaxf(M, part[c * ROWS * KA_ROW + ROWS * KV_D + r]);
     M = warp_max(M);
     float den = 0.f;
     float4 num = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll 4
     for (int c = 0; c < n; ++c) {
-        const float* p = part + int64_t(c) * ROWS * (KV_D + 2);
-        const float k = M == -INFINITY ? 1.f : ex2(p[ROWS * KV_D + r] - M);
+        const float* p = part + int64_t(c) * ROWS * KA_ROW;
+        const float k = M == -INFINITY ? 1.f : ex2((p[ROWS * KV_D + r] - M) * f);
         const float4 v = *reinterpret_cast<const float4*>(p + r * KV_D + lane * 4);
         den += k * p[ROWS * (KV_D + 1) + r];
         num.x += k * v.x; num.y += k * v.y; num.z += k * v.z; num.w += k * v.w;
@@ -398,7 +399,7 @@ int kv_attn_join(const KvAttnArgs& a, int rows, int64_t tiles, cudaStream_t s) {
 size_t kv_attn_few_work(const Kv* kv, const elb_kv_batch* b, int n_head, int few_max) {
     const FewPlan p = few_plan(kv, b, n_head, few_max);
     if (p.splits == 1) return 0;
-    return size_t(b->n_seq) * p.tiles * kv->HKV * p.splits * 8 * p.nt * (KV_D + 2) * 4;
+    return size_t(b->n_seq) * p.tiles * kv->HKV * p.splits * 8 * p.nt * KA_ROW * 4;
 }
 
 int kv_attn_few_launch(const Kv* kv, KvAttnArgs a, const elb_kv_batch* b, cudaStream_t s) {

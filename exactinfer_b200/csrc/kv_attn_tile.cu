@@ -2,7 +2,7 @@
 // 5th-generation tensor cores.
 //
 // A CTA takes 128 query rows of one sequence and key head (tokens x the query heads that share the key head) and walks the keys
-// that they see, 128 at a time: S = Q K^T, weights 2^(scale2 S - m + 14), O += P V. fp32 accuracy from fp16 operands as in
+// that they see, 128 at a time: S = Q K^T, weights 2^((S - m) f + 14), O += P V. fp32 accuracy from fp16 operands as in
 // kv_attn_few.cu: a query row is scaled by a power of two and held as hi + lo (22 bits), the weights as well, keys and
 // values are one fp16 or a pair as the cache holds them; lo lo is left out, so that a product costs 2 MMAs (F16 cache) or 3 (pairs).
 // The tensor core adds with truncation: the small products of a step go first, hi hi (8 links for S, 4 for O) last, and
@@ -200,17 +200,17 @@ template <bool EDGE> __device__ __forceinline__ float tile_weights(uint32_t sp, 
         }
         mx = fmaxf(max3(u[0], u[1], u[2]), u[3]);
     }
-    mx = fmaxf(m, mx * f);
-    const float corr = mx == -INFINITY ? 1.f : ex2(m - mx), base = mx == -INFINITY ? 0.f : mx - KA_P;
+    mx = fmaxf(m, mx);
+    const float corr = mx == -INFINITY ? 1.f : ex2((m - mx) * f), base = mx == -INFINITY ? 0.f : mx;
     m = mx;
-    const Two ff = two(f, f), nb = two(-base, -base), minus = two(-1.f, -1.f);
+    const Two ff = two(f, f), nb = two(-base, -base), up = two(KA_P, KA_P), minus = two(-1.f, -1.f);
     Two sum = two(0.f, 0.f), sum_b = sum;
     auto weigh = [&](const uint32_t (&x)[16], int h) {
         uint32_t p[16];
 #pragma unroll
         for (int i = 0; i < 16; i += 2) {
             const uint32_t x0 = EDGE && i >= left - h ? 0xff800000u : x[i], x1 = EDGE && i + 1 >= left - h ? 0xff800000u : x[i + 1];
-            const float2 y = parts(fma2(two(x0, x1), ff, nb));
+            const float2 y = parts(fma2(add2(two(x0, x1), nb), ff, up));
             const float p0 = ex2(y.x), p1 = ex2(y.y);
             const Two pp = two(p0, p1);
             if (i & 2) sum_b = add2(sum_b, pp);
@@ -507,10 +507,9 @@ __global__ void __launch_bounds__(KT_THREADS, 1) k_kv_attn_tile(const __grid_con
                 }
                 ex[team * 128 + r] = mx;
                 asm volatile("bar.sync 1, 256;" ::: "memory");
-                const RowScale rs = row_scale(fmaxf(ex[r], ex[128 + r]), fabsf(a.scale2));  // (a negative scale goes into the queries)
-                f = fmaxf(rs.f, 1e-37f);  // (0 would make NaN of the masked scores, which are -infinity; scores are below 2^39)
-                const float s1 = a.scale2 < 0.f ? -rs.up.s1 : rs.up.s1;
-                const Two k1 = two(s1, s1), k2 = two(rs.up.s2, rs.up.s2);
+                const RowScale rs = row_scale(fmaxf(ex[r], ex[128 + r]), a.scale2);
+                f = rs.f;
+                const Two k1 = two(rs.up.s1, rs.up.s1), k2 = two(rs.up.s2, rs.up.s2);
                 uint32_t hi[32], lo[32];
 #pragma unroll
                 for (int u = 0; u < 16; ++u) {
@@ -603,7 +602,7 @@ __global__ void __launch_bounds__(KT_THREADS, 1) k_kv_attn_tile(const __grid_con
             ex[257 + (team * 128 + r) * 2] = l;
             asm volatile("bar.sync 1, 256;" ::: "memory");
             const float m0 = ex[256 + r * 2], l0 = ex[257 + r * 2], m1 = ex[512 + r * 2], l1 = ex[513 + r * 2];
-            const float M = fmaxf(m0, m1), k0 = M == -INFINITY ? 1.f : ex2(m0 - M), k1 = M == -INFINITY ? 1.f : ex2(m1 - M);
+            const float M = fmaxf(m0, m1), k0 = M == -INFINITY ? 1.f : ex2((m0 - M) * f), k1 = M == -INFINITY ? 1.f : ex2((m1 - M) * f);
             const float den = k0 * l0 + k1 * l1, k = team ? k1 : k0;
             const bool final_here = !b.cut || b.vis <= a.chunk;
             const float inv = final_here ? (den == 0.f ? 0.f : 1.f / den) : 1.f;
@@ -616,8 +615,8 @@ __global__ void __launch_bounds__(KT_THREADS, 1) k_kv_attn_tile(const __grid_con
                 own_row[d / 4] = make_float4(x.x * ki, x.y * ki, y.x * ki, y.y * ki);
             }
             const int64_t slot = (int64_t(u) * a.HKV + b.j) * a.splits + b.c;
-            float* part = a.part + slot * KT_ROWS * (KV_D + 2);
-            if (!final_here && team == 0) { part[KT_ROWS * KV_D + r] = M; part[KT_ROWS * (KV_D + 1) + r] = den; }
+            float* part = a.part + slot * KT_ROWS * KA_ROW;
+            if (!final_here && team == 0) { part[KT_ROWS * KV_D + r] = M; part[KT_ROWS * (KV_D + 1) + r] = den; part[KT_ROWS * (KV_D + 2) + r] = f; }
             asm volatile("bar.sync 1, 256;" ::: "memory");
             if (ok) {
                 RowWalk w = first;
@@ -698,7 +697,7 @@ int kv_attention_check() {
 size_t kv_attn_tile_work(const Kv* kv, const elb_kv_batch* b, int n_head, int few_max) {
     const TilePlan p = tile_plan(kv, b, n_head, few_max);
     if (p.splits == 1) return 0;
-    return size_t(p.tiles) * kv->HKV * p.splits * KT_ROWS * (KV_D + 2) * 4;
+    return size_t(p.tiles) * kv->HKV * p.splits * KT_ROWS * KA_ROW * 4;
 }
 
 int kv_attn_tile_launch(const Kv* kv, int layer, KvAttnArgs a, const elb_kv_batch* b, cudaStream_t s) {
