@@ -35,6 +35,28 @@ __device__ __forceinline__ int kv_visible(const KvRows& b, const KvSeq& s, int t
     return int(min(int64_t(max(s.len - s.nq + t + 1, 0)), cap));
 }
 
+// Dimension d of a row whose sum came out as NaN though its scores are finite: there are values that are not. Every weight is above 0, so
+// the sum of these values alone is the result: the infinity among them, NaN beside one of the other sign or a NaN. (In the products 0 *
+// infinity spoils it: the lower half of a weight is often 0. To search every tile for infinities would cost every call.)
+__device__ __forceinline__ float kv_not_finite(const KvAttnArgs& a, int s, int j, int vis, int d) {
+    const int64_t plane = int64_t(a.rows.page) * KV_D;
+    float sum = 0.f;
+#pragma unroll 1
+    for (int key0 = 0; key0 < vis && sum == sum; key0 += 16) {  // (a page holds 16 positions at least)
+        const int pg = kv_page(a.rows, s, key0);
+        if (pg < 0) continue;
+        const __half* v = a.pool + ((int64_t(pg) * 2 + 1) * a.HKV + j) * a.planes * plane + (key0 & (a.rows.page - 1)) * KV_D + d;
+#pragma unroll 4
+        for (int i = 0; i < 16; ++i) {
+            if (key0 + i >= vis) continue;
+            float x = __half2float(v[i * KV_D]);
+            if (a.planes == 2) x += __half2float(v[plane + i * KV_D]);
+            if (!(fabsf(x) < INFINITY)) sum += x;
+        }
+    }
+    return sum == 0.f ? NAN : sum;
+}
+
 // The u-th 128-row tile of a batch: its sequence and its number there; false when there are fewer. A whole warp calls it with the same u.
 __device__ __forceinline__ bool kv_tile_of(const KvAttnArgs& a, int u, int* s, int* i) {
     if (a.rows.n_seq == 1) {

@@ -291,7 +291,9 @@ __global__ void __launch_bounds__(KF_THREADS) k_kv_attn_few(const KvAttnArgs a) 
                 num += k * sO[(w * S::ROWS + r) * KF_LD + tid];
             }
             if (final_here) {
-                a.out[(sq.row0 + row / a.group) * a.ldo + (j * a.group + row % a.group) * KV_D + tid] = den == 0.f ? 0.f : num / den;
+                float y = den == 0.f ? 0.f : num / den;
+                if (y != y && den > 0.f) y = kv_not_finite(a, s, j, kv_visible(a.rows, sq, row / a.group), tid);
+                a.out[(sq.row0 + row / a.group) * a.ldo + (j * a.group + row % a.group) * KV_D + tid] = y;
             } else {
                 part[r * KV_D + tid] = num;
                 if (tid == 0) { part[S::ROWS * KV_D + r] = M; part[S::ROWS * (KV_D + 1) + r] = den; part[S::ROWS * (KV_D + 2) + r] = sml[r].z; }
@@ -343,8 +345,15 @@ __global__ void __launch_bounds__(256) k_kv_attn_join(const KvAttnArgs a) {
         num.x += k * v.x; num.y += k * v.y; num.z += k * v.z; num.w += k * v.w;
     }
     const float inv = den == 0.f ? 0.f : 1.f / den;
-    *reinterpret_cast<float4*>(a.out + (sq.row0 + row / a.group) * a.ldo + (j * a.group + row % a.group) * KV_D + lane * 4) =
-        make_float4(num.x * inv, num.y * inv, num.z * inv, num.w * inv);
+    float* out = a.out + (sq.row0 + row / a.group) * a.ldo + (j * a.group + row % a.group) * KV_D + lane * 4;
+    const float4 y = make_float4(num.x * inv, num.y * inv, num.z * inv, num.w * inv);
+    *reinterpret_cast<float4*>(out) = y;
+    if (den > 0.f && !((y.x + y.y) + (y.z + y.w) < INFINITY))
+#pragma unroll 1
+        for (int e = 0; e < 4; ++e) {
+            const float z = e == 0 ? y.x : e == 1 ? y.y : e == 2 ? y.z : y.w;
+            if (z != z) out[e] = kv_not_finite(a, s, j, kv_visible(a.rows, sq, row / a.group), lane * 4 + e);
+        }
 }
 
 struct FewPlan { int nt, tiles, splits, chunk; };

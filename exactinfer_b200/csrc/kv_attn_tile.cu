@@ -620,12 +620,30 @@ __global__ void __launch_bounds__(KT_THREADS, 1) k_kv_attn_tile(const __grid_con
             asm volatile("bar.sync 1, 256;" ::: "memory");
             if (ok) {
                 RowWalk w = first;
+                bool odd = false;  // some result may be NaN
 #pragma unroll 4
                 for (int q = warp * 16; q < warp * 16 + 16; ++q, w.step(a.group)) {
                     const float4 x = *reinterpret_cast<const float4*>(stage + q * KT_LD + lane * 4);
                     const float4 y = *reinterpret_cast<const float4*>(stage + (KT_ROWS + q) * KT_LD + lane * 4);
                     float* dst = final_here ? a.out + (b.sq.row0 + w.token) * a.ldo + (b.j * a.group + w.head) * KV_D : part + q * KV_D;
-                    if (w.row < nrows) *reinterpret_cast<float4*>(dst + lane * 4) = make_float4(x.x + y.x, x.y + y.y, x.z + y.z, x.w + y.w);
+                    const float4 z = make_float4(x.x + y.x, x.y + y.y, x.z + y.z, x.w + y.w);
+                    if (w.row < nrows) *reinterpret_cast<float4*>(dst + lane * 4) = z;
+                    odd |= !((z.x + z.y) + (z.z + z.w) < INFINITY);
+                }
+                if (final_here && __any_sync(0xffffffffu, odd)) {
+                    w = first;
+#pragma unroll 1
+                    for (int q = warp * 16; q < warp * 16 + 16 && w.row < nrows; ++q, w.step(a.group)) {
+                        const float most = fmaxf(ex[256 + q * 2], ex[512 + q * 2]), sums = ex[257 + q * 2] + ex[513 + q * 2];
+                        if (!(sums > 0.f) || most == -INFINITY) continue;  // (its scores are not finite)
+#pragma unroll 1
+                        for (int d = lane * 4; d < lane * 4 + 4; ++d) {
+                            const float z = stage[q * KT_LD + d] + stage[(KT_ROWS + q) * KT_LD + d];
+                            if (z != z)
+                                a.out[(b.sq.row0 + w.token) * a.ldo + (b.j * a.group + w.head) * KV_D + d] =
+                                    kv_not_finite(a, b.s, b.j, kv_visible(a.rows, b.sq, w.token), d);
+                        }
+                    }
                 }
             }
         }

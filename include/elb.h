@@ -351,7 +351,9 @@ int elb_kv_append_dev(elb_kv* kv, int layer, const elb_kv_batch* b, const elb_ro
  * key head h / (n_head / n_head_kv): out = sum_j softmax_j(scale q.k_j) v_j. Every row's queries are used as given (append's
  * q_out). A row at a negative position has no keys: its output is 0. Rows outside every range are left as they are.
  * What lies in a page behind a sequence's length has no influence, infinities and NaN included; nor has a key or value that
- * a row does not attend to. A row that attends to an infinite or NaN key is NaN or 0. d_out must not overlap d_q. n_head: a multiple of n_head_kv, at most 64 times it. Row strides in floats, rows on 16-byte
+ * a row does not attend to. A row that attends to an infinite or NaN key, or has one among its queries, is NaN or 0. An infinite value that
+ * a row of finite scores attends to makes that dimension of it infinite, however small its weight; with one of the other sign, or a NaN,
+ * it is NaN. d_out must not overlap d_q. n_head: a multiple of n_head_kv, at most 64 times it. Row strides in floats, rows on 16-byte
  * boundaries. d_work: elb_kv_attention_work bytes, 256-byte aligned; what it holds before and after does not matter. */
 size_t elb_kv_attention_work(const elb_kv* kv, const elb_kv_batch* b, int n_head); /* 0: bad argument */
 int elb_kv_attention_dev(const elb_kv* kv, int layer, const elb_kv_batch* b, const float* d_q, int64_t ldq, int n_head, float scale,

@@ -1,4 +1,4 @@
-"""Attention over the pages at the ends of the numbers' range: scores of any size."""
+"""Attention over the pages at the ends of the numbers' range: scores of any size, values that are not finite."""
 import math
 
 import pytest
@@ -42,3 +42,40 @@ def test_scores_of_any_size(nq, n, h, hkv, size, scale, kind):
             assert ((mine - v[at]).abs() <= tol)[alone].all()
             decided, rows = decided + int(alone.sum()), rows + m
     assert decided > rows // 2
+
+
+INF, NAN = math.inf, math.nan
+
+
+@pytest.mark.parametrize("kind", (e.KV_F16, e.KV_PAIR))
+@pytest.mark.parametrize("scale", (0.09, 30.0))
+@pytest.mark.parametrize("nq,n,h,hkv,page", [(1, 90, 4, 2, 16), (1, 4000, 2, 1, 64), (4, 90, 4, 2, 16), (4, 3000, 8, 4, 128), (50, 90, 4, 2, 32), (200, 700, 2, 2, 256),
+                                             (60, 5000, 4, 2, 16)])
+def test_attended_values_that_are_not_finite(nq, n, h, hkv, page, scale, kind):
+    """Every weight is above 0, so an infinite value is the result of its dimension in all rows that attend to it, wherever in a tile it lies
+    and however little it weighs; infinities of both signs, or a NaN, give NaN. Other dimensions and earlier rows do not notice."""
+    p = base.Paged(51, hkv, page, kind, (nq,), (n,)).fill()
+    # (position, dimension, value), in the last key head
+    places = [(0, 3, INF), (n - 1, 7, -INF), (n - nq // 2 - 1, 64, INF), (n // 3, 127, INF), (n // 2, 127, -INF), (n // 4, 90, NAN), (n // 5, 90, INF),
+              (n - 2, 31, NAN), (n // 2 + 1, 0, -INF), (n // 2 + 2, 0, -INF)]
+    v = p.vals[0][1, hkv - 1]
+    for t, d, x in places:
+        p.pool[1, int(p.table[0, t // page]), 1, hkv - 1, 0, t % page, d] = x
+        if kind == e.KV_PAIR:
+            p.pool[1, int(p.table[0, t // page]), 1, hkv - 1, 1, t % page, d] = 0.0
+        v[t, d] = x
+    q = base.randn(p.g, nq, h * D)
+    got = p.attention(h, q, scale=scale).to(F64)
+    want, tol = p.expected(h, q, scale)
+    last = torch.arange(n - nq, n, device="cuda")
+    for d in {d for _, d, _ in places}:
+        odd = torch.zeros(nq, dtype=F64, device="cuda")
+        for t, dd, x in places:
+            if dd == d:
+                odd += torch.where(last >= t, x, 0.0)
+        for i in range(h - h // hkv, h):
+            rows = odd != 0
+            want[rows, i * D + d], tol[rows, i * D + d] = odd[rows], 0.0
+    fine = want.isfinite()
+    assert ((got - want).abs() <= tol)[fine].all()
+    assert torch.equal(got[~fine].nan_to_num(5.0, INF, -INF), want[~fine].nan_to_num(5.0, INF, -INF))
