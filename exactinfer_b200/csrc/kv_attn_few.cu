@@ -274,6 +274,16 @@ __global__ void __launch_bounds__(KF_THREADS) k_kv_attn_few(const KvAttnArgs a) 
                 for (int e = 0; e < 4; ++e) dst[(e & 1) * KF_LD + mt * 16 + (e >> 1) * 8] = O[nt][mt][e];
         }
         __syncthreads();
+        if (NT == 2) {  // what each warp's sums count, once for all 128 dimensions (four tokens behind 300 keys 11.9 -> 11.3 us; 8 rows lose by the wait)
+            if (tid < KF_WARPS * S::ROWS) {
+                const int r = tid % S::ROWS;
+                float M = -INFINITY;
+#pragma unroll
+                for (int w = 0; w < KF_WARPS; ++w) M = fmaxf(M, sml[w * S::ROWS + r].x);
+                sml[tid].w = M == -INFINITY ? 1.f : ex2((sml[tid].x - M) * sml[tid].z);
+            }
+            __syncthreads();
+        }
         const bool final_here = !cut || vis <= a.chunk;
         const int64_t slot = ((int64_t(s) * a.tiles_max + i) * a.HKV + j) * a.splits + c;
         float* part = a.part + slot * S::ROWS * KA_ROW;
@@ -286,7 +296,7 @@ __global__ void __launch_bounds__(KF_THREADS) k_kv_attn_few(const KvAttnArgs a) 
 #pragma unroll
             for (int w = 0; w < KF_WARPS; ++w) {
                 const float4 ml = sml[w * S::ROWS + r];
-                const float k = M == -INFINITY ? 1.f : ex2((ml.x - M) * ml.z);
+                const float k = NT == 2 ? ml.w : M == -INFINITY ? 1.f : ex2((ml.x - M) * ml.z);
                 den += k * ml.y;
                 num += k * sO[(w * S::ROWS + r) * KF_LD + tid];
             }
