@@ -31,7 +31,7 @@ struct BeamBest { unsigned long long score; int token, pad; };  // score: beam_o
 
 // order of a logit as an unsigned number; 0: not a candidate (-infinity or NaN)
 __device__ __forceinline__ unsigned beam_key(float x) {
-    const unsigned u = __float_as_uint(x);
+    const unsigned u = __float_as_uint(x + 0.f);  // (-0 and 0 are equal logits)
     return x > -INFINITY ? (u & 0x80000000u ? ~u : u | 0x80000000u) : 0u;
 }
 __device__ __forceinline__ float beam_logit(unsigned key) {

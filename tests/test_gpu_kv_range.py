@@ -1,4 +1,5 @@
-"""Attention over the pages at the ends of the numbers' range: scores of any size, values that are not finite."""
+"""Attention over the pages and beam search's selection at the ends of the numbers' range: scores of any size, values that are not finite,
+zeros of both signs."""
 import math
 
 import pytest
@@ -79,3 +80,20 @@ def test_attended_values_that_are_not_finite(nq, n, h, hkv, page, scale, kind):
     fine = want.isfinite()
     assert ((got - want).abs() <= tol)[fine].all()
     assert torch.equal(got[~fine].nan_to_num(5.0, INF, -INF), want[~fine].nan_to_num(5.0, INF, -INF))
+
+
+@pytest.mark.parametrize("v", (1, 5, 700, 9001, 1100000))
+@pytest.mark.parametrize("masked", (False, True))
+def test_zeros_of_both_signs_are_equal_logits(v, masked):
+    """The lower token goes first, whichever sign its zero has; with few zeros at the top and with more than a block keeps."""
+    g = base.gen(52)
+    zero = torch.where(torch.rand(4, v, generator=g, device="cuda") < 0.5, -0.0, 0.0)
+    x = torch.where(torch.rand(4, v, generator=g, device="cuda") < 0.01, zero, -1.0)
+    x[1], x[2, :-1] = zero[1], -2.0
+    x[2, -1] = -0.0
+    x[3] = -zero[1]
+    allowed = torch.rand(4, v, generator=g, device="cuda") < 0.6 if masked else None
+    scores = torch.tensor([-1.0, -1.0, -2.0, -2.0], dtype=F64, device="cuda")
+    for k in (1, 2, 40):
+        if k <= 2 * v:
+            base.agree(base.select(x, scores, 2, 2, k, allowed), base.selected(x, scores, 2, 2, k, allowed), v)
