@@ -146,7 +146,8 @@ int kv_create(int device, int n_layer, int n_head_kv, int head_dim, int page, in
             return fail(ELB_ERR_MEMORY, "kv_create: out of device memory");
         }
         kv->owned = true;
-        const cudaError_t e = cudaMemset(kv->mem, 0, bytes);
+        cudaError_t e = cudaMemset(kv->mem, 0, bytes);  // (returns before it is done, and a caller's stream need not wait for the default one)
+        if (e == cudaSuccess) e = cudaStreamSynchronize(nullptr);
         if (e != cudaSuccess) {
             kv_destroy(kv);
             return fail(ELB_ERR_CUDA, std::string("kv_create: ") + cudaGetErrorString(e));

@@ -366,7 +366,8 @@ int rope_create(int device, const elb_rope_config* c, Rope** out) {
         delete r;
         return fail(ELB_ERR_MEMORY, "rope_create: out of device memory");
     }
-    const cudaError_t e = cudaMemcpy(r->d_turns, freq.data(), freq.size() * sizeof(double), cudaMemcpyHostToDevice);
+    cudaError_t e = cudaMemcpy(r->d_turns, freq.data(), freq.size() * sizeof(double), cudaMemcpyHostToDevice);
+    if (e == cudaSuccess) e = cudaStreamSynchronize(nullptr);  // (pageable memory: the copy returns once it is staged)
     if (e != cudaSuccess) {
         rope_destroy(r);
         return fail(ELB_ERR_CUDA, std::string("rope_create: ") + cudaGetErrorString(e));
