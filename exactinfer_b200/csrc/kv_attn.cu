@@ -29,7 +29,10 @@ int kv_attention_prepare() {
 }
 
 size_t kv_attention_work(const Kv* kv, const elb_kv_batch* b, int n_head) {
-    if (!kv || !b || n_head <= 0 || n_head % kv->HKV) return 0;
+    if (!kv || !b || n_head <= 0 || n_head % kv->HKV || n_head / kv->HKV > 64) return 0;
+    if (b->n_seq < 0 || b->n_seq > 65536 || b->n_tok < 0 || b->max_q < 0 || b->max_len < 0 || b->table_ld < 0 || b->table_ld > (int64_t(1) << 30) / kv->page) return 0;
+    if (b->n_seq == 0 || b->n_tok == 0) return 256;  // (the call has nothing to do, and the plans below divide by the sequences)
+    if (b->table_ld == 0) return 0;
     const AttnWay w = attn_way(b, n_head / kv->HKV);
     return std::max<size_t>(256, (w.few ? up256(kv_attn_few_work(kv, b, n_head, w.few_max)) : 0) + (w.tile ? kv_attn_tile_work(kv, b, n_head, w.few_max) : 0));
 }

@@ -35,3 +35,21 @@ def test_a_new_cache_is_used_at_once_on_another_stream(pages):
         want, tol = base.turned(x[:, :2 * D].double().view(1, 2, D), pos, rope.config)
         assert ((turned.double().view(1, 2, D) - want).abs() <= tol).all()
         kv.close()
+
+
+def test_working_memory_of_an_empty_batch_and_of_bad_ones():
+    """No rows or no sequences: nothing to plan for, and the call does nothing with that much memory. What the call refuses needs 0 bytes."""
+    kv = e.KvCache(1, 2, 16, 4)
+    t = torch.zeros(16, dtype=torch.int32, device="cuda")
+    batch = lambda **kw: e.KvBatch(**(dict(n_seq=2, n_tok=2, max_q=1, max_len=10, q_start=t, length=t, table=t, table_ld=2) | kw))
+    work = torch.empty(1 << 16, dtype=torch.uint8, device="cuda")
+    q = torch.zeros(2, 4 * D, device="cuda")
+    for kw in (dict(n_seq=0), dict(n_tok=0), dict(n_seq=0, n_tok=0, max_q=0, max_len=0, q_start=None, length=None, table=None, table_ld=0)):
+        need = kv.attention_work(batch(**kw), 4)
+        assert 0 < need <= work.numel()
+        kv.attention(0, batch(**kw), q, q, 4, 1.0, work, need, stream=base.stream())
+    for kw in (dict(n_seq=-1), dict(n_seq=65537), dict(n_tok=-1), dict(max_q=-1), dict(max_len=-1), dict(table_ld=-1), dict(table_ld=0), dict(table_ld=1 << 40)):
+        assert kv.attention_work(batch(**kw), 4) == 0
+    for h in (0, -2, 3, 2 * 65):
+        assert kv.attention_work(batch(), h) == 0
+    assert kv.attention_work(batch(), 2 * 64) > 0
