@@ -1229,6 +1229,19 @@ int model_eval_batch_top(Model* m, int n, const int32_t* tokens, const int32_t* 
     return eval_batch_impl(m, n, tokens, seq, pos, want, nullptr, &top);
 }
 
+// Is there room for count[s] rows of every sequence s from position first[s] on? Nothing is changed.
+static int paged_room(Model* m, const std::vector<int>& first, const std::vector<int>& count) {
+    for (size_t s = 0; s < count.size(); ++s)
+        if (count[s] && first[s] > m->book.len[s]) return fail(ELB_ERR_RANGE, "eval_batch: a sequence's rows must continue what it has cached");
+    return m->book.fits(first, count) ? ELB_OK : fail(ELB_ERR_MEMORY, "eval_batch: no free page left in the cache");
+}
+static int paged_room(Model* m, int seq, int pos0, int n) {
+    std::vector<int> first(size_t(m->n_seq), 0), count(size_t(m->n_seq), 0);
+    first[size_t(seq)] = pos0;
+    count[size_t(seq)] = n;
+    return paged_room(m, first, count);
+}
+
 // Rows of a batch over the paged cache: order[i] = place of the caller's row i when the rows of every sequence stand together;
 // pages for all positions that will be written (a last page that others use as well is copied first), lengths and tables to
 // the device. Nothing is changed when a page is missing.
@@ -1240,10 +1253,7 @@ static int paged_batch(Model* m, int n, const int32_t* seq, const int32_t* pos, 
         ++count[size_t(seq[i])];
     }
     PageBook& book = m->book;
-    for (int s = 0; s < S; ++s)
-        if (count[size_t(s)] && first[size_t(s)] > book.len[size_t(s)])
-            return fail(ELB_ERR_RANGE, "eval_batch: a sequence's rows must continue what it has cached");
-    if (!book.fits(first, count)) return fail(ELB_ERR_MEMORY, "eval_batch: no free page left in the cache");
+    ELB_TRY(paged_room(m, first, count));
     for (int s = 0; s < S; ++s)
         if (count[size_t(s)]) book.shorten(s, first[size_t(s)]);
     int at = 0, max_q = 1, max_len = 1;
@@ -1426,8 +1436,9 @@ static int eval_batch_impl(Model* m, int n, const int32_t* tokens, const int32_t
     return ELB_OK;
 }
 
-// model_eval over the paged cache: chunks of rows of sequence 0
+// model_eval over the paged cache: chunks of rows of sequence 0, when there are pages for all of them
 static int paged_eval(Model* m, const int32_t* tokens, int n, int pos0, float* logits, const TopOut* top) {
+    ELB_TRY(paged_room(m, 0, pos0, n));
     float ms = 0.f;
     int64_t launches = 0;
     for (int done = 0; done < n;) {
@@ -1547,6 +1558,7 @@ int model_eval_steps(Model* m, const int32_t* tokens, int n, int pos0, float* de
         if (tokens[i] < 0 || tokens[i] >= m->cfg.n_vocab) return fail(ELB_ERR_RANGE, "eval_steps: token id out of range");
     ELB_CUDA(cudaSetDevice(m->device));
     if (m->kv) {  // row by row
+        ELB_TRY(paged_room(m, 0, pos0, n));
         float ms = 0.f;
         int64_t launches = 0;
         for (int i = 0; i < n; ++i) {
