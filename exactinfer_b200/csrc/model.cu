@@ -122,7 +122,7 @@ struct Model {
     int *rows_dev = nullptr, *rows_host = nullptr;     // [n_seq + 1] first rows, [n_seq] lengths, pinned
     void* kv_work = nullptr;
     size_t kv_work_bytes = 0;
-    int* fork_dev = nullptr;                           // reorder: parent, spare, new lengths, taken [n_seq] each, then a table
+    int* fork_dev = nullptr;                           // reorder: parent, spare, new lengths, taken [n_seq] each, then a table; or a tail's copy: two rows
     // beam selection over the rows of a batch, for up to n_seq rows
     uint8_t *beam_dev = nullptr, *beam_host = nullptr;
     void* beam_work = nullptr;
@@ -913,7 +913,7 @@ static int finalize_pages(Model* m) {
     ELB_CUDA(cudaMallocHost(&m->table_host, table));
     ELB_CUDA(cudaMalloc(&m->rows_dev, rows));
     ELB_CUDA(cudaMallocHost(&m->rows_host, rows));
-    ELB_CUDA(cudaMalloc(&m->fork_dev, size_t(4 * m->n_seq) * sizeof(int) + table));
+    ELB_CUDA(cudaMalloc(&m->fork_dev, std::max(size_t(4 * m->n_seq) * sizeof(int) + table, size_t(10 + 4 * m->book.width) * sizeof(int))));
     return ELB_OK;
 }
 static int finalize_beams(Model* m) {
@@ -1242,21 +1242,42 @@ static int paged_room(Model* m, int seq, int pos0, int n) {
     return paged_room(m, first, count);
 }
 
+// Working memory for the attention of n rows, max_q of a sequence, up to max_len positions
+static int paged_work(Model* m, int n, int max_q, int max_len) {
+    const elb_kv_batch b{m->n_seq, n, max_q, max_len, nullptr, nullptr, nullptr, m->book.width};
+    const size_t work = kv_attention_work(m->kv, &b, m->H);
+    if (work <= m->kv_work_bytes) return ELB_OK;
+    void* more = nullptr;
+    if (device_malloc(&more, work) != cudaSuccess) return fail(ELB_ERR_MEMORY, "eval_batch: out of device memory");
+    cudaFree(m->kv_work);
+    m->kv_work = more;
+    m->kv_work_bytes = work;
+    return ELB_OK;
+}
+
 // Rows of a batch over the paged cache: order[i] = place of the caller's row i when the rows of every sequence stand together;
 // pages for all positions that will be written (a last page that others use as well is copied first), lengths and tables to
-// the device. Nothing is changed when a page is missing.
-static int paged_batch(Model* m, int n, const int32_t* seq, const int32_t* pos, std::vector<int>* order, elb_kv_batch* b) {
+// the device. Nothing is changed when a page or memory is missing; what fails later is undone by `rows`.
+static int paged_batch(Model* m, int n, const int32_t* seq, const int32_t* pos, std::vector<int>* order, elb_kv_batch* b, PagedRows* rows) {
     const int S = m->n_seq;
-    std::vector<int> count(size_t(S), 0), first(size_t(S), -1);
+    std::vector<int>&count = rows->count, &first = rows->first;
+    count.assign(size_t(S), 0);
+    first.assign(size_t(S), -1);
     for (int i = 0; i < n; ++i) {
         if (first[size_t(seq[i])] < 0) first[size_t(seq[i])] = pos[i];
         ++count[size_t(seq[i])];
     }
     PageBook& book = m->book;
     ELB_TRY(paged_room(m, first, count));
+    int at = 0, max_q = 1, max_len = 1;
+    for (int s = 0; s < S; ++s) {
+        max_q = std::max(max_q, count[size_t(s)]);
+        max_len = std::max(max_len, first[size_t(s)] + count[size_t(s)]);
+    }
+    ELB_TRY(paged_work(m, n, max_q, max_len));
+    rows->book = &book;
     for (int s = 0; s < S; ++s)
         if (count[size_t(s)]) book.shorten(s, first[size_t(s)]);
-    int at = 0, max_q = 1, max_len = 1;
     for (int s = 0; s < S; ++s) {
         m->rows_host[s] = at;
         m->rows_host[S + 1 + s] = 0;
@@ -1270,16 +1291,10 @@ static int paged_batch(Model* m, int n, const int32_t* seq, const int32_t* pos, 
             two.insert(two.end(), t.begin(), t.begin() + p0 / m->page + 1);
             const int width = p0 / m->page + 1;
             two.insert(two.end(), t.begin(), t.begin() + width);
-            int* d = nullptr;
-            if (cudaMalloc(&d, (two.size() + 4 + size_t(2) * width) * sizeof(int)) != cudaSuccess) {
-                book.drop(mine);
-                return fail(ELB_ERR_MEMORY, "eval_batch: out of device memory");
-            }
-            int* out = d + two.size();
+            int *d = m->fork_dev, *out = d + two.size();
             cudaError_t e = cudaMemcpyAsync(d, two.data(), two.size() * sizeof(int), cudaMemcpyHostToDevice, m->stream);
             const int rc = e == cudaSuccess ? kv_reorder_launch(m->kv, 2, d, d + 4, d + 6, width, d + 2, out, out + 4, out + 2, m->stream) : ELB_OK;
             if (e == cudaSuccess) e = cudaStreamSynchronize(m->stream);
-            cudaFree(d);
             if (rc != ELB_OK || e != cudaSuccess) {
                 book.drop(mine);
                 if (rc != ELB_OK) return rc;
@@ -1293,8 +1308,6 @@ static int paged_batch(Model* m, int n, const int32_t* seq, const int32_t* pos, 
         book.len[size_t(s)] = p1;
         m->rows_host[S + 1 + s] = p1;
         at += q;
-        max_q = std::max(max_q, q);
-        max_len = std::max(max_len, p1);
         for (int i = 0; i < book.width; ++i) m->table_host[size_t(s) * book.width + i] = i < int(t.size()) ? t[size_t(i)] : -1;
     }
     m->rows_host[S] = at;
@@ -1304,14 +1317,6 @@ static int paged_batch(Model* m, int n, const int32_t* seq, const int32_t* pos, 
     ELB_CUDA(cudaMemcpyAsync(m->rows_dev, m->rows_host, size_t(2 * S + 1) * sizeof(int), cudaMemcpyHostToDevice, m->stream));
     ELB_CUDA(cudaMemcpyAsync(m->table_dev, m->table_host, size_t(S) * book.width * sizeof(int), cudaMemcpyHostToDevice, m->stream));
     *b = elb_kv_batch{S, n, max_q, max_len, m->rows_dev, m->rows_dev + S + 1, m->table_dev, book.width};
-    const size_t work = kv_attention_work(m->kv, b, m->H);
-    if (work > m->kv_work_bytes) {
-        cudaFree(m->kv_work);
-        m->kv_work = nullptr;
-        m->kv_work_bytes = 0;
-        if (device_malloc(&m->kv_work, work) != cudaSuccess) return fail(ELB_ERR_MEMORY, "eval_batch: out of device memory");
-        m->kv_work_bytes = work;
-    }
     return ELB_OK;
 }
 
@@ -1346,8 +1351,9 @@ static int eval_batch_impl(Model* m, int n, const int32_t* tokens, const int32_t
     elb_kv_batch pages{};
     std::vector<int> order;
     std::vector<int32_t> sorted;
+    PagedRows paged_rows;
     if (m->kv) {
-        ELB_TRY(paged_batch(m, n, seq, pos, &order, &pages));
+        ELB_TRY(paged_batch(m, n, seq, pos, &order, &pages, &paged_rows));
         sorted.resize(size_t(n));
         for (int i = 0; i < n; ++i) sorted[size_t(order[size_t(i)])] = tokens[i];
         tokens = sorted.data();
@@ -1419,6 +1425,7 @@ static int eval_batch_impl(Model* m, int n, const int32_t* tokens, const int32_t
     ELB_TRY(gemm_tc_check());
     ELB_TRY(gemm_f16_tc_check());
     if (m->kv) ELB_TRY(kv_attention_check());
+    paged_rows.book = nullptr;  // they count
     if (out_dev && beam) {
         std::memcpy(beam->score, m->beam_host, picks * sizeof(double));
         std::memcpy(beam->parent, m->beam_host + picks * sizeof(double), picks * sizeof(int32_t));
@@ -1436,9 +1443,13 @@ static int eval_batch_impl(Model* m, int n, const int32_t* tokens, const int32_t
     return ELB_OK;
 }
 
-// model_eval over the paged cache: chunks of rows of sequence 0, when there are pages for all of them
+// model_eval over the paged cache: chunks of rows of sequence 0, when there are pages and memory for all of them
 static int paged_eval(Model* m, const int32_t* tokens, int n, int pos0, float* logits, const TopOut* top) {
     ELB_TRY(paged_room(m, 0, pos0, n));
+    for (int done = 0; done < n; done += m->max_batch) {
+        const int b = std::min(m->max_batch, n - done);
+        ELB_TRY(paged_work(m, b, b, pos0 + done + b));
+    }
     float ms = 0.f;
     int64_t launches = 0;
     for (int done = 0; done < n;) {
@@ -1559,6 +1570,7 @@ int model_eval_steps(Model* m, const int32_t* tokens, int n, int pos0, float* de
     ELB_CUDA(cudaSetDevice(m->device));
     if (m->kv) {  // row by row
         ELB_TRY(paged_room(m, 0, pos0, n));
+        for (int i = 1; i <= n; ++i) ELB_TRY(paged_work(m, 1, 1, pos0 + i));
         float ms = 0.f;
         int64_t launches = 0;
         for (int i = 0; i < n; ++i) {

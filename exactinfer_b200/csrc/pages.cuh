@@ -101,4 +101,17 @@ struct PageBook {
     }
 };
 
+// The rows of an evaluation that is under way: until it has ended well their positions do not count. When it goes out of scope before
+// that, its sequences end where its rows began.
+struct PagedRows {
+    PageBook* book = nullptr;        // null: nothing has been changed yet, or all is done
+    std::vector<int> first, count;   // per sequence
+    PagedRows() = default;
+    PagedRows(const PagedRows&) = delete;
+    ~PagedRows() {
+        for (size_t s = 0; book && s < count.size(); ++s)
+            if (count[s]) book->shorten(int(s), first[s]);
+    }
+};
+
 }  // namespace elb

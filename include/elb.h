@@ -218,8 +218,9 @@ int elb_model_eval_batch_beam(elb_model* m, int n, const int32_t* tokens, const 
 
 /* A paged cache instead of n_ctx contiguous fp32 rows per sequence: between create and finalize, n_pages pages of `page`
  * positions for all n_seq sequences together, values as in elb_kv_create (ELB_KV_F16, ELB_KV_PAIR). Pages are given out as
- * sequences grow; when none is left, an evaluation returns ELB_ERR_MEMORY and changes nothing. A sequence's rows must start at
- * most at its length, and cut it there. Every evaluation runs as a batch of rows through elb_kv_append_dev and
+ * sequences grow; when none is left, or no device memory, an evaluation returns ELB_ERR_MEMORY and changes nothing. After any other error
+ * of an evaluation that had begun, its sequences end where its rows began (or at the last chunk of a prompt that was finished). A
+ * sequence's rows must start at most at its length, and cut it there. Every evaluation runs as a batch of rows through elb_kv_append_dev and
  * elb_kv_attention_dev; the single-kernel decode step needs the contiguous cache. Not under tensor parallelism. */
 int elb_model_set_pages(elb_model* m, int page, int n_pages, int type);
 /* Sequence seq[i] goes on from the state of sequence parent[i], for all i at once (a beam search's step, or a shared prefix);

@@ -1,10 +1,12 @@
 """A paged model that lacks pages or device memory: the call is refused and leaves every sequence as it was."""
+import ctypes as C
+
 import numpy as np
 import pytest
 
 import exactinfer_b200 as e
 import test_gpu_paged_model as base
-from exactinfer_b200 import synth
+from exactinfer_b200 import capi, synth
 
 pytestmark = pytest.mark.gpu
 
@@ -35,3 +37,65 @@ def test_a_prompt_of_several_chunks_that_runs_out_of_pages(models, call, pos0):
     assert base.rel(paged.eval(toks[20:22], 20), flat.eval(toks[20:22], 20)) <= base.REL_TOL
     # what does fit: all four pages but the other sequence's
     assert base.rel(paged.eval(more[:48], 0), flat.eval(more[:48], 0)) <= base.REL_TOL
+
+
+@pytest.fixture
+def full_device():
+    """Calls that take all free device memory, down to pieces of 512 bytes, and give it back."""
+    held = []
+
+    def fill():
+        for size in (1 << 30, 1 << 26, 1 << 21, 1 << 16, 1 << 12, 512):
+            while True:
+                p = C.c_void_p()
+                if capi.lib().elb_malloc(0, size, C.byref(p)):
+                    break
+                held.append(p)
+
+    def give_back():
+        while held:
+            capi.lib().elb_free(held.pop())
+
+    yield fill, give_back
+    give_back()
+
+
+@pytest.mark.parametrize("call", ("eval", "eval_batch"))
+def test_no_device_memory_for_working_space(models, full_device, call):
+    """Longer contexts need more of it: without any the call is refused before a length or a table changes, and succeeds later."""
+    spec, make, _ = models
+    fill, give_back = full_device
+    flat, paged = make(n_ctx=1200), make(n_ctx=1200, pages=(16, 160, e.KV_PAIR))
+    rng = np.random.default_rng(31)
+    toks = rng.integers(0, spec.n_vocab, 1100)
+    paged.eval(toks[:505], 0)
+    free = paged.free_pages()
+    fill()
+    with pytest.raises(MemoryError):
+        if call == "eval":
+            paged.eval(toks[200:1100], 200)
+        else:
+            rows = np.concatenate([toks[:16], toks[500:515]])
+            paged.eval_batch(rows, [1] * 16 + [0] * 15, list(range(16)) + list(range(500, 515)), [0] * 30 + [1])
+    assert paged.free_pages() == free
+    give_back()
+    want = flat.eval(toks, 0)
+    assert base.rel(paged.eval(toks[505:], 505), want) <= base.REL_TOL
+
+
+def test_a_shared_last_page_is_copied_without_an_allocation(models, full_device):
+    spec, make, flat = models
+    fill, give_back = full_device
+    paged = make(pages=(16, 20, e.KV_PAIR))
+    rng = np.random.default_rng(32)
+    toks = rng.integers(0, spec.n_vocab, 40)
+    for s in (0, 1):
+        base.prompt(flat, s, toks[:32])
+    base.prompt(paged, 0, toks[:32])
+    paged.reorder([1], [0])
+    want = flat.eval_batch(toks[32:40], [0] * 4 + [1] * 4, list(range(20, 24)) * 2, [0, 0, 0, 1] * 2)
+    paged.eval_batch(toks[:1], [3], [0])  # (every kernel of the call has run)
+    fill()
+    got = paged.eval_batch(toks[32:40], [0] * 4 + [1] * 4, list(range(20, 24)) * 2, [0, 0, 0, 1] * 2)
+    give_back()
+    assert base.rel(got, want) <= base.REL_TOL
