@@ -1525,14 +1525,11 @@ int model_reorder(Model* m, int n, const int32_t* seq, const int32_t* parent) {
         named[size_t(seq[i])] = 1;
         from[size_t(seq[i])] = parent[i];
     }
-    const std::vector<char> copy = book.copies(from);
-    const int64_t need = std::count(copy.begin(), copy.end(), char(1));
-    if (need > int64_t(book.free.size())) return fail(ELB_ERR_MEMORY, "reorder: no free page left in the cache");
+    std::vector<int> spare;
+    if (!book.spares(from, book.copies(from), &spare)) return fail(ELB_ERR_MEMORY, "reorder: no free page left in the cache");
     if (n == 0) return ELB_OK;
     ELB_CUDA(cudaSetDevice(m->device));
-    std::vector<int> spare(size_t(S), -1);
     for (int s = 0; s < S; ++s) {
-        if (copy[size_t(s)]) spare[size_t(s)] = book.take();
         m->rows_host[s] = book.len[size_t(s)];
         const auto& t = book.table[size_t(s)];
         for (int i = 0; i < book.width; ++i) m->table_host[size_t(s) * book.width + i] = i < int(t.size()) ? t[size_t(i)] : -1;
@@ -1548,12 +1545,7 @@ int model_reorder(Model* m, int n, const int32_t* seq, const int32_t* parent) {
         ELB_CUDA(cudaStreamSynchronize(m->stream));
         return ELB_OK;
     };
-    const int rc = run();
-    if (rc != ELB_OK) {
-        for (int p : spare)
-            if (p >= 0) book.drop(p);
-        return rc;
-    }
+    ELB_TRY(run());
     book.reorder(from, spare);
     return ELB_OK;
 }

@@ -83,7 +83,28 @@ struct PageBook {
         }
         return copy;
     }
-    void reorder(const std::vector<int>& parent, const std::vector<int>& spare) {  // spare[s]: a page taken for s, or -1
+    // spare[s] = a page for every s that needs a copy, else -1: free pages, then those that only sequences which are replaced have. (Copies
+    // are made from pages that a first child keeps, so none of the latter is a source.) False: there are too few.
+    bool spares(const std::vector<int>& parent, const std::vector<char>& copy, std::vector<int>* spare) const {
+        size_t left = size_t(std::count(copy.begin(), copy.end(), char(1)));
+        std::vector<int> pages(free.end() - std::ptrdiff_t(std::min(left, free.size())), free.end());
+        if (pages.size() < left) {
+            std::vector<char> kept(refs.size(), 0);
+            for (size_t s = 0; s < parent.size(); ++s) {
+                const auto& t = table[size_t(parent[s])];
+                const int n = pages_of(len[size_t(parent[s])]) - copy[s];
+                for (int i = 0; i < n; ++i) kept[size_t(t[size_t(i)])] = 1;
+            }
+            for (size_t p = 0; p < refs.size() && pages.size() < left; ++p)
+                if (refs[p] && !kept[p]) pages.push_back(int(p));
+            if (pages.size() < left) return false;
+        }
+        spare->assign(parent.size(), -1);
+        for (size_t s = 0; s < parent.size(); ++s)
+            if (copy[s]) (*spare)[s] = pages[--left];
+        return true;
+    }
+    void reorder(const std::vector<int>& parent, const std::vector<int>& spare) {  // spare: as spares() gave them
         std::vector<std::vector<int>> next(table.size());
         std::vector<int> next_len(len.size());
         for (size_t s = 0; s < parent.size(); ++s) {
@@ -91,9 +112,9 @@ struct PageBook {
             next_len[s] = len[p];
             next[s].assign(table[p].begin(), table[p].begin() + pages_of(len[p]));
             if (spare[s] >= 0) next[s].back() = spare[s];
-            for (int pg : next[s])
-                if (pg != spare[s]) ++refs[size_t(pg)];
+            for (int pg : next[s]) ++refs[size_t(pg)];
         }
+        while (!free.empty() && refs[size_t(free.back())]) free.pop_back();  // (spares come from its end)
         for (auto& t : table)
             for (int pg : t) drop(pg);
         table.swap(next);

@@ -224,7 +224,8 @@ int elb_model_eval_batch_beam(elb_model* m, int n, const int32_t* tokens, const 
  * elb_kv_attention_dev; the single-kernel decode step needs the contiguous cache. Not under tensor parallelism. */
 int elb_model_set_pages(elb_model* m, int page, int n_pages, int type);
 /* Sequence seq[i] goes on from the state of sequence parent[i], for all i at once (a beam search's step, or a shared prefix);
- * the other sequences stay as they are. Full pages are shared, last pages copied (elb_kv_reorder_dev). Paged models only. */
+ * the other sequences stay as they are. Full pages are shared, last pages copied (elb_kv_reorder_dev) into free pages and those that
+ * nobody has afterwards; when there are too few, ELB_ERR_MEMORY and nothing changes. Paged models only. */
 int elb_model_reorder(elb_model* m, int n, const int32_t* seq, const int32_t* parent);
 /* Gives a sequence's pages back: its length is 0. */
 int elb_model_drop(elb_model* m, int seq);

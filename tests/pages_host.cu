@@ -20,6 +20,15 @@ int book_pages(const PageBook* b, int s, int* out) {
 }
 int book_refs(const PageBook* b, int page) { return b->refs[size_t(page)]; }
 void book_drop(PageBook* b, int s) { b->shorten(s, 0); }
+// 1: sequences go on from parent[s], spare[s] is the page of its copy or -1; 0: no pages for the copies
+int book_reorder(PageBook* b, int n_seq, const int* parent, int* spare) {
+    const std::vector<int> from(parent, parent + n_seq);
+    std::vector<int> pages;
+    if (!b->spares(from, b->copies(from), &pages)) return 0;
+    std::copy(pages.begin(), pages.end(), spare);
+    b->reorder(from, pages);
+    return 1;
+}
 // An evaluation of count[s] rows from first[s] on: 1 when it fits. `stop` >= 0: it fails when so many sequences have their pages
 int book_eval(PageBook* b, int n_seq, const int* first, const int* count, int stop) {
     PagedRows rows;

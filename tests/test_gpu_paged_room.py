@@ -99,3 +99,26 @@ def test_a_shared_last_page_is_copied_without_an_allocation(models, full_device)
     got = paged.eval_batch(toks[32:40], [0] * 4 + [1] * 4, list(range(20, 24)) * 2, [0, 0, 0, 1] * 2)
     give_back()
     assert base.rel(got, want) <= base.REL_TOL
+
+
+def test_beams_that_fill_the_pool_go_on_from_one_of_them(models):
+    """No page is free, but the call itself gives up three half-filled ones: they take the copies."""
+    spec, make, flat = models
+    rng = np.random.default_rng(33)
+    paged = make(pages=(16, 5, e.KV_PAIR))
+    toks, own = rng.integers(0, spec.n_vocab, 16), rng.integers(0, spec.n_vocab, (5, 4))
+    base.prompt(paged, 0, toks)
+    paged.reorder([1, 2, 3], [0, 0, 0])
+    for i in range(5):
+        paged.eval_batch(own[i], range(4), [16 + i] * 4)
+    assert paged.free_pages() == 0
+    paged.reorder(range(4), [2, 2, 2, 2])
+    assert paged.free_pages() == 0
+    for s in range(4):
+        base.prompt(flat, s, np.concatenate([toks, own[:, 2]]))
+    for step in range(4):
+        nxt = rng.integers(0, spec.n_vocab, 4)
+        a, b = paged.eval_batch(nxt, range(4), [21 + step] * 4), flat.eval_batch(nxt, range(4), [21 + step] * 4)
+        assert base.rel(a, b) <= base.REL_TOL
+    with pytest.raises(MemoryError):
+        paged.reorder([4], [0])  # this one needs a page more than there are
