@@ -109,6 +109,7 @@ SIGNATURES |= {
     "elb_kv_create": (_i, [_i] * 7 + [_vp, C.POINTER(_vp)]),
     "elb_kv_destroy": (None, [_vp]),
     "elb_kv_memory": (_vp, [_vp]),
+    "elb_selftest_kv_wait_expiry": (_i, [_vp]),
     "elb_kv_append_dev": (_i, [_vp, _i, _kvb, _vp, _vp, _l, _vp, _l, _vp, C.c_float, _vp, _l, _i, _vp, _vp, _l, _vp]),
     "elb_kv_attention_work": (C.c_size_t, [_vp, _kvb, _i]),
     "elb_kv_attention_dev": (_i, [_vp, _i, _kvb, _vp, _l, _i, C.c_float, _vp, _l, _vp, C.c_size_t, _vp]),

@@ -566,6 +566,12 @@ int elb_kv_create(int device, int n_layer, int n_head_kv, int head_dim, int page
     *out = reinterpret_cast<elb_kv*>(kv);
     return ELB_OK;
 }
+int elb_selftest_kv_wait_expiry(elb_kv* kv) {
+    if (!kv) return fail(ELB_ERR_INVALID, "selftest: null argument");
+    DeviceScope on(K(kv)->device);
+    if (on.rc != ELB_OK) return on.rc;
+    return kv_attention_wait_expiry(K(kv));
+}
 void elb_kv_destroy(elb_kv* kv) { kv_destroy(K(kv)); }
 void* elb_kv_memory(const elb_kv* kv) { return kv ? K(kv)->mem : nullptr; }
 int elb_kv_append_dev(elb_kv* kv, int layer, const elb_kv_batch* b, const elb_rope* rope, const float* d_k, int64_t ldk, const float* d_v,

@@ -140,8 +140,16 @@ int kv_create(int device, int n_layer, int n_head_kv, int head_dim, int page, in
     kv->device = device; kv->n_layer = n_layer; kv->HKV = n_head_kv; kv->page = page; kv->n_pages = n_pages; kv->planes = type;
     kv->sm_count = di.sm_count;
     kv->mem = static_cast<__half*>(mem);
+    if (cudaHostAlloc(&kv->err, sizeof(int), cudaHostAllocMapped) != cudaSuccess || cudaHostGetDevicePointer(&kv->err_dev, kv->err, 0) != cudaSuccess) {
+        cudaGetLastError();
+        if (kv->err) cudaFreeHost(kv->err);
+        delete kv;
+        return fail(ELB_ERR_MEMORY, "kv_create: no error word");
+    }
+    *kv->err = 0;
     if (!mem) {
         if (device_malloc(&kv->mem, bytes) != cudaSuccess) {
+            cudaFreeHost(kv->err);
             delete kv;
             return fail(ELB_ERR_MEMORY, "kv_create: out of device memory");
         }
@@ -171,6 +179,7 @@ void kv_destroy(Kv* kv) {
     DeviceScope on(kv->device);
     if (kv->owned) cudaFree(kv->mem);
     else cudaDeviceSynchronize();
+    cudaFreeHost(kv->err);
     delete kv;
 }
 

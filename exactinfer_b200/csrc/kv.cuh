@@ -21,6 +21,7 @@ struct Kv {
     int device = 0, n_layer = 0, HKV = 0, page = 0, n_pages = 0, planes = 1, sm_count = 0;
     __half* mem = nullptr;
     bool owned = false;
+    int *err = nullptr, *err_dev = nullptr;  // pinned word that a kernel raises when one of its bounded waits runs out, and its device address
     CUtensorMap map{};  // the pool as rows of 128 halves, box of 64 halves x min(page, 64) rows, 128-byte swizzle
     int64_t head_halves() const { return int64_t(planes) * page * KV_D; }         // keys or values of one head in a page
     int64_t page_halves() const { return 2 * HKV * head_halves(); }              // one page of one layer
@@ -96,7 +97,8 @@ size_t kv_attention_work(const Kv* kv, const elb_kv_batch* b, int n_head);
 int kv_attention_launch(const Kv* kv, int layer, const elb_kv_batch* b, const float* q, int64_t ldq, int n_head, float scale, float* out,
                         int64_t ldo, void* work, size_t work_bytes, cudaStream_t s);
 int kv_attention_prepare();  // on the current device: what a captured call must find in place
-int kv_attention_check();    // did a kernel of an earlier call give up on a bounded wait?
+int kv_attention_check(const Kv* kv);  // did a kernel of an earlier call on this cache give up on a bounded wait?
+int kv_attention_wait_expiry(const Kv* kv);
 // beam.cu
 size_t beam_select_work(int n_vocab, int n_group, int beams, int k);
 int beam_select_launch(int device, const float* logits, int64_t ld, int n_vocab, int n_group, int beams, const double* scores,

@@ -61,7 +61,7 @@ int kv_attention_launch(const Kv* kv, int layer, const elb_kv_batch* b, const fl
     const AttnWay w = attn_way(b, a.group);
     a.few_max = w.few_max;
     uint8_t* at = static_cast<uint8_t*>(work);
-    ELB_TRY(kv_attention_check());
+    ELB_TRY(kv_attention_check(kv));
     if (w.few) {
         a.part = reinterpret_cast<float*>(at);
         at += up256(kv_attn_few_work(kv, b, n_head, w.few_max));

@@ -67,8 +67,8 @@ __device__ __forceinline__ bool bar_try(uint64_t* b, uint32_t parity) {
     return done != 0;
 }
 // bounded: false when it ran out, or when another warp's wait has
-__device__ __forceinline__ bool bar_wait(uint64_t* b, uint32_t parity, TileBars* bars) {
-    for (unsigned it = 0; it < KT_SPIN; ++it) {
+template <unsigned SPIN = KT_SPIN> __device__ __forceinline__ bool bar_wait(uint64_t* b, uint32_t parity, TileBars* bars) {
+    for (unsigned it = 0; it < SPIN; ++it) {
         if (bar_try(b, parity)) return true;
         if ((it & 1023u) == 1023u && *reinterpret_cast<volatile int*>(&bars->fail)) return false;
     }
@@ -657,14 +657,15 @@ __global__ void __launch_bounds__(KT_THREADS, 1) k_kv_attn_tile(const __grid_con
     if (warp == 9) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(bars->tmem) : "memory");
 }
 
-int* tile_error_word() {  // pinned, mapped: raised by a kernel whose bounded wait ran out
-    static int* host = [] {
-        int* p = nullptr;
-        if (cudaHostAlloc(&p, sizeof(int), cudaHostAllocMapped | cudaHostAllocPortable) != cudaSuccess) return static_cast<int*>(nullptr);
-        *p = 0;
-        return p;
-    }();
-    return host;
+// The bounded wait on a barrier that nobody arrives at, with a short limit: it must give up and raise the error word
+__global__ void k_kv_wait_expiry(int* err) {
+    __shared__ TileBars bars;
+    if (threadIdx.x == 0) {
+        bars.fail = 0;
+        bar_init(&bars.q_full, 1);
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+        if (!bar_wait<1u << 12>(&bars.q_full, 0, &bars) && bars.fail) atomicExch(err, 1);
+    }
 }
 
 struct TilePlan { int64_t tiles; int splits, chunk; };
@@ -698,17 +699,22 @@ TilePlan tile_plan(const Kv* kv, const elb_kv_batch* b, int n_head, int few_max)
 }  // namespace
 
 int kv_attn_tile_prepare() {
-    if (!tile_error_word()) return fail(ELB_ERR_CUDA, "kv_create: no error word");
     ELB_TRY(ensure_dyn_smem(reinterpret_cast<const void*>(k_kv_attn_tile<1>), TileShape<1>::SMEM));
     return ensure_dyn_smem(reinterpret_cast<const void*>(k_kv_attn_tile<2>), TileShape<2>::SMEM);
 }
 
-int kv_attention_check() {
-    int* e = tile_error_word();
-    if (e && *reinterpret_cast<volatile int*>(e)) {
-        *e = 0;
+int kv_attention_check(const Kv* kv) {
+    if (*reinterpret_cast<volatile int*>(kv->err)) {
+        *kv->err = 0;
         return fail(ELB_ERR_CUDA, "kv_attention: a bounded wait ran out in an earlier call");
     }
+    return ELB_OK;
+}
+
+int kv_attention_wait_expiry(const Kv* kv) {  // kv_attention_check() behind a synchronize reports it
+    k_kv_wait_expiry<<<1, 32>>>(kv->err_dev);
+    ELB_CUDA(cudaGetLastError());
+    ELB_CUDA(cudaStreamSynchronize(nullptr));
     return ELB_OK;
 }
 
@@ -719,8 +725,6 @@ size_t kv_attn_tile_work(const Kv* kv, const elb_kv_batch* b, int n_head, int fe
 }
 
 int kv_attn_tile_launch(const Kv* kv, int layer, KvAttnArgs a, const elb_kv_batch* b, cudaStream_t s) {
-    int* err = nullptr;
-    if (cudaHostGetDevicePointer(&err, tile_error_word(), 0) != cudaSuccess) return fail(ELB_ERR_CUDA, "kv_attention: no error word");
     const TilePlan p = tile_plan(kv, b, a.H, a.few_max);
     const int64_t blocks = p.tiles * kv->HKV;
     if (blocks * p.splits > 0x7fffffff || blocks * KT_ROWS / 8 > 0x7fffffff) return fail(ELB_ERR_UNSUPPORTED, "kv_attention: too many rows");
@@ -728,7 +732,7 @@ int kv_attn_tile_launch(const Kv* kv, int layer, KvAttnArgs a, const elb_kv_batc
     a.splits = p.splits; a.chunk = p.chunk; a.tiles_max = int(p.tiles);
     const int64_t layer_rows = kv->layer_halves() / KV_D;
     auto run = [&](auto kernel, int smem) -> int {
-        kernel<<<unsigned(blocks * p.splits), KT_THREADS, smem, s>>>(kv->map, a, int(layer * layer_rows), int(kv->n_layer * layer_rows), err);
+        kernel<<<unsigned(blocks * p.splits), KT_THREADS, smem, s>>>(kv->map, a, int(layer * layer_rows), int(kv->n_layer * layer_rows), kv->err_dev);
         ELB_CUDA(cudaGetLastError());
         return ELB_OK;
     };

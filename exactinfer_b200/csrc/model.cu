@@ -1424,7 +1424,7 @@ static int eval_batch_impl(Model* m, int n, const int32_t* tokens, const int32_t
     ELB_CUDA(cudaStreamSynchronize(m->stream));
     ELB_TRY(gemm_tc_check());
     ELB_TRY(gemm_f16_tc_check());
-    if (m->kv) ELB_TRY(kv_attention_check());
+    if (m->kv) ELB_TRY(kv_attention_check(m->kv));
     paged_rows.book = nullptr;  // they count
     if (out_dev && beam) {
         std::memcpy(beam->score, m->beam_host, picks * sizeof(double));

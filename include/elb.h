@@ -284,7 +284,7 @@ int elb_model_load_gguf_tp(const char* path, int n_ctx, int device, int max_batc
  * memory of the handle's device, and the caller's current device stays as it is. Calls that may overlap need work buffers
  * of their own. Errors that only the device can see (a page number outside the pool, lengths longer than a table) touch no
  * memory outside the given buffers: such a page is not written, and reads as zeros. A wait inside a kernel that runs out of time
- * (all are bounded) makes the next elb_kv_attention_dev call of the process return ELB_ERR_CUDA. */
+ * (all are bounded) makes the next elb_kv_attention_dev call on that cache return ELB_ERR_CUDA, once. */
 
 /* Rotary positions (rope of the reference, src/model.cpp:23-32, with what other checkpoints and longer contexts need). The
  * first `dim` values of a head are rotated in pairs, pair i by the angle pos * f_i in double precision, and multiplied
@@ -327,6 +327,9 @@ size_t elb_kv_bytes(int n_layer, int n_head_kv, int head_dim, int page, int n_pa
 int elb_kv_create(int device, int n_layer, int n_head_kv, int head_dim, int page, int n_pages, int type, void* d_mem, elb_kv** out);
 void elb_kv_destroy(elb_kv* kv); /* waits for the device */
 void* elb_kv_memory(const elb_kv* kv);
+/* Self-test of the failure path, as elb_selftest_wait_expiry: a wait of the attention kernels runs out on this cache. The next
+ * elb_kv_attention_dev call on it, and on no other cache, returns ELB_ERR_CUDA. Nothing faults or hangs. */
+int elb_selftest_kv_wait_expiry(elb_kv* kv);
 
 /* New tokens of several sequences, in device memory. Rows d_q_start[s] .. d_q_start[s + 1] - 1 are the newest tokens of
  * sequence s, which then has d_len[s] positions (the new ones included): its i-th new row is at position

@@ -1,9 +1,10 @@
-"""Handles of the paged cache and of rotary positions: ready for any stream when they are created."""
+"""Handles of the paged cache and of rotary positions: ready for any stream when they are created, errors of their own."""
 import pytest
 import torch
 
 import exactinfer_b200 as e
 import test_gpu_kv as base
+from exactinfer_b200 import capi
 
 pytestmark = pytest.mark.gpu
 D = 128
@@ -53,3 +54,18 @@ def test_working_memory_of_an_empty_batch_and_of_bad_ones():
     for h in (0, -2, 3, 2 * 65):
         assert kv.attention_work(batch(), h) == 0
     assert kv.attention_work(batch(), 2 * 64) > 0
+
+
+@pytest.mark.parametrize("nq", (1, 40))
+def test_a_wait_that_ran_out_is_reported_on_its_own_cache(nq):
+    """The next attention call on that cache is refused, once; another cache's calls go on as if nothing had happened."""
+    a, b = (base.Paged(61 + i, 2, 16, 1, (nq,), (50,)).fill() for i in range(2))
+    qa, qb = base.randn(a.g, nq, 4 * D), base.randn(b.g, nq, 4 * D)
+    want = a.attention(4, qa), b.attention(4, qb)
+    for _ in range(2):
+        assert capi.lib().elb_selftest_kv_wait_expiry(a.kv._h) == capi.OK
+        assert torch.equal(b.attention(4, qb), want[1])
+        with pytest.raises(e.ElbError, match="wait"):
+            a.attention(4, qa)
+        assert torch.equal(a.attention(4, qa), want[0])
+    assert capi.lib().elb_selftest_kv_wait_expiry(None) == capi.ERR_INVALID
