@@ -1171,7 +1171,7 @@ int model_finalize(Model* m) {
 }
 
 namespace { struct TopOut; }
-static int paged_eval(Model* m, const int32_t* tokens, int n, int pos0, float* logits, const TopOut* top);
+static int paged_eval(Model* m, const int32_t* tokens, int n, int pos0, float* logits, const TopOut* top, bool head = false);
 int model_eval_impl(Model* m, const int32_t* tokens, int n, int pos0, float* logits, const TopOut* top);
 
 int model_eval_top(Model* m, const int32_t* tokens, int n, int pos0, int k, int32_t* ids, float* vals, double* lse,
@@ -1212,8 +1212,9 @@ namespace {
 struct TopRows { int k; int32_t* ids; float* vals; double* lse; const uint32_t* allowed = nullptr; };  // allowed: one row wanted
 struct BeamRows { int groups, beams, k; const double* scores; int32_t *parent, *token; double* score; };
 }
+// head: the wanted rows' logits are formed even when nobody takes them (they stay on the device)
 static int eval_batch_impl(Model* m, int n, const int32_t* tokens, const int32_t* seq, const int32_t* pos, const uint8_t* want,
-                           float* logits, const TopRows* top, const BeamRows* beam = nullptr);
+                           float* logits, const TopRows* top, const BeamRows* beam = nullptr, bool head = false);
 
 int model_eval_batch(Model* m, int n, const int32_t* tokens, const int32_t* seq, const int32_t* pos, const uint8_t* want,
                      float* logits) {
@@ -1321,7 +1322,7 @@ static int paged_batch(Model* m, int n, const int32_t* seq, const int32_t* pos, 
 }
 
 static int eval_batch_impl(Model* m, int n, const int32_t* tokens, const int32_t* seq, const int32_t* pos, const uint8_t* want,
-                           float* logits, const TopRows* top, const BeamRows* beam) {
+                           float* logits, const TopRows* top, const BeamRows* beam, bool head) {
     if (!m || !tokens || !seq || !pos) return fail(ELB_ERR_INVALID, "eval_batch: null argument");
     if (!m->finalized) return fail(ELB_ERR_STATE, "eval_batch: model not finalized");
     if (n <= 0) return fail(ELB_ERR_INVALID, "eval_batch: empty batch");
@@ -1333,7 +1334,7 @@ static int eval_batch_impl(Model* m, int n, const int32_t* tokens, const int32_t
         if (seq[i] < 0 || seq[i] >= m->n_seq) return fail(ELB_ERR_RANGE, "eval_batch: sequence index out of range");
         if (pos[i] < 0 || pos[i] >= m->n_ctx) return fail(ELB_ERR_RANGE, "eval_batch: context window full");
         uniform = uniform && seq[i] == seq[0] && pos[i] == pos[0] + i;
-        if ((logits || top || beam) && (!want || want[i])) rows.push_back(i);
+        if ((logits || top || beam || head) && (!want || want[i])) rows.push_back(i);
     }
     for (int i = 0; i < n; ++i)  // rows of one sequence: increasing, consecutive positions
         for (int j = i + 1; j < n; ++j)
@@ -1420,7 +1421,7 @@ static int eval_batch_impl(Model* m, int n, const int32_t* tokens, const int32_t
     ELB_CUDA(cudaEventRecord(m->ev1, m->stream));
     if (out_dev && top) ELB_CUDA(cudaMemcpyAsync(m->top_rows_host, m->top_rows_dev, rows.size() * TOP_BYTES, cudaMemcpyDeviceToHost, m->stream));
     else if (out_dev && beam) ELB_CUDA(cudaMemcpyAsync(m->beam_host, beam_scores + rows.size(), picks * 16, cudaMemcpyDeviceToHost, m->stream));
-    else if (out_dev) ELB_CUDA(cudaMemcpyAsync(logits, out_dev, rows.size() * size_t(V) * sizeof(float), cudaMemcpyDeviceToHost, m->stream));
+    else if (out_dev && logits) ELB_CUDA(cudaMemcpyAsync(logits, out_dev, rows.size() * size_t(V) * sizeof(float), cudaMemcpyDeviceToHost, m->stream));
     ELB_CUDA(cudaStreamSynchronize(m->stream));
     ELB_TRY(gemm_tc_check());
     ELB_TRY(gemm_f16_tc_check());
@@ -1444,7 +1445,7 @@ static int eval_batch_impl(Model* m, int n, const int32_t* tokens, const int32_t
 }
 
 // model_eval over the paged cache: chunks of rows of sequence 0, when there are pages and memory for all of them
-static int paged_eval(Model* m, const int32_t* tokens, int n, int pos0, float* logits, const TopOut* top) {
+static int paged_eval(Model* m, const int32_t* tokens, int n, int pos0, float* logits, const TopOut* top, bool head) {
     ELB_TRY(paged_room(m, 0, pos0, n));
     for (int done = 0; done < n; done += m->max_batch) {
         const int b = std::min(m->max_batch, n - done);
@@ -1461,7 +1462,8 @@ static int paged_eval(Model* m, const int32_t* tokens, int n, int pos0, float* l
         want.back() = 1;
         TopRows rows{};
         if (top) { rows.k = top->k; rows.ids = top->ids; rows.vals = top->vals; rows.lse = top->lse; rows.allowed = top->allowed; }
-        ELB_TRY(eval_batch_impl(m, b, tokens + done, seq.data(), pos.data(), want.data(), last ? logits : nullptr, last && top ? &rows : nullptr));
+        ELB_TRY(eval_batch_impl(m, b, tokens + done, seq.data(), pos.data(), want.data(), last ? logits : nullptr, last && top ? &rows : nullptr, nullptr,
+                                last && head));
         ms += m->last_ms;
         launches += m->last_launches;
         done += b;
@@ -1566,7 +1568,7 @@ int model_eval_steps(Model* m, const int32_t* tokens, int n, int pos0, float* de
         float ms = 0.f;
         int64_t launches = 0;
         for (int i = 0; i < n; ++i) {
-            ELB_TRY(paged_eval(m, tokens + i, 1, pos0 + i, nullptr, nullptr));
+            ELB_TRY(paged_eval(m, tokens + i, 1, pos0 + i, nullptr, nullptr, true));
             ms += m->last_ms;
             launches += m->last_launches;
         }

@@ -233,7 +233,8 @@ int elb_model_free_pages(const elb_model* m, int* n);
 
 /* n single-token steps at positions pos0.., enqueued back to back without reading logits back (the tg loop of the
  * reference's bench command, src/main.cpp:639, without its per-token host round trip). device_ms receives the device
- * time of the whole run (CUDA events on the model's stream). Same argument checks as elb_model_eval. */
+ * time of the whole run (CUDA events on the model's stream; of a paged model, whose steps wait for the host, the sum of the steps'). Same
+ * argument checks as elb_model_eval. */
 int elb_model_eval_steps(elb_model* m, const int32_t* tokens, int n, int pos0, float* device_ms);
 
 /* Same step, measured: device time in milliseconds of the last elb_model_eval (CUDA events on the model's own

@@ -1,4 +1,4 @@
-"""A paged model that lacks pages or device memory: the call is refused and leaves every sequence as it was."""
+"""A paged model that lacks pages or device memory: the call is refused and leaves every sequence as it was. Its decode loop."""
 import ctypes as C
 
 import numpy as np
@@ -122,3 +122,17 @@ def test_beams_that_fill_the_pool_go_on_from_one_of_them(models):
         assert base.rel(a, b) <= base.REL_TOL
     with pytest.raises(MemoryError):
         paged.reorder([4], [0])  # this one needs a page more than there are
+
+
+def test_steps_form_their_logits(models):
+    """eval_steps is a decode loop without reading back: every step is all of a step, the output head as well."""
+    spec, make, flat = models
+    rng = np.random.default_rng(34)
+    toks = rng.integers(0, spec.n_vocab, 12)
+    for model in (make(pages=(16, 8, e.KV_PAIR)), flat):
+        model.eval(toks[:5], 0)
+        model.eval(toks[5:6], 5)
+        one = model.last_eval_stats()[1]
+        model.eval_steps(toks[6:9], 6)
+        ms, launches = model.last_eval_stats()
+        assert launches == 3 * one and ms > 0
