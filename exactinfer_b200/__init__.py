@@ -6,6 +6,7 @@
 from __future__ import annotations
 
 import ctypes as C
+import operator
 import os
 
 import numpy as np
@@ -148,13 +149,17 @@ def split_limbs(x: np.ndarray, nl: int, device: int = 0):
 # ---- the paged cache, rotary positions and beam selection (device pointers, stream-ordered: see include/elb.h)
 
 def _ptr(x):
-    """Device address of x: a number, a DeviceBuffer, anything with data_ptr() (a torch tensor, say) or None."""
+    """Device address of x: a whole number, a DeviceBuffer, anything with data_ptr() (a torch tensor, say) or None. Arrays and tensors in
+    pageable host memory are refused: a kernel that read there would fault."""
     if x is None or type(x) is int:
         return x
     try:  # (a decoding step makes a few of these calls per layer: every microsecond of them counts)
-        return x.data_ptr()
+        p = x.data_ptr()
     except AttributeError:
-        return x.ptr if isinstance(x, DeviceBuffer) else int(x)
+        return x.ptr if isinstance(x, DeviceBuffer) else operator.index(x)
+    if not getattr(x, "is_cuda", True) and not x.is_pinned():
+        raise ValueError("a tensor in host memory was given where device memory is needed")
+    return p
 
 
 ROPE_HALF, ROPE_INTERLEAVED = 0, 1
