@@ -97,3 +97,17 @@ def test_zeros_of_both_signs_are_equal_logits(v, masked):
     for k in (1, 2, 40):
         if k <= 2 * v:
             base.agree(base.select(x, scores, 2, 2, k, allowed), base.selected(x, scores, 2, 2, k, allowed), v)
+
+
+@pytest.mark.parametrize("v", (2, 3, 5, 17, 64))
+@pytest.mark.parametrize("size", (0.5, 3.0, 40.0))
+def test_scores_of_small_vocabularies(v, size):
+    """Few terms in a sum: every exponential counts with its own error, 11 * 2^-52 at most, and the additions with n 2^-53 on either side.
+    Then each side rounds, by 2^-53 of the number: log-sum-exp (at most max |x| + ln v), logit less it (at most |want| + |score|) and the
+    score (|want|); the scores are below 4, ln v below 5."""
+    g = base.gen(53)
+    x = base.randn(g, 2000, v) * size
+    scores = torch.randn(2000, generator=g, device="cuda", dtype=F64)
+    got, want = base.select(x, scores, 500, 4, 4), base.selected(x, scores, 500, 4, 4)
+    assert (got[0] == want[0]).all() and (got[1] == want[1]).all()
+    assert (abs(got[2] - want[2]) <= (11 + v + 8 + float(x.abs().max()) + 9 + 2 * abs(want[2])) * 2.0 ** -52).all()
