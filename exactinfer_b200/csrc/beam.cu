@@ -11,7 +11,7 @@
 // Exponentials are the work beside the loads: double precision, e^y = 2^(i/64) 2^n e^r with y = (64 n + i) ln 2 / 64 + r, |r| <= a =
 // ln 2 / 128, and the Taylor sum of e^r to the fifth power, whose last term is put into the lower ones by its Chebyshev expansion: r^5 =
 // 5/4 a^2 r^3 - 5/16 a^4 r but for a^5 / 16 (e^r is 2.5e-15 off at most; the sum to r^4 / 24 by itself 4e-14), nine double operations a logit. 64 rows of 151936 logits
-// in 16 groups under masks: 26.5 us, 17 of them k_beam_segments (65 % of the issue slots; bytes alone 6); one group of 4 rows 12 us,
+// in 16 groups under masks: 26.5 us, 17 of them k_beam_segments (65 % of the issue slots, 38 % of the fp64 pipe; bytes alone 6); one group of 4 rows 12 us,
 // the length of the two kernels' chains.
 #include <algorithm>
 #include <cmath>

@@ -16,7 +16,7 @@ constexpr int KR_THREADS = 256, KR_MAXROWS = 4096, KR_CHUNK = 16384;  // KR_CHUN
 // Row r goes on from row parent[r]. Its first child keeps a last page that is not full, every other child gets a copy in
 // its spare page. The copies of all layers are cut into pieces of 16 KB and dealt out evenly over the blocks; every block
 // works out the list of copies for itself (n words of shared memory: cheaper than a launch before this one). Bound by memory: bytes
-// of the copied pages, read and written once (64 rows, 12 layers, 119 MB: 22 us, 5.4 TB/s).
+// of the copied pages, read and written once (64 rows, 12 layers, 119 MB: 23 us, 5.2 TB/s).
 __global__ void __launch_bounds__(KR_THREADS) k_kv_reorder(uint8_t* __restrict__ pool, int64_t layer_bytes, int64_t page_bytes, int n_layer,
                                                            int n_pages, int page, int n, const int* __restrict__ parent,
                                                            const int* __restrict__ len, const int* __restrict__ table, int64_t table_ld,

@@ -5,14 +5,14 @@
 // CTA of four warps takes a range of the keys; a warp walks every fourth step of 16 keys on its own, with its own running
 // maximum and sum (in fp32), its next steps on their way by cp.async into its own ring, and meets the others once at
 // the end. A step is S^T = K q^T and O^T += V^T P^T on mma.sync m16n8k16: the keys and values are the 16-row operand, 8
-// query rows the narrow one, so that the one to eight rows of a decode step waste nothing. (The tensor pipe is a tenth busy: tcgen05 with
-// its 128 rows would leave 120 of them empty.) 64 tokens behind 100-8000 keys, 32 heads on 8, F16: 190 us, 6.4 TB/s; one behind
-// 100003 keys, pairs: 129 us, 6.3 TB/s; one behind 41 keys 4.3 us.
+// query rows the narrow one, so that the one to eight rows of a decode step waste nothing. (The tensor pipe is a fifth busy: tcgen05 with
+// its 128 rows would leave 120 of them empty.) 64 tokens behind 100-8000 keys, 32 heads on 8, F16: 193 us, 6.3 TB/s; one behind
+// 100003 keys, pairs: 131 us, 6.3 TB/s; one behind 41 keys 4.4 us.
 //
 // fp32 accuracy from fp16 operands: a query row is scaled by a power of two and held as hi + lo (22 bits), so are the
 // weights; keys and values are what the cache holds, one fp16 or a pair. Products hi hi, hi lo, lo hi are exact, lo lo
-// (2^-22) is left out. The tensor core adds with truncation: every chain is at most 8 products long and joins an fp32 sum with
-// rounding (a step's O^T starts from zero).
+// (2^-22) is left out. The tensor core adds with truncation: hi hi of a score is two chains of 4 MMAs, the small products one of 8 (of 16 with
+// pairs, 2^-11 of the score together), a step's O^T one of 2 or 3 that starts from zero; what a chain ends in joins fp32 sums with rounding.
 #include <algorithm>
 
 #include "kv_attn.cuh"

@@ -18,12 +18,13 @@
 // [key][dimension] as in the page and is a B operand with N along the rows.
 // A tile's 128 keys take 2048 (F16) or 3 * 1024 (pairs) clocks of the tensor pipe. (64-key tiles: an MMA with N = 64 took 51
 // clocks instead of 32, and the whole 1860 a tile.) What bounds it is the chain S, weights, O, sums of a tile with one O: the
-// tensor pipe is 54 % busy. 4096 causal rows, 32 query heads on 8: F16 260 us (528 TFLOP/s of useful products, 1056 of both
-// halves), pairs 330 us. (Four teams' warps with half a row a thread: 277 us.)
+// tensor pipe is 54 to 59 % busy. 4096 causal rows, 32 query heads on 8: F16 257 us (535 TFLOP/s of useful products, 1070 of both
+// halves), pairs 348 us (335 to 365 with the clock under the power cap). (Four teams' warps with half a row a thread: 277 us.)
 //
 // Behind the last visible key the weights are 0, but 0 * NaN is not: the PV product stops at the last 16 keys, and the rows of
 // V behind the last key are emptied in shared memory. In the few tiles that only some rows see, V is searched for infinities and
-// NaN; where there are any, the tile's product is done by the threads, key by key, for the rows that see it.
+// NaN; where there are any, the tile's product is done by the threads, key by key, for the rows that see it. Infinite values that a row does
+// see are left to its end: where a result is NaN, they are added up by themselves (kv_not_finite).
 #include <algorithm>
 
 #include "kv_attn.cuh"
@@ -180,7 +181,7 @@ __device__ __forceinline__ float max3(float a, float b, float c) {
     return r;
 }
 
-// A row's scores of one key tile in tensor memory (64 columns from sp) -> weights in their place, per 16 keys 8 columns of hi and 8
+// A row's scores of one key tile in tensor memory (128 columns from sp) -> weights in their place, per 16 keys 8 columns of hi and 8
 // of lo; running maximum m and denominator l. Returns what earlier sums are to be multiplied by. EDGE: only the first
 // `left` keys are seen. The loops stay rolled: straight-line code that a warp runs once per tile comes in at the
 // speed of instruction fetch (unrolled, with both forms in one body, this took 3000 clocks a tile).

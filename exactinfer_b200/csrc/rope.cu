@@ -7,7 +7,7 @@
 // values (a "unit": 4 pairs, or 8 values that are kept) as two 16-byte quads. Angles are formed in turns, t = pos * (f / 2 pi) and
 // the fraction of t, so that no position needs more than one double-precision product and a sine of at most one turn.
 // 4096 rows of 32 heads of 128, interleaved: 23.5 us, 5.7 TB/s (26.7 with a thread's eight values side by side: every load and
-// store touched half of its sectors). Append of 2048 tokens, 32 + 8 + 8 heads, pairs: 37.5 us, 4.3 TB/s: one wave of blocks, whose first
+// store touched half of its sectors). Append of 2048 tokens, 64 + 8 + 8 heads, F16: 37.2 us, 4.3 TB/s: one wave of blocks, whose first
 // loads wait beside the search for their tokens and the angles.
 #include <algorithm>
 #include <cmath>
