@@ -76,6 +76,21 @@ struct DeviceScope {
     }
 };
 
+// Do n rows of wx floats, ldx apart from x on, share memory with n rows of wy floats, ldy apart from y on? Columns of one buffer (equal
+// strides) are told apart; with unequal strides ranges that interleave count as apart.
+inline bool rows_meet(const float* x, int64_t ldx, int64_t wx, const float* y, int64_t ldy, int64_t wy, int64_t n) {
+    using Wide = __int128;
+    const Wide ux = Wide(reinterpret_cast<uintptr_t>(x)), uy = Wide(reinterpret_cast<uintptr_t>(y));
+    if (ux + (Wide(n - 1) * ldx + wx) * 4 <= uy || uy + (Wide(n - 1) * ldy + wy) * 4 <= ux) return false;
+    if (n == 1) return true;
+    if (ldx != ldy) return false;
+    const Wide row = Wide(ldx) * 4;
+    Wide r = (uy - ux) % row;
+    if (r < 0) r += row;
+    const Wide k = (uy - ux - r) / row;  // row j of y starts r bytes behind the start of row k + j of x, row - r in front of the next one's
+    return (r < wx * 4 && k < n && -k < n) || (row - r < wy * 4 && k + 1 < n && -k - 1 < n);
+}
+
 // rope.cu
 int rope_frequencies(const elb_rope_config* c, std::vector<double>* freq, double* m);
 int rope_create(int device, const elb_rope_config* c, Rope** out);

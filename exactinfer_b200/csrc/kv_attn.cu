@@ -48,6 +48,7 @@ int kv_attention_launch(const Kv* kv, int layer, const elb_kv_batch* b, const fl
     if (ldq < int64_t(n_head) * KV_D || ldo < int64_t(n_head) * KV_D) return fail(ELB_ERR_INVALID, "kv_attention: a row stride is shorter than the row");
     if (reinterpret_cast<uintptr_t>(q) % 16 || reinterpret_cast<uintptr_t>(out) % 16 || ldq % 4 || ldo % 4)
         return fail(ELB_ERR_UNSUPPORTED, "kv_attention: rows must start on 16-byte boundaries");
+    if (rows_meet(q, ldq, int64_t(n_head) * KV_D, out, ldo, int64_t(n_head) * KV_D, b->n_tok)) return fail(ELB_ERR_INVALID, "kv_attention: the output must not overlap the queries");
     if (!work || work_bytes < kv_attention_work(kv, b, n_head)) return fail(ELB_ERR_INVALID, "kv_attention: the work buffer is too small");
     if (reinterpret_cast<uintptr_t>(work) % 256) return fail(ELB_ERR_INVALID, "kv_attention: the work buffer must start on a 256-byte boundary");
     DeviceScope on(kv->device);

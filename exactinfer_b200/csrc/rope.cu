@@ -392,6 +392,7 @@ int rope_launch(const Rope* r, const float* x, int64_t ldx, float* y, int64_t ld
     const int64_t width = int64_t(heads) * r->head_dim;
     if (ldx < width || ldy < width) return fail(ELB_ERR_INVALID, "rope: a row stride is shorter than the row");
     if (x == y && ldx != ldy) return fail(ELB_ERR_INVALID, "rope: in place needs equal strides");
+    if (x != y && rows_meet(x, ldx, width, y, ldy, width, n)) return fail(ELB_ERR_INVALID, "rope: the result must not overlap the input, or must be in its place");
     if (n > 0x7fffffff) return fail(ELB_ERR_UNSUPPORTED, "rope: too many rows");
     if (norm && !(eps >= 0.f)) return fail(ELB_ERR_INVALID, "rope: eps must not be negative");
     DeviceScope on(r->device);
@@ -425,6 +426,10 @@ int kv_append_launch(Kv* kv, int layer, const elb_kv_batch* b, const Rope* rope,
     if (rope && (rope->head_dim != KV_D || rope->device != kv->device)) return fail(ELB_ERR_INVALID, "kv_append: the positions are for another head_dim or device");
     if (rope && rope->dim % 8) return fail(ELB_ERR_UNSUPPORTED, "kv_append: the rotated part of a head must be a multiple of 8");
     if (b->n_tok == 0 || b->n_seq == 0) return ELB_OK;
+    const int64_t qd = int64_t(n_head) * KV_D;
+    if (q && ((q != q_out && rows_meet(q, ldq, qd, q_out, ldqo, qd, b->n_tok)) || rows_meet(k, ldk, kd, q_out, ldqo, qd, b->n_tok) ||
+              rows_meet(v, ldv, kd, q_out, ldqo, qd, b->n_tok)))
+        return fail(ELB_ERR_INVALID, "kv_append: the rotated queries must not overlap the inputs, or must be in the queries' place");
     DeviceScope on(kv->device);
     if (on.rc != ELB_OK) return on.rc;
     RopeArgs a{};

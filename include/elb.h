@@ -345,7 +345,7 @@ typedef struct {
 } elb_kv_batch;
 
 /* Keys and values of the new tokens into their pages of one layer: k = rotation(norm(k)), v as it is; with d_q also
- * q_out = rotation(norm(q)) for n_head query heads (q_out may be q with the same stride). rope NULL: no rotation. d_k_norm,
+ * q_out = rotation(norm(q)) for n_head query heads (q_out may be q with the same stride, and must not overlap the inputs otherwise). rope NULL: no rotation. d_k_norm,
  * d_q_norm: [128] weights of the per-head RMSNorm or NULL. Row strides in floats; every row, and the weights, start on a
  * 16-byte boundary.
  * Rows that belong to nothing are left as they are, and so is their q_out. Two rows must not share a position. */

@@ -1,4 +1,5 @@
-"""Handles of the paged cache and of rotary positions: ready for any stream when they are created, errors of their own."""
+"""Handles of the paged cache and of rotary positions: ready for any stream when they are created, errors of their own, what their calls
+refuse."""
 import pytest
 import torch
 
@@ -69,3 +70,40 @@ def test_a_wait_that_ran_out_is_reported_on_its_own_cache(nq):
             a.attention(4, qa)
         assert torch.equal(a.attention(4, qa), want[0])
     assert capi.lib().elb_selftest_kv_wait_expiry(None) == capi.ERR_INVALID
+
+
+def test_results_that_overlap_what_they_are_made_from_are_refused():
+    """Shared memory in any row, whatever the distance; columns of one buffer and neighbouring buffers are told apart from it."""
+    buf = base.randn(base.gen(64), 40, 12 * D)
+    at = lambda floats: buf.data_ptr() + 4 * floats
+    ld, n = 12 * D, 8
+    t = lambda *v: torch.tensor(v, dtype=torch.int32, device="cuda")
+    rope, pos, kv = e.Rope(D), torch.arange(n, device="cuda", dtype=torch.int32), e.KvCache(1, 2, 16, 4)
+    b = e.KvBatch(1, n, n, n, t(0, n), t(n), t(0, 1), 2)
+    work = torch.empty(kv.attention_work(b, 4), dtype=torch.uint8, device="cuda")
+    turn = lambda x, y, ldx=ld, ldy=ld, rows=n: rope.apply(at(x), pos, at(y), rows, 4, ldx=ldx, ldy=ldy)
+    attend = lambda x, y, ldx=ld, ldy=ld: kv.attention(0, b, at(x), at(y), 4, 0.1, work, work.numel(), ldq=ldx, ldo=ldy)
+    append = lambda q, out, k, v, ldo=ld: kv.append(0, b, at(k), at(v), ld, ld, q=at(q), ldq=ld, n_head=4, q_out=at(out), ldqo=ldo)
+    apart = [(0, 4 * D), (4 * D, 0), (8 * D, 0), (0, 7 * ld + 4 * D), (0, 8 * ld), (8 * ld, 0), (5 * ld + 4 * D, 0)]  # (4 heads are 4 D floats)
+    for x, y in apart:
+        turn(x, y)
+        attend(x, y)
+    meet = [(0, D), (D, 0), (0, 4), (0, 4 * D - 4), (0, 7 * ld), (7 * ld + 3 * D, 0), (2 * ld, ld + 9 * D), (ld + 9 * D, 0), (0, 3 * ld - 2 * D)]
+    for x, y in meet:
+        with pytest.raises(ValueError, match="overlap"):
+            turn(x, y)
+        with pytest.raises(ValueError, match="overlap"):
+            attend(x, y)
+        with pytest.raises(ValueError, match="overlap"):
+            append(x, y, 16 * ld, 24 * ld)
+        for k, v in ((y + 2 * D, 16 * ld), (16 * ld, y + D)):  # (keys and values are 2 D floats)
+            with pytest.raises(ValueError, match="overlap"):
+                append(30 * ld, y, k, v)
+    with pytest.raises(ValueError, match="overlap"):
+        attend(0, 0)
+    with pytest.raises(ValueError, match="overlap"):
+        turn(0, 2 * D, ldx=ld, ldy=4 * D, rows=1)
+    turn(0, 0)
+    append(0, 0, 4 * D, 6 * D)
+    append(0, 8 * D, 4 * D, 6 * D)
+    torch.cuda.synchronize()
